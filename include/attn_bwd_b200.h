@@ -130,6 +130,77 @@ int attn_bwd_b200_host(const void* grad_attn_output_h, const void* attn_weights_
                        uint8_t* dropout_mask_d, void* grad_attn_scores_d, void* grad_value_states_d, int chunks,
                        attn_bwd_stream_t stream);
 
+/* ---- Operators around the attention backward -------------------------------------------
+ * Rotary positions and attention without materialised weights (no reference counterpart:
+ * the reference starts from given attn_weights).  All pointers are device pointers, all
+ * calls are asynchronous on `stream` and allocate nothing. */
+
+/* element types */
+enum { ATTN_BWD_DT_BF16 = 0, ATTN_BWD_DT_FP16 = 1, ATTN_BWD_DT_FP32 = 2 };
+
+/* Rotary positions.  x[.., 0:rotary_dim] of every head is rotated pair by pair,
+ *   (a, b) -> factor * (a cos t - b sin t, b cos t + a sin t),   t = 2 pi position * turns / 2^64,
+ * pair n being (n, n + rotary_dim/2), or (2n, 2n+1) with `interleaved`; the rest of the head
+ * is copied.  `inverse` negates t: with the same factor that is the gradient of the call.
+ * turns[n] is the frequency as a 64-bit fixed-point fraction of a turn (two's complement), so
+ * position * turns wraps exactly and far positions lose nothing.  Strides are in elements,
+ * in the order batch, head, position; the head's own elements are contiguous.  An output may
+ * be its own input (same strides).  position_stride is the positions' batch stride (0: one
+ * row for all batches); positions are int64. */
+typedef struct {
+  int bs, seq, q_heads, k_heads, head_dim, rotary_dim; /* q_heads or k_heads may be 0 */
+  int dtype;                                           /* ATTN_BWD_DT_* */
+  int interleaved, inverse;
+  float factor;
+  int64_t position_stride;
+  int64_t q_in[3], k_in[3], q_out[3], k_out[3];
+} attn_bwd_rope_t;
+
+int attn_bwd_b200_rope(const attn_bwd_rope_t* args, const void* q, const void* k, const int64_t* positions,
+                       const int64_t* turns, void* q_out, void* k_out, attn_bwd_stream_t stream);
+
+/* Attention with modified scores.  For head h of a query at position i (i = its row +
+ * seq_kv - seq_q: the queries are the last seq_q positions) and key j:
+ *   x = scale * q.k,  s = softcap > 0 ? softcap * tanh(x / softcap) : x,  s -= slopes[h] * |i - j|
+ * j is seen if  (!causal || j < max(i + 1, prefix_lens[b]))  and, with documents,
+ * q_documents[b, row] == kv_documents[b, j] >= 0.  A row that sees nothing has output 0, row
+ * statistic -inf and gradient 0.  Keys and queries whose document is negative are never read
+ * into a result, whatever they hold.  slopes, prefix_lens and documents may be null;
+ * prefix_lens needs causal; both document arrays or neither.
+ *   q [bs, heads, seq_q, head_dim], k and v [bs, kv_heads, seq_kv, head_dim]: strides in
+ *     elements in the order batch, head, position (positive multiples of 8, head elements
+ *     contiguous, 16-byte aligned), heads a multiple of kv_heads, head_dim 64 or 128
+ *   o [bs, seq_q, heads, head_dim] contiguous; lse [bs, heads, seq_q] fp32 (natural log)
+ *   dq, dk, dv: shaped as q, k, v, strides in dq_stride / dk_stride / dv_stride
+ * workspace: at least attn_bwd_b200_fused_workspace() bytes, 256-byte aligned, private to the call until
+ * the stream has finished it (two graphs that may run at once need one each). */
+typedef struct {
+  int bs, seq_q, seq_kv, heads, kv_heads, head_dim;
+  int dtype; /* ATTN_BWD_DT_BF16 or ATTN_BWD_DT_FP16 */
+  int causal;
+  float scale;   /* > 0 */
+  float softcap; /* 0: none */
+  const float* slopes;         /* [heads] */
+  const int32_t* prefix_lens;  /* [bs] */
+  const int32_t* q_documents;  /* [bs, seq_q] */
+  const int32_t* kv_documents; /* [bs, seq_kv] */
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int64_t dq_stride[3], dk_stride[3], dv_stride[3]; /* backward only */
+} attn_bwd_fused_t;
+
+/* Bytes of workspace that the forward (backward = 0) or backward (1) call needs on the
+ * current device, or a negative ATTN_BWD_E* code. */
+int64_t attn_bwd_b200_fused_workspace(const attn_bwd_fused_t* args, int backward);
+
+int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* args, const void* q, const void* k, const void* v, void* o,
+                            float* lse, void* workspace, int64_t workspace_bytes, attn_bwd_stream_t stream);
+
+/* Gradients of the call above, from its o and lse.  Sums over the heads of a group and over
+ * rows are taken in a fixed order: equal inputs give equal bits. */
+int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* args, const void* grad_o, const void* q, const void* k,
+                            const void* v, const void* o, const float* lse, void* dq, void* dk, void* dv,
+                            void* workspace, int64_t workspace_bytes, attn_bwd_stream_t stream);
+
 /* Synchronises the current device, returns the code a kernel's bounded wait
  * recorded since the last poll (0 if none) and clears it.  The reference's
  * evaluator has no counterpart; it reports exceptions (eval_modal_attn_bwd.py:294-302). */

@@ -12,6 +12,8 @@ import torch
 
 from . import _lib
 from ._lib import AttnBwdError
+from .fused import fused_attn_bwd, fused_attn_fwd
+from .rope import RopeTable, rope_bwd, rope_fwd, rope_table
 
 NUM_ATTENTION_HEADS = 80
 NUM_KEY_VALUE_HEADS = 8
@@ -19,8 +21,8 @@ NUM_GROUPS = NUM_ATTENTION_HEADS // NUM_KEY_VALUE_HEADS
 HEAD_DIM = 128
 
 __all__ = ["custom_kernel", "attn_bwd", "attn_bwd_shard", "attn_bwd_host", "ds_shard", "dv_shard", "run",
-           "AttnBwdError", "poll_error", "release", "options", "attn_bwd_from_mask", "NUM_ATTENTION_HEADS", "NUM_KEY_VALUE_HEADS",
-           "HEAD_DIM"]
+           "AttnBwdError", "poll_error", "release", "options", "attn_bwd_from_mask", "rope_table", "rope_fwd", "rope_bwd",
+           "RopeTable", "fused_attn_fwd", "fused_attn_bwd", "NUM_ATTENTION_HEADS", "NUM_KEY_VALUE_HEADS", "HEAD_DIM"]
 
 
 def _ptr(t):

@@ -14,8 +14,30 @@ LIB_PATH = os.environ.get("ATTN_BWD_B200_LIB") or os.path.join(os.path.dirname(o
 # C-ABI error codes (enum in include/attn_bwd_b200.h)
 OK, EINVAL, EALIGN, EUNSUPPORTED, ETMAP, ECUDA, EDEVICE, EKERNEL = range(8)
 
+_VP, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
+_L3 = ctypes.c_int64 * 3
+
+DT_BF16, DT_FP16, DT_FP32 = range(3)   # ATTN_BWD_DT_*
+
+
+class RopeArgs(ctypes.Structure):
+    """attn_bwd_rope_t"""
+    _fields_ = [(n, _I) for n in ("bs", "seq", "q_heads", "k_heads", "head_dim", "rotary_dim", "dtype", "interleaved",
+                                  "inverse")] + [
+        ("factor", _F), ("position_stride", _L), ("q_in", _L3), ("k_in", _L3), ("q_out", _L3), ("k_out", _L3)]
+
+
+class FusedArgs(ctypes.Structure):
+    """attn_bwd_fused_t"""
+    _fields_ = [(n, _I) for n in ("bs", "seq_q", "seq_kv", "heads", "kv_heads", "head_dim", "dtype", "causal")] + [
+        ("scale", _F), ("softcap", _F)] + [
+        (n, _VP) for n in ("slopes", "prefix_lens", "q_documents", "kv_documents")] + [
+        (n, _L3) for n in ("q_stride", "k_stride", "v_stride", "dq_stride", "dk_stride", "dv_stride")]
+
+
+_ROPE_P, _FUSED_P = ctypes.POINTER(RopeArgs), ctypes.POINTER(FusedArgs)
+
 # Every symbol the header declares, with its ctypes signature.
-_VP, _I, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
 SIGNATURES = {
     "attn_bwd_b200": (_I, [_VP, _VP, _VP, _VP, _VP, _F, _I, _I, _I, _VP, _VP, _VP]),
     "attn_bwd_b200_shard": (_I, [_VP, _VP, _VP, _VP, _VP, _F, _I, _I, _I, _I, _I, _VP, _VP, _VP]),
@@ -24,6 +46,10 @@ SIGNATURES = {
     "attn_bwd_b200_shard_from_mask": (_I, [_VP, _VP, _VP, _VP, _F, _I, _I, _I, _I, _I, _VP, _VP, _VP]),
     "attn_bwd_b200_host_shard": (_I, [_VP] * 5 + [_F, _I, _I, _I, _I, _I] + [_VP] * 9 + [_I, _VP]),
     "attn_bwd_b200_host": (_I, [_VP] * 5 + [_F, _I, _I, _I] + [_VP] * 9 + [_I, _VP]),
+    "attn_bwd_b200_rope": (_I, [_ROPE_P] + [_VP] * 7),
+    "attn_bwd_b200_fused_workspace": (_L, [_FUSED_P, _I]),
+    "attn_bwd_b200_fused_fwd": (_I, [_FUSED_P] + [_VP] * 6 + [_L, _VP]),
+    "attn_bwd_b200_fused_bwd": (_I, [_FUSED_P] + [_VP] * 10 + [_L, _VP]),
     "attn_bwd_b200_poll_error": (_I, []),
     "attn_bwd_b200_selftest_wait_timeout": (_I, [_I, _VP]),
     "attn_bwd_b200_strerror": (ctypes.c_char_p, [_I]),

@@ -1,0 +1,180 @@
+"""Rotary positions of query and key states, forward and gradient, over ``attn_bwd_b200_rope``."""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+__all__ = ["RopeTable", "rope_table", "rope_fwd", "rope_bwd"]
+
+_TYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_FP16, torch.float32: _lib.DT_FP32}
+
+
+class RopeTable:
+    """Frequencies of a rotation, made once by :func:`rope_table` and kept by the caller.
+
+    ``turns`` [rotary_dim / 2] int64 on the GPU: each frequency as a 64-bit fixed-point fraction
+    of a turn a position; ``factor`` multiplies the rotated part of a head."""
+
+    __slots__ = ("turns", "rotary_dim", "factor")
+
+    def __init__(self, turns, rotary_dim, factor):
+        self.turns, self.rotary_dim, self.factor = turns, rotary_dim, factor
+
+
+def rope_table(rotary_dim, base=10000.0, scaling=None, device="cuda"):
+    """Table for angles position * f_n, f_n = base^(-2n / rotary_dim), n < rotary_dim / 2.
+
+    ``scaling`` stretches the positions for contexts longer than the model was trained for:
+      {"type": "linear", "factor": s}: every f_n divided by s;
+      {"type": "base", "factor": s}: the base times s^(rotary_dim / (rotary_dim - 2)), which
+        leaves the fastest pair alone and divides the slowest frequency by s;
+      {"type": "ramp", "factor": s, "original_length": L, "low": a, "high": b}: pairs that turn
+        fewer than a times over L positions are divided by s, pairs that turn more than b times
+        are kept, linear between; both coordinates are multiplied by 0.1 ln(s) + 1 (or by
+        "attention_factor" if given)."""
+    if not isinstance(rotary_dim, int) or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be a positive even number, got {rotary_dim!r}")
+    base = float(base)
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError(f"base must be positive, got {base}")
+    factor, kind, s = 1.0, None, 1.0
+    if scaling is not None:
+        scaling = dict(scaling)
+        kind = scaling.pop("type", None)
+        known = {"linear": {"factor"}, "base": {"factor"},
+                 "ramp": {"factor", "original_length", "low", "high", "attention_factor"}}
+        if kind not in known:
+            raise ValueError(f"unknown scaling type {kind!r}; known: {sorted(known)}")
+        if set(scaling) - known[kind]:
+            raise ValueError(f"unknown scaling keys {sorted(set(scaling) - known[kind])} for {kind!r}")
+        s = float(scaling.get("factor", 0.0))
+        if not (s >= 1.0 and math.isfinite(s)):
+            raise ValueError(f"scaling factor must be at least 1, got {s}")
+    if kind == "base":
+        if rotary_dim == 2:
+            raise ValueError("base scaling needs rotary_dim > 2")
+        base *= s ** (rotary_dim / (rotary_dim - 2))
+    f = [base ** (-2.0 * n / rotary_dim) for n in range(rotary_dim // 2)]
+    if kind == "linear":
+        f = [x / s for x in f]
+    elif kind == "ramp":
+        length, low, high = (float(scaling.get(k, d)) for k, d in (("original_length", 0.0), ("low", 1.0), ("high", 32.0)))
+        if not (length > 0 and high > low):
+            raise ValueError("ramp scaling needs original_length > 0 and high > low")
+        keep = [min(1.0, max(0.0, (length * x / (2 * math.pi) - low) / (high - low))) for x in f]
+        f = [x * w + x / s * (1.0 - w) for x, w in zip(f, keep)]
+        factor = float(scaling.get("attention_factor", 0.1 * math.log(s) + 1.0))
+    turns = [round(math.fmod(x / (2 * math.pi), 1.0) * 2.0 ** 64) % 2 ** 64 for x in f]
+    turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
+    return RopeTable(torch.tensor(turns, dtype=torch.int64).to(device), rotary_dim, factor)
+
+
+def _check(x, name):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(x).__name__}")
+    if x.device.type != "cuda":
+        raise ValueError(f"{name}: tensor must be on a CUDA device (no CPU path), got {x.device}")
+    if x.dtype not in _TYPES:
+        raise TypeError(f"{name}: expected bfloat16, float16 or float32, got {x.dtype}")
+    if x.dim() != 4:
+        raise ValueError(f"{name}: expected [bs, heads, seq, head_dim], got {tuple(x.shape)}")
+
+
+def _overlaps_itself(t):
+    return any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape))
+
+
+def _rotate(q, k, position_ids, table, interleaved, inverse, out):
+    if not isinstance(table, RopeTable):
+        raise TypeError(f"table: expected a RopeTable (rope_table(...)), got {type(table).__name__}")
+    names = ("query", "key")
+    xs = [x for x in (q, k) if x is not None]
+    if not xs:
+        raise ValueError("nothing to rotate: both tensors are None")
+    for x, name in zip((q, k), names):
+        if x is not None:
+            _check(x, name)
+    first = xs[0]
+    bs, _, seq, d = first.shape
+    for x in xs:
+        if (x.shape[0], x.shape[2], x.shape[3]) != (bs, seq, d) or x.dtype != first.dtype or x.device != first.device:
+            raise ValueError("query and key must agree in batch, positions, head_dim, dtype and device, got "
+                             f"{[(tuple(x.shape), x.dtype, x.device) for x in xs]}")
+    if table.rotary_dim > d:
+        raise ValueError(f"table rotates {table.rotary_dim} elements, heads have {d}")
+    if table.turns.device != first.device:
+        raise ValueError(f"table is on {table.turns.device}, tensors on {first.device}")
+    if not isinstance(position_ids, torch.Tensor) or position_ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError("position_ids: expected an int64 or int32 tensor")
+    if position_ids.device != first.device:
+        raise ValueError(f"position_ids is on {position_ids.device}, tensors on {first.device}")
+    shape = tuple(position_ids.shape)
+    if shape not in ((seq,), (1, seq), (bs, seq)):
+        raise ValueError(f"position_ids: expected [{seq}], [1, {seq}] or [{bs}, {seq}], got {shape}")
+    with torch.cuda.device(first.device):
+        pos = position_ids.to(torch.int64).contiguous()
+        per_batch = pos.dim() == 2 and pos.shape[0] == bs and bs > 1
+        outs = []
+        if out is None:
+            out = (None, None)
+        elif not isinstance(out, (tuple, list)) or len(out) != 2:
+            raise ValueError("out: expected a pair (query, key) of tensors or None")
+        ins = []
+        for x, o, name in zip((q, k), out, names):
+            if x is None:
+                if o is not None:
+                    raise ValueError(f"out: {name} was not given")
+                ins.append(None)
+                outs.append(None)
+                continue
+            if x.stride(3) != 1 and d > 1:
+                x = x.contiguous()
+            if o is None:
+                o = torch.empty_like(x)   # same order in memory as the input
+                if o.stride(3) != 1:
+                    o = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            else:
+                if (not isinstance(o, torch.Tensor) or o.shape != x.shape or o.dtype != x.dtype or
+                        o.device != x.device or (o.stride(3) != 1 and d > 1)):
+                    raise ValueError(f"out: {name} must match the input's shape, dtype and device, head elements contiguous")
+                if _overlaps_itself(o):
+                    raise ValueError(f"out: {name} overlaps itself")
+                if o.data_ptr() == x.data_ptr() and o.stride() != x.stride():
+                    raise ValueError(f"out: {name} shares the input's memory in another order")
+            ins.append(x)
+            outs.append(o)
+        a = _lib.RopeArgs()
+        a.bs, a.seq, a.head_dim, a.rotary_dim = bs, seq, d, table.rotary_dim
+        a.q_heads = q.shape[1] if q is not None else 0
+        a.k_heads = k.shape[1] if k is not None else 0
+        a.dtype = _TYPES[first.dtype]
+        a.interleaved, a.inverse = int(bool(interleaved)), int(inverse)
+        a.factor = table.factor
+        a.position_stride = seq if per_batch else 0
+        for t, dst in zip((ins[0], ins[1], outs[0], outs[1]), (a.q_in, a.k_in, a.q_out, a.k_out)):
+            if t is not None:
+                dst[:] = t.stride()[:3]
+        ptr = [0 if t is None else t.data_ptr() for t in (ins[0], ins[1])]
+        optr = [0 if t is None else t.data_ptr() for t in outs]
+        _lib.call("attn_bwd_b200_rope", ctypes.byref(a), ptr[0], ptr[1], pos.data_ptr(), table.turns.data_ptr(),
+                  optr[0], optr[1], torch.cuda.current_stream().cuda_stream)
+    return outs[0], outs[1]
+
+
+def rope_fwd(query_states, key_states, position_ids, table, interleaved=False, out=None):
+    """Rotates query_states [bs, heads, seq, d] and key_states [bs, kv_heads, seq, d] (either may
+    be None) at position_ids ([seq], [1, seq] or [bs, seq]; any integer, however far) in one launch.
+
+    The first ``table.rotary_dim`` elements of a head are rotated, the rest is copied.  Pairs are
+    (n, n + rotary_dim / 2), or neighbours with ``interleaved``.  bfloat16, float16 or float32;
+    any strides (heads inside positions or positions inside heads); the results keep the inputs' order in
+    memory.  ``out`` takes preallocated results and may be the inputs themselves."""
+    return _rotate(query_states, key_states, position_ids, table, interleaved, False, out)
+
+
+def rope_bwd(grad_query, grad_key, position_ids, table, interleaved=False, out=None):
+    """Gradients of :func:`rope_fwd`'s inputs from those of its results: the inverse rotation,
+    times the table's factor.  Arguments as there."""
+    return _rotate(grad_query, grad_key, position_ids, table, interleaved, True, out)

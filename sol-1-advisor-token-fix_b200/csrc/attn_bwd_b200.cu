@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "../../include/attn_bwd_b200.h"
+#include "host_shared.h"
 #include "ds_kernel.cuh"
 #include "dv_kernel.cuh"
 
@@ -763,6 +764,25 @@ int run_host(DeviceState* st, const Shape& s, int chunks, const void* dO_h, cons
 }
 
 }  // namespace
+
+namespace attn_bwd {
+
+int host_device(HostDevice* out) {
+  DeviceState* st = nullptr;
+  const int rc = device_state(&st);
+  if (rc) return rc;
+  out->index = int(st - g_dev);
+  out->sm_count = st->sm_count;
+  out->err = st->err;
+  return ATTN_BWD_OK;
+}
+
+bool host_make_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* ptr, const cuuint64_t* dims,
+                   const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle sw) {
+  return make_map(m, dt, rank, ptr, dims, strides, box, sw);
+}
+
+}  // namespace attn_bwd
 
 extern "C" {
 

@@ -25,7 +25,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 HEADER = os.path.join(ROOT, "include", "attn_bwd_b200.h")
-KERNEL_SOURCES = ("attn_bwd_b200.cu", "ds_kernel.cuh", "dv_kernel.cuh", "sm100.cuh")
+# what attn_bwd_b200.cu includes; the library's other translation units (rope, fused attention)
+# serve calls that a submission does not make
+KERNEL_SOURCES = ("attn_bwd_b200.cu", "host_shared.h", "ds_kernel.cuh", "dv_kernel.cuh", "sm100.cuh")
 
 _TEMPLATE = r'''"""Single-file submission: GQA attention backward on hand-written sm_100a (B200) kernels.
 
@@ -67,7 +69,7 @@ def _build():
         if os.path.exists(lib):
             return lib
         for name, text in _SOURCES.items():
-            sub = "include" if name.endswith(".h") else os.path.join("src", "csrc")
+            sub = "include" if name == "attn_bwd_b200.h" else os.path.join("src", "csrc")
             with open(os.path.join(d, sub, name), "w") as f:
                 f.write(text)
         nvcc = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")
