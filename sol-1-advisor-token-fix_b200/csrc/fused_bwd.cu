@@ -25,7 +25,7 @@ static int dkv_splits(const attn_bwd_fused_t* a, int sm_count) {
 
 struct BwdLayout {
   int sq_pad, splits;
-  int64_t stat, part, total;   // bytes
+  int64_t stat, part, range, total;   // bytes
 };
 static BwdLayout layout_bwd(const attn_bwd_fused_t* a, int sm_count) {
   BwdLayout l;
@@ -33,7 +33,9 @@ static BwdLayout layout_bwd(const attn_bwd_fused_t* a, int sm_count) {
   l.splits = dkv_splits(a, sm_count);
   l.stat = (int64_t)a->bs * a->heads * l.sq_pad * 4;
   l.part = l.splits > 1 ? (int64_t)l.splits * a->bs * a->kv_heads * a->seq_kv * 2 * a->head_dim * 4 : 0;
-  l.total = 2 * l.stat + l.part;
+  // document ranges of the query tiles and of the key tiles
+  l.range = a->q_documents ? (int64_t)a->bs * (tiles_of(a->seq_q) + tiles_of(a->seq_kv)) * int64_t(sizeof(DocRange)) : 0;
+  l.total = 2 * l.stat + l.part + l.range;
   return l;
 }
 
@@ -50,6 +52,13 @@ static int launch(const BwdParams& f, const void* go, const void* o, const float
     bwd_stats_kernel<D, F16><<<unsigned((threads + 255) / 256), 256, 0, s>>>(
         static_cast<const uint8_t*>(go), static_cast<const uint8_t*>(o), lse, const_cast<float*>(f.nlse),
         const_cast<float*>(f.ndelta), p.bs, p.sq, f.sq_pad, p.H);
+    if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
+  }
+  if (p.has_docs) {
+    const long long tiles = (long long)p.bs * (p.n_tiles + f.n_kt);
+    doc_ranges_kernel<<<unsigned((tiles + 7) / 8), 256, 0, s>>>(p.kdoc, p.skv, p.qdoc, p.sq, p.bs,
+                                                                const_cast<DocRange*>(p.krange),
+                                                                const_cast<DocRange*>(p.qrange));
     if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
   }
   if (p.skv > 0) {
@@ -95,7 +104,8 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
   if (a->seq_kv && (!k || !v || !dk || !dv)) return ATTN_BWD_EINVAL;
   if (!al16(go) || !al16(q) || !al16(k) || !al16(v) || !al16(o) || !al16(dq) || !al16(dk) || !al16(dv))
     return ATTN_BWD_EALIGN;
-  if (tiles_of(a->seq_q) > kMaxListBwd || tiles_of(a->seq_kv) > kMaxListBwd) return ATTN_BWD_EUNSUPPORTED;
+  // with documents a unit lists its tiles
+  if (a->q_documents && (tiles_of(a->seq_q) > kMaxList || tiles_of(a->seq_kv) > kMaxList)) return ATTN_BWD_EUNSUPPORTED;
   HostDevice dev;
   if ((rc = host_device(&dev))) return rc;
   const BwdLayout l = layout_bwd(a, dev.sm_count);
@@ -111,7 +121,10 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
   float* ws = static_cast<float*>(workspace);
   f.nlse = ws;
   f.ndelta = ws + l.stat / 4;
+  f.n_kt = tiles_of(a->seq_kv);
   f.part = ws + l.stat / 2;
+  f.c.qrange = reinterpret_cast<const DocRange*>(reinterpret_cast<const uint8_t*>(f.part) + l.part);
+  f.c.krange = f.c.qrange + (int64_t)a->bs * f.c.n_tiles;
   f.dq = dq;
   f.dk = dk;
   f.dv = dv;

@@ -12,9 +12,11 @@ namespace fused {
 using namespace sm100;
 
 constexpr int TILE = 128;        // rows of a query tile, keys of a key tile
-constexpr int kMaxList = 2048;   // tiles that one CTA visits at most
+constexpr int kMaxList = 2048;   // documents: tiles of one unit at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+struct DocRange;
 
 struct Params {
   int bs, sq, skv, H, Hkv, G;
@@ -27,6 +29,7 @@ struct Params {
   const float* slopes;     // [H] or null
   const int* prefix;       // [bs] or null
   const int *qdoc, *kdoc;  // [bs, sq], [bs, skv] or null
+  const DocRange *qrange, *krange;   // of the 128-position tiles, [bs, tiles]
   int n_tiles;             // tiles of the axis a CTA loops over
   int splits, tiles_per_split;
   int* err;
@@ -39,12 +42,12 @@ __device__ __forceinline__ int row_limit(const Params& p, int r, int pre) {
   return min(p.skv, max(r + p.off + 1, pre));
 }
 
-// Lowest and highest document number (>= 0) of n ids, and whether any id is negative, over
-// one warp; every lane returns the same values.  No id >= 0: lo > hi.
+// Lowest and highest document number (>= 0) of some ids, and whether any id is negative.  No
+// id >= 0: lo > hi.
 struct DocRange {
-  int lo, hi;
-  bool neg;
+  int lo, hi, neg, pad;
 };
+// The same on every lane of a warp.
 __device__ __forceinline__ DocRange warp_doc_range(const int* ids, int n, uint32_t lane) {
   int lo = 0x7fffffff, hi = -1;
   bool neg = false;
@@ -60,41 +63,152 @@ __device__ __forceinline__ DocRange warp_doc_range(const int* ids, int n, uint32
   r.lo = __reduce_min_sync(0xffffffffu, lo);
   r.hi = __reduce_max_sync(0xffffffffu, hi);
   r.neg = __any_sync(0xffffffffu, neg);
+  r.pad = 0;
   return r;
 }
-
-// List entry: tile offset from the CTA's first tile, and whether single scores of the tile
-// have to be masked, and whether rows of the streamed tile belong to no document and so are
-// cleared before a product reads them.
-constexpr uint32_t kEntMask = 0x8000u, kEntScrub = 0x4000u, kEntTile = 0x3fffu;
-constexpr int kStSkip = 0, kStFull = 1, kStMask = 2, kStScrub = 4;
-
-// State of the pair (query range, key range): rows of the range [r0, r1], keys [j0, j1].
-__device__ __forceinline__ int pair_state(const Params& p, int pre, int r0, int r1, int j0, int j1, bool docs,
-                                          const DocRange& qd, const DocRange& kd) {
-  const int lim0 = row_limit(p, r0, pre), lim1 = row_limit(p, r1, pre);   // limits grow with the row
-  if (lim1 <= j0) return kStSkip;
-  bool full = lim0 > j1;
-  if (docs) {
-    if (qd.hi < qd.lo || kd.hi < kd.lo || qd.hi < kd.lo || kd.hi < qd.lo) return kStSkip;
-    full = full && !qd.neg && !kd.neg && qd.lo == qd.hi && kd.lo == kd.hi;
-  }
-  return full ? kStFull : kStMask;
+// Ranges of all key tiles, then (sq > 0) of all query tiles, one warp a tile.
+static __global__ void __launch_bounds__(256) doc_ranges_kernel(const int* __restrict__ kdoc, int skv,
+                                                         const int* __restrict__ qdoc, int sq, int bs,
+                                                         DocRange* __restrict__ kr, DocRange* __restrict__ qr) {
+  const int nk = (skv + TILE - 1) / TILE, nq = (sq + TILE - 1) / TILE;
+  long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t lane = threadIdx.x & 31;
+  const bool q = t >= (long long)bs * nk;
+  if (q) t -= (long long)bs * nk;
+  const int n = q ? nq : nk, s = q ? sq : skv;
+  if (t >= (long long)bs * n) return;
+  const int b = int(t / n), r0 = int(t - (long long)b * n) * TILE;
+  const DocRange r = warp_doc_range((q ? qdoc : kdoc) + (size_t)b * s + r0, min(TILE, s - r0), lane);
+  if (lane == 0) (q ? qr : kr)[t] = r;
 }
 
-// Turns states[0..n) (shared memory) into the list of tiles that are not skipped; one warp.
-__device__ __forceinline__ int compact_list(const uint8_t* states, int n, uint16_t* list, uint32_t lane) {
-  int cnt = 0;
-  for (int t0 = 0; t0 < n; t0 += 32) {
-    const int t = t0 + int(lane);
-    const int st = t < n ? states[t] : kStSkip;
-    const uint32_t vote = __ballot_sync(0xffffffffu, st != kStSkip);
-    if (st != kStSkip)
-      list[cnt + __popc(vote & ((1u << lane) - 1u))] =
-          uint16_t(uint32_t(t) | ((st & kStMask) ? kEntMask : 0u) | ((st & kStScrub) ? kEntScrub : 0u));
-    cnt += __popc(vote);
+// A tile of a CTA's loop: number (from the unit's first tile), whether single scores have to be
+// masked, and whether rows of the streamed tile belong to no document and so are cleared before
+// a product reads them.
+constexpr uint32_t kEntMask = 0x8000u, kEntScrub = 0x4000u, kEntTile = 0x3fffu;
+constexpr int kStSkip = 0, kStFull = 1, kStMask = 2;
+
+// State of the pair (query range, key range): rows of the range [r0, r1], keys [j0, j1].
+__device__ __forceinline__ int pair_state(const Params& p, int pre, int r0, int r1, int j0, int j1, const DocRange& qd,
+                                          const DocRange& kd) {
+  const int lim0 = row_limit(p, r0, pre), lim1 = row_limit(p, r1, pre);   // limits grow with the row
+  if (lim1 <= j0 || qd.hi < qd.lo || kd.hi < kd.lo || qd.hi < kd.lo || kd.hi < qd.lo) return kStSkip;
+  return lim0 > j1 && !qd.neg && !kd.neg && qd.lo == qd.hi && kd.lo == kd.hi ? kStFull : kStMask;
+}
+
+// Appends the lanes' tiles to a list, in order; one warp.  state: of tile t, kStSkip: left out.
+__device__ __forceinline__ int list_append(uint16_t* list, int cnt, int t, int state, bool scrub, uint32_t lane) {
+  const uint32_t vote = __ballot_sync(0xffffffffu, state != kStSkip);
+  if (state != kStSkip)
+    list[cnt + __popc(vote & ((1u << lane) - 1u))] =
+        uint16_t(uint32_t(t) | (state == kStMask ? kEntMask : 0u) | (scrub ? kEntScrub : 0u));
+  return cnt + __popc(vote);
+}
+
+// ---- units: a kernel's blocks are taken up by CTAs that stay, one an SM.  The scheduler warp
+// asks the hardware for the next block that has not started (cluster launch control) while
+// the current one is worked on, so its loads and first products start early and no SM waits
+// for a launch.  Two slots: the unit in work and the next.
+struct alignas(16) Unit {
+  int x, y, z;     // block index; x < 0: no more units
+  int n;           // documents: tiles of the list
+};
+struct Scheduler {
+  Unit* slot;          // [2]
+  uint64_t *full, *empty, *answer;
+  uint64_t* ask;       // the producer has issued the last loads of a unit: time to take up another
+  uint32_t handle;     // shared address of the hardware's answer (16 bytes)
+};
+__device__ __forceinline__ void ask_next(const Scheduler& s) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   s.handle),
+               "r"(smem_u32(s.answer))
+               : "memory");
+}
+// Block index of the answer; false: no block is left.
+__device__ __forceinline__ bool read_answer(const Scheduler& s, int& x, int& y, int& z) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\t"
+      "ld.shared.b128 h, [%4];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %3, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, %1, %2, _}, h;\n\t}\n"
+      : "=&r"(x), "=&r"(y), "=&r"(z), "=&r"(ok)
+      : "r"(s.handle)
+      : "memory");
+  return ok != 0;
+}
+constexpr int kUnitReaders = 10;   // producer, tensor cores, 8 warps of rows
+__device__ __forceinline__ void scheduler_init(const Scheduler& s) {
+  for (int i = 0; i < 2; ++i) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], kUnitReaders); }
+  mbar_init(s.answer, 1);
+  mbar_init(s.ask, 1);
+}
+// The scheduler warp.  build(unit, slot) -> n prepares a unit's list (one warp).
+template <typename F>
+__device__ __forceinline__ void run_scheduler(const Scheduler& s, volatile int* abort, int* err, int code, F build) {
+  const uint32_t lane = lane_id();
+  int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z;
+  bool have = true;
+  for (uint32_t k = 0;; ++k) {
+    const uint32_t i = k & 1;
+    if (!warp_wait(&s.empty[i], ((k >> 1) & 1) ^ 1, abort, err, code)) return;
+    const int n = have ? build(x, y, z, i) : 0;
+    __syncwarp();
+    if (lane == 0) {
+      s.slot[i] = Unit{have ? x : -1, y, z, n};
+      mbar_arrive(&s.full[i]);
+    }
+    if (!have) return;
+    // not earlier: a CTA that took its next unit at once would hold it while others run dry
+    if (!warp_wait(s.ask, k & 1, abort, err, code + 2)) return;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(s.answer, 16);
+      ask_next(s);
+    }
+    if (!warp_wait(s.answer, k & 1, abort, err, code + 1)) return;
+    have = read_answer(s, x, y, z);
+    fence_proxy_async_smem();   // the next answer is written by the async proxy
+    __syncwarp();
   }
-  return cnt;
+}
+// A reader's next unit; false: none left (or the kernel gives up).
+__device__ __forceinline__ bool next_unit(const Scheduler& s, uint32_t k, Unit& u, volatile int* abort, int* err,
+                                          int code) {
+  if (!warp_wait(&s.full[k & 1], (k >> 1) & 1, abort, err, code)) return false;
+  u = s.slot[k & 1];
+  return u.x >= 0;
+}
+__device__ __forceinline__ void ask_for_unit(const Scheduler& s) {   // producer
+  __syncwarp();
+  if (lane_id() == 0) mbar_arrive(s.ask);
+}
+__device__ __forceinline__ void unit_done(const Scheduler& s, uint32_t k) {
+  __syncwarp();
+  if (lane_id() == 0) mbar_arrive(&s.empty[k & 1]);
+}
+
+// ---- results: a warp holds 32 rows of 16-bit values, one a lane, and writes them 64 bytes of
+// each row at a time through its 2 KB of shared memory, so that 4 neighbouring lanes write one row's
+// 64 bytes (a lane writing its own row would touch 32 lines an instruction).
+// w: 32 values of this lane's row as 16 pairs; dst: where they go, null for a row that does not exist.
+__device__ __forceinline__ void write_rows(uint32_t stage, const uint32_t (&w)[16], uint8_t* dst, uint32_t lane) {
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    sts128(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+  __syncwarp();
+  const uint32_t c = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t r = i * 8 + (lane >> 2);
+    uint8_t* row = reinterpret_cast<uint8_t*>(
+        __shfl_sync(0xffffffffu, static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(dst)), int(r)));
+    const uint4 v = lds128(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+    if (row) *reinterpret_cast<uint4*>(row + c * 16) = v;
+  }
 }
 
 // Register split of the attention kernels: three warpgroups are launched with 168 registers a
@@ -133,9 +247,41 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   return make_float2(bf16lo(w), bf16hi(w));
 }
 
-// 1 / (1 + e^(2x)) with 2 x log2(e) given: tanh x = 1 - 2r and tanh' x = 4 r (1 - r), both to
-// fp32 accuracy (2^z overflows to inf, whose reciprocal is 0: the limit).
-__device__ __forceinline__ float cap_r(float z) { return rcp(1.f + ex2(z)); }
+// r = 1 / (1 + 2^z) of four z = 2 x log2(e): tanh x = 1 - 2r and tanh' x = 4 r (1 - r), both to
+// fp32 accuracy.  Special functions bound the capped kernels, so four share one reciprocal,
+// 1 / ((1 + a)(1 + b)(1 + c)(1 + d)); z is cut at 30 (r = 2^-30: the tanh is 1 in fp32) so that
+// the product stays below 2^121.
+__device__ __forceinline__ void cap_r4(float (&z)[4]) {
+  float a[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = 1.f + ex2(fminf(z[i], 30.f));
+  const float ab = a[0] * a[1], cd = a[2] * a[3];
+  const float inv = rcp(ab * cd);
+  const float iab = inv * cd, icd = inv * ab;
+  z[0] = iab * a[1];
+  z[1] = iab * a[0];
+  z[2] = icd * a[3];
+  z[3] = icd * a[2];
+}
+
+// Which of 32 ids per word (this lane holds ids[k * 32 + lane] in v[k]) equal this lane's own id:
+// one ballot a word for each different id of the warp's rows, usually one or two.
+template <int N>
+__device__ __forceinline__ void same_ids(const int (&v)[N], int id, uint32_t (&same)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) same[k] = 0u;
+  uint32_t todo = __ballot_sync(0xffffffffu, id >= 0);
+  while (todo) {
+    const int cur = __shfl_sync(0xffffffffu, id, __ffs(int(todo)) - 1);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const uint32_t m = __ballot_sync(0xffffffffu, v[k] == cur);
+      if (id == cur) same[k] = m;
+    }
+    todo &= ~__ballot_sync(0xffffffffu, id == cur);
+  }
+}
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // kind::f16 instruction descriptor for fp16 (0) or bf16 (1) operands, f32 accumulator.
 __host__ __device__ constexpr uint32_t idesc16(bool f16, int M, int N, bool a_mn, bool b_mn) {

@@ -28,11 +28,11 @@ static FwdParams plan_fwd(const attn_bwd_fused_t* a, int sm_count) {
   f.blocks_q = (p.sq + pos_per_unit - 1) / pos_per_unit;
   p.n_tiles = (p.skv + TILE - 1) / TILE;
   // Too few units for the GPU: split the keys, two tiles a split at least (below that the
-  // join costs more than it saves), and never more tiles a CTA than its list holds.
+  // join costs more than it saves), and never more tiles than a unit's list holds.
   const long long units = (long long)f.blocks_q * f.head_slots * p.bs;
   long long splits = units > 0 ? sm_count / units : 1;
   if (splits > p.n_tiles / 2) splits = p.n_tiles / 2;
-  const long long least = (p.n_tiles + kMaxList - 1) / kMaxList;
+  const long long least = p.has_docs ? (p.n_tiles + kMaxList - 1) / kMaxList : 1;
   if (splits < least) splits = least;
   if (splits < 1) splits = 1;
   p.tiles_per_split = int((p.n_tiles + splits - 1) / splits);
@@ -42,12 +42,15 @@ static FwdParams plan_fwd(const attn_bwd_fused_t* a, int sm_count) {
   return f;
 }
 
-static int64_t rows_pad(const Params& p) { return (int64_t)p.splits * p.bs * p.H * p.sq; }
+// Workspace: document ranges of the key tiles, then the splits' outputs and row statistics.
+static int64_t range_bytes(const Params& p) {
+  return p.has_docs ? ((int64_t)p.bs * p.n_tiles * int64_t(sizeof(DocRange)) + 255) / 256 * 256 : 0;
+}
+static int64_t part_rows(const Params& p) { return p.splits > 1 ? (int64_t)p.splits * p.bs * p.H * p.sq : 0; }
 
 int64_t fwd_workspace(const attn_bwd_fused_t* a, int sm_count) {
   const FwdParams f = plan_fwd(a, sm_count);
-  if (f.c.splits == 1) return 0;
-  return rows_pad(f.c) * (a->head_dim + 1) * 4;
+  return range_bytes(f.c) + part_rows(f.c) * (a->head_dim + 1) * 4;
 }
 
 template <int D, bool F16, bool CAP>
@@ -57,6 +60,12 @@ static int launch(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k
   auto kern = fwd_kernel<D, F16, CAP>;
   const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
   if (rc) return rc;
+  if (f.c.has_docs && f.c.n_tiles > 0) {
+    const long long tiles = (long long)f.c.bs * f.c.n_tiles;
+    doc_ranges_kernel<<<unsigned((tiles + 7) / 8), 256, 0, stream>>>(f.c.kdoc, f.c.skv, nullptr, 0, f.c.bs,
+                                                                    const_cast<DocRange*>(f.c.krange), nullptr);
+    if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
+  }
   kern<<<dim3(unsigned(f.blocks_q) * f.head_slots, f.c.bs, f.c.splits), kThreads, C::SMEM_BYTES, stream>>>(q, k, v, f);
   if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
   if (f.c.splits > 1) {
@@ -86,12 +95,13 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
   f.o = o;
   f.lse = lse;
   if (f.blocks_q > (1 << 30) / f.head_slots || p.splits > 65535) return ATTN_BWD_EINVAL;
-  if (p.splits > 1) {
-    const int64_t need = fwd_workspace(a, dev.sm_count);
+  const int64_t need = range_bytes(p) + part_rows(p) * (a->head_dim + 1) * 4;
+  if (need) {
     if (!workspace || workspace_bytes < need) return ATTN_BWD_EINVAL;
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return ATTN_BWD_EALIGN;
-    f.part_o = static_cast<float*>(workspace);
-    f.part_lse = f.part_o + rows_pad(p) * a->head_dim;
+    p.krange = static_cast<const DocRange*>(workspace);
+    f.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + range_bytes(p));
+    f.part_lse = f.part_o + part_rows(p) * a->head_dim;
   }
   const bool f16 = a->dtype == ATTN_BWD_DT_FP16;
   CUtensorMap mq, mk, mv;

@@ -4,8 +4,10 @@
 // One CTA holds up to two query tiles of 128 rows and streams key / value tiles of 128 keys
 // through a ring in shared memory; both tiles use each of them.  While the tensor cores work
 // for one query tile, the other one's softmax runs:
-//   warp 8  TMA producer      warp 9  tcgen05 issuer, TMEM owner
+//   warp 8  TMA producer      warp 9  tcgen05 issuer, TMEM owner      warp 10  units and their lists
 //   warps 0-3 softmax of tile 0, warps 4-7 of tile 1: one thread a row
+// A CTA stays on its SM and takes up unit after unit: the next unit's tiles are loaded and its
+// first scores computed while this one's rows are still written.
 // TMEM: two score tiles (128 columns each) and two outputs (D columns each).  The weights go
 // back to TMEM as 16-bit pairs over the scores they came from and are the A operand of the
 // second product, so they never touch shared memory.
@@ -42,33 +44,57 @@ struct FwdCfg {
   static constexpr int ST = D == 128 ? 4 : 8;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = 2 * TILE_BYTES;
-  static constexpr int OFF_LIST = OFF_KV + ST * TILE_BYTES;
-  static constexpr int OFF_STATE = OFF_LIST + kMaxList * 2;
-  static constexpr int OFF_DOC = OFF_STATE + kMaxList;          // per softmax warp: 128 ids
-  static constexpr int OFF_BAR = OFF_DOC + 8 * TILE * 4;
-  static constexpr int NBAR = 1 + 2 * ST + 6;
+  static constexpr int OFF_STAGE = OFF_KV + ST * TILE_BYTES;   // per warp of rows: 2 KB
+  static constexpr int OFF_LIST = OFF_STAGE + 8 * 2048;        // a list for each unit slot
+  static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
+  static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;            // two slots, the scheduler's answer
+  static constexpr int NBAR = 3 + 2 * ST + 6 + 6;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
-  static constexpr int SMEM_BYTES = OFF_MISC + 64 + 1024;
+  static constexpr int SMEM_BYTES = OFF_MISC + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024, "forward kernel shared memory");
 };
 
-// Applies the score transform to 128 raw scores of one row (in place, log2 units).
-// Keys j0..j0+127; lim: keys below it are seen; mask words: further keys taken out.
-template <bool CAP>
-__device__ __forceinline__ void transform_row(const Params& p, uint32_t (&s)[4][32], float slope2, float dist0) {
-  const float sl = p.scale_log2;
-#pragma unroll
-  for (int g = 0; g < 4; ++g)
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      float x = __uint_as_float(s[g][i]);
-      if (CAP) x = fmaf(-2.f * p.cap_out, cap_r(x * p.cap_in), p.cap_out);
-      else x *= sl;
-      x = fmaf(-slope2, fabsf(dist0 - float(g * 32 + i)), x);
-      s[g][i] = __float_as_uint(x);
-    }
+// What a unit is: its tiles' heads and positions, and the key tiles it visits.
+struct FwdUnit {
+  int b, split, kvh, nt;
+  int head[2], pos[2];
+  int last_pos;
+  int t0, n;          // first key tile of the split, number of visited ones
+  int pre, lim0;      // prefix; number of keys that the first row sees (documents aside)
+};
+__device__ __forceinline__ FwdUnit fwd_unit(const FwdParams& prm, const Unit& u) {
+  const Params& p = prm.c;
+  FwdUnit f;
+  // later positions see more keys and come first
+  const int qb = prm.blocks_q - 1 - u.x / prm.head_slots;
+  const int slot = u.x % prm.head_slots;
+  f.b = u.y;
+  f.split = u.z;
+  if (prm.packed) {
+    f.kvh = slot;
+    f.head[0] = f.head[1] = slot * p.G;
+    f.pos[0] = qb * 2 * prm.pos_per_tile;
+    f.pos[1] = f.pos[0] + prm.pos_per_tile;
+  } else if (prm.pair_heads) {
+    f.head[0] = slot * 2;
+    f.head[1] = slot * 2 + 1;
+    f.kvh = f.head[0] / p.G;
+    f.pos[0] = f.pos[1] = qb * TILE;
+  } else {
+    f.head[0] = f.head[1] = slot;
+    f.kvh = slot / p.G;
+    f.pos[0] = qb * 2 * TILE;
+    f.pos[1] = f.pos[0] + TILE;
+  }
+  f.nt = f.pos[1] < p.sq ? 2 : 1;
+  f.last_pos = min(p.sq, (f.nt == 2 ? f.pos[1] : f.pos[0]) + prm.pos_per_tile) - 1;
+  f.pre = p.prefix ? __ldg(p.prefix + f.b) : 0;
+  f.lim0 = row_limit(p, f.pos[0], f.pre);
+  f.t0 = f.split * p.tiles_per_split;
+  const int hi = max(0, row_limit(p, f.last_pos, f.pre) + TILE - 1) / TILE;
+  f.n = p.has_docs ? u.n : max(0, min(min(p.n_tiles, f.t0 + p.tiles_per_split), hi) - f.t0);
+  return f;
 }
-
 template <int D, bool F16, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64, heads of a row, positions, 1)
@@ -80,49 +106,34 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* q_full = bars;
-  uint64_t* kv_full = bars + 1;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* all_done = bars + 2;
+  uint64_t* kv_full = bars + 3;
   uint64_t* kv_empty = kv_full + ST;
   uint64_t* s_full = kv_empty + ST;    // [2] scores ready
   uint64_t* p_ready = s_full + 2;      // [2] weights written
   uint64_t* o_done = p_ready + 2;      // [2] second product done
+  Scheduler sched;
+  sched.slot = reinterpret_cast<Unit*>(smem + C::OFF_UNIT);
+  sched.handle = smem_u32(smem + C::OFF_UNIT + 32);
+  sched.full = o_done + 2;
+  sched.empty = sched.full + 2;
+  sched.answer = sched.empty + 2;
+  sched.ask = sched.answer + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
-  int* n_list_slot = reinterpret_cast<int*>(smem + C::OFF_MISC + 8);
-  uint16_t* list = reinterpret_cast<uint16_t*>(smem + C::OFF_LIST);
-  uint8_t* states = smem + C::OFF_STATE;
+  uint16_t* lists = reinterpret_cast<uint16_t*>(smem + C::OFF_LIST);
 
   const Params& p = prm.c;
   const uint32_t warp = warp_id(), lane = lane_id();
-  // unit: later positions see more keys and come first
-  const int qb = prm.blocks_q - 1 - int(blockIdx.x) / prm.head_slots;
-  const int slot = int(blockIdx.x) % prm.head_slots;
-  const int b = blockIdx.y, split = blockIdx.z;
-  const int ppt = prm.pos_per_tile;
-  // tile t: first head, first position
-  int kvh, head0, head1, pos0, pos1;
-  if (prm.packed) {
-    kvh = slot;
-    head0 = head1 = kvh * p.G;
-    pos0 = qb * 2 * ppt;
-    pos1 = pos0 + ppt;
-  } else if (prm.pair_heads) {
-    head0 = slot * 2;
-    head1 = head0 + 1;
-    kvh = head0 / p.G;
-    pos0 = pos1 = qb * TILE;
-  } else {
-    head0 = head1 = slot;
-    kvh = head0 / p.G;
-    pos0 = qb * 2 * TILE;
-    pos1 = pos0 + TILE;
-  }
-  const int nt = pos1 < p.sq ? 2 : 1;
-  const int last_pos = min(p.sq, (nt == 2 ? pos1 : pos0) + ppt) - 1;
-
+  int* err = p.err;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(all_done, 1);
     for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_done[i], 1); }
+    scheduler_init(sched);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -132,203 +143,260 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     prefetch_tmap(&tm_v);
   }
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
-
-  // key tiles of this CTA: [t0, t1) of the split, minus those that none of its rows sees
-  const int t0 = split * p.tiles_per_split;
-  const int t1 = min(p.n_tiles, t0 + p.tiles_per_split);
-  const int pre = p.prefix ? __ldg(p.prefix + b) : 0;
-  {
-    DocRange qd{0, -1, false};
-    if (p.has_docs) qd = warp_doc_range(p.qdoc + (size_t)b * p.sq + pos0, last_pos - pos0 + 1, lane);
-    if (p.has_docs) {
-      for (int t = t0 + int(warp); t < t1; t += kThreads / 32) {
-        const int j0 = t * TILE, j1 = min(p.skv, j0 + TILE) - 1;
-        const DocRange kd = warp_doc_range(p.kdoc + (size_t)b * p.skv + j0, j1 - j0 + 1, lane);
-        // keys behind the end are masked like unseen ones
-        int st = pair_state(p, pre, pos0, last_pos, j0, j0 + TILE - 1, true, qd, kd);
-        if (st != kStSkip && kd.neg) st |= kStScrub;
-        if (lane == 0) states[t - t0] = uint8_t(st);
-      }
-    } else {
-      for (int t = t0 + int(threadIdx.x); t < t1; t += kThreads) {
-        const int j0 = t * TILE;
-        states[t - t0] = uint8_t(pair_state(p, pre, pos0, last_pos, j0, j0 + TILE - 1, false, qd, qd));
-      }
-    }
-  }
-  __syncthreads();
-  if (warp == 0) {
-    const int n = compact_list(states, max(0, t1 - t0), list, lane);
-    if (lane == 0) *n_list_slot = n;
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int n = *n_list_slot;
-  int* err = p.err;
+  Unit u;
 
   if (warp >= 8) {
-   regs_shrink();
-   if (warp == 8) {
-    // ---------------------------------------------------------------- producer
-    if (n > 0) {
-      if (lane == 0) {
-        // a tile's box covers ppt positions x 1 head, or x the group's heads
-        const int rows = prm.packed ? ppt * p.G : TILE;
-        mbar_arrive_expect_tx(q_full, uint32_t(nt) * rows * D * 2);
-        for (int t = 0; t < nt; ++t)
-          for (int x = 0; x < D / 64; ++x)
-            tma_load_4d(smem + C::OFF_Q + t * C::TILE_BYTES + x * (TILE * 128), &tm_q, q_full, x * 64,
-                        t ? head1 : head0, t ? pos1 : pos0, b);
-      }
-      uint32_t si = 0;
-      bool ok = true;
-      for (int i = 0; i < n && ok; ++i) {
-        const int j0 = (t0 + int(list[i] & kEntTile)) * TILE;
-        for (int m = 0; m < 2; ++m) {
-          const uint32_t s = si % ST;
-          ok = warp_wait(&kv_empty[s], ((si / ST) & 1) ^ 1, abort_flag, err, 0x2101);
+    regs_shrink();
+    if (warp == 8) {
+      // -------------------------------------------------------------- producer
+      uint32_t si = 0, qi = 0;   // key / value tiles, query tiles loaded so far
+      for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, err, 0x2103); ++k) {
+        const FwdUnit f = fwd_unit(prm, u);
+        const uint16_t* list = lists + (k & 1) * kMaxList;
+        bool ok = true;
+        if (f.n > 0) {
+          ok = warp_wait(q_empty, (qi & 1) ^ 1, abort_flag, err, 0x2102);
           if (!ok) break;
+          ++qi;
           if (lane == 0) {
-            mbar_arrive_expect_tx(&kv_full[s], C::TILE_BYTES);
-            for (int x = 0; x < D / 64; ++x)
-              tma_load_4d(smem + C::OFF_KV + s * C::TILE_BYTES + x * (TILE * 128), m ? &tm_v : &tm_k, &kv_full[s],
-                          x * 64, j0, kvh, b);
+            // a tile's box covers pos_per_tile positions x 1 head, or x the group's heads
+            const int rows = prm.packed ? prm.pos_per_tile * p.G : TILE;
+            mbar_arrive_expect_tx(q_full, uint32_t(f.nt) * rows * D * 2);
+            for (int t = 0; t < f.nt; ++t)
+              for (int x = 0; x < D / 64; ++x)
+                tma_load_4d(smem + C::OFF_Q + t * C::TILE_BYTES + x * (TILE * 128), &tm_q, q_full, x * 64,
+                            t ? f.head[1] : f.head[0], t ? f.pos[1] : f.pos[0], f.b);
           }
-          ++si;
         }
+        for (int i = 0; i < f.n && ok; ++i) {
+          const int j0 = (f.t0 + (p.has_docs ? int(list[i] & kEntTile) : i)) * TILE;
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t s = si % ST;
+            ok = warp_wait(&kv_empty[s], ((si / ST) & 1) ^ 1, abort_flag, err, 0x2101);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&kv_full[s], C::TILE_BYTES);
+              for (int x = 0; x < D / 64; ++x)
+                tma_load_4d(smem + C::OFF_KV + s * C::TILE_BYTES + x * (TILE * 128), m ? &tm_v : &tm_k, &kv_full[s],
+                            x * 64, j0, f.kvh, f.b);
+            }
+            ++si;
+          }
+        }
+        if (!ok) break;
+        ask_for_unit(sched);
+        unit_done(sched, k);
       }
       if (lane == 0) {
-        mbar_drain(q_full, 0, err, 0x2111);
+        if (qi) mbar_drain(q_full, (qi - 1) & 1, err, 0x2111);
         for (uint32_t k = 0; k < uint32_t(ST) && k < si; ++k) {
           const uint32_t i = si - 1 - k;
           mbar_drain(&kv_full[i % ST], (i / ST) & 1, err, 0x2112);
         }
       }
       __syncwarp();
-    }
-   } else if (warp == 9) {
-    // ---------------------------------------------------------------- tensor cores
-    constexpr uint32_t id_s = idesc16(F16, TILE, TILE, false, false);
-    constexpr uint32_t id_o = idesc16(F16, TILE, D, false, true);
-    const uint32_t qs = smem_u32(smem + C::OFF_Q), kvs = smem_u32(smem + C::OFF_KV);
-    auto stage = [&](uint32_t si) { return kvs + (si % ST) * C::TILE_BYTES; };
-    auto full = [&](uint32_t si, int code) {
-      return warp_wait(&kv_full[si % ST], (si / ST) & 1, abort_flag, err, code);
-    };
-    if (n > 0 && warp_wait(q_full, 0, abort_flag, err, 0x2201) && full(0, 0x2202)) {
-      tc_fence_after();
-      if (lane == 0) {
-        for (int t = 0; t < nt; ++t) {
-          mma_kk<D>(tmem + t * TILE, qs + t * C::TILE_BYTES, stage(0), id_s);
-          umma_commit(&s_full[t]);
-        }
-        umma_commit(&kv_empty[0]);
-      }
-      __syncwarp();
-      for (int i = 0; i < n; ++i) {
-        const uint32_t kn = 2 * i + 2, vi = 2 * i + 1;
-        if (!full(vi, 0x2203)) break;
-        if (list[i] & kEntScrub) {
-          const int j0 = (t0 + int(list[i] & kEntTile)) * TILE;
-          scrub_rows<D>(stage(vi), p.kdoc + (size_t)b * p.skv + j0, p.skv - j0, lane);
-        }
-        if (i + 1 < n && !full(kn, 0x2204)) break;
-        bool ok = true;
-        for (int t = 0; t < nt && ok; ++t) {
-          ok = warp_wait(&p_ready[t], i & 1, abort_flag, err, 0x2205);
-          if (!ok) break;
+    } else if (warp == 9) {
+      // -------------------------------------------------------------- tensor cores
+      constexpr uint32_t id_s = idesc16(F16, TILE, TILE, false, false);
+      constexpr uint32_t id_o = idesc16(F16, TILE, D, false, true);
+      const uint32_t qs = smem_u32(smem + C::OFF_Q), kvs = smem_u32(smem + C::OFF_KV);
+      auto stage = [&](uint32_t si) { return kvs + (si % ST) * C::TILE_BYTES; };
+      auto full = [&](uint32_t si, int code) {
+        return warp_wait(&kv_full[si % ST], (si / ST) & 1, abort_flag, err, code);
+      };
+      uint32_t si = 0, qi = 0, cnt[2] = {0, 0};
+      for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, err, 0x2206); ++k) {
+        const FwdUnit f = fwd_unit(prm, u);
+        const uint16_t* list = lists + (k & 1) * kMaxList;
+        if (f.n > 0) {
+          if (!warp_wait(q_full, qi & 1, abort_flag, err, 0x2201) || !full(si, 0x2202)) break;
+          ++qi;
           tc_fence_after();
           if (lane == 0) {
-            mma_tn<D>(tmem + 2 * TILE + t * D, tmem + t * TILE, tmem + t * TILE + 32, stage(vi), id_o, i > 0);
-            umma_commit(&o_done[t]);
-            if (i + 1 < n) {   // after the last tile nobody waits for a free stage
-              if (t == nt - 1) umma_commit(&kv_empty[vi % ST]);
-              mma_kk<D>(tmem + t * TILE, qs + t * C::TILE_BYTES, stage(kn), id_s);
+            for (int t = 0; t < f.nt; ++t) {
+              mma_kk<D>(tmem + t * TILE, qs + t * C::TILE_BYTES, stage(si), id_s);
               umma_commit(&s_full[t]);
-              if (t == nt - 1) umma_commit(&kv_empty[kn % ST]);
             }
+            umma_commit(&kv_empty[si % ST]);
+            if (f.n == 1) umma_commit(q_empty);
           }
           __syncwarp();
+          bool ok = true;
+          for (int i = 0; i < f.n; ++i) {
+            const uint32_t vi = si + 1, kn = si + 2;
+            const bool more = i + 1 < f.n;
+            if (!(ok = full(vi, 0x2203))) break;
+            if (p.has_docs && (list[i] & kEntScrub)) {
+              const int j0 = (f.t0 + int(list[i] & kEntTile)) * TILE;
+              scrub_rows<D>(stage(vi), p.kdoc + (size_t)f.b * p.skv + j0, p.skv - j0, lane);
+            }
+            if (more && !(ok = full(kn, 0x2204))) break;
+            for (int t = 0; t < f.nt && ok; ++t) {
+              ok = warp_wait(&p_ready[t], cnt[t] & 1, abort_flag, err, 0x2205);
+              if (!ok) break;
+              ++cnt[t];
+              tc_fence_after();
+              if (lane == 0) {
+                mma_tn<D>(tmem + 2 * TILE + t * D, tmem + t * TILE, tmem + t * TILE + 32, stage(vi), id_o, i > 0);
+                umma_commit(&o_done[t]);
+                if (t == f.nt - 1) umma_commit(&kv_empty[vi % ST]);
+                if (more) {
+                  mma_kk<D>(tmem + t * TILE, qs + t * C::TILE_BYTES, stage(kn), id_s);
+                  umma_commit(&s_full[t]);
+                  if (t == f.nt - 1) {
+                    umma_commit(&kv_empty[kn % ST]);
+                    if (i + 2 == f.n) umma_commit(q_empty);
+                  }
+                }
+              }
+              __syncwarp();
+            }
+            if (!ok) break;
+            si += 2;
+          }
+          if (!ok) break;
         }
-        if (!ok) break;
+        unit_done(sched, k);
       }
+      // no commit may arrive after the block has left
+      if (lane == 0) umma_commit(all_done);
+      __syncwarp();
+      warp_wait(all_done, 0, abort_flag, err, 0x2207);
+    } else if (warp == 10) {
+      // -------------------------------------------------------------- units and their lists
+      run_scheduler(sched, abort_flag, err, 0x2401, [&](int x, int y, int z, uint32_t slot) {
+        if (!p.has_docs) return 0;
+        const FwdUnit f = fwd_unit(prm, Unit{x, y, z, 0});
+        const DocRange qd = warp_doc_range(p.qdoc + (size_t)f.b * p.sq + f.pos[0], f.last_pos - f.pos[0] + 1, lane);
+        const int hi = max(0, row_limit(p, f.last_pos, f.pre) + TILE - 1) / TILE;
+        const int t1 = min(min(p.n_tiles, f.t0 + p.tiles_per_split), hi);
+        int n = 0;
+        for (int t = f.t0; t < t1; t += 32) {
+          int st = kStSkip;
+          bool scrub = false;
+          if (t + int(lane) < t1) {
+            const int j0 = (t + int(lane)) * TILE;
+            const DocRange kd = p.krange[(size_t)f.b * p.n_tiles + t + lane];
+            // keys behind the end are masked like unseen ones
+            st = pair_state(p, f.pre, f.pos[0], f.last_pos, j0, j0 + TILE - 1, qd, kd);
+            scrub = kd.neg != 0;
+          }
+          n = list_append(lists + slot * kMaxList, n, t - f.t0 + int(lane), st, scrub, lane);
+        }
+        return n;
+      });
     }
-   }
   } else {
     // ---------------------------------------------------------------- softmax, one thread a row
     regs_grow();
     const int t = warp >> 2;
-    if (t < nt) {
-      const int row = int(warp & 3) * 32 + int(lane);
-      const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
-      const uint32_t t_s = tmem + t_lane + t * TILE, t_o = tmem + t_lane + 2 * TILE + t * D;
+    const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + t_lane + t * TILE, t_o = tmem + t_lane + 2 * TILE + t * D;
+    const int row = int(warp & 3) * 32 + int(lane);
+    const uint32_t stage = smem_u32(smem + C::OFF_STAGE) + warp * 2048;
+    const bool biased = p.slopes != nullptr;
+    const bool raw = !CAP && !biased;                      // raw scores scaled inside the exponent
+    const float c = raw ? p.scale_log2 : 1.f;
+    const float grow = 8.f / c;
+    uint32_t cnt = 0;
+    for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, err, 0x2304); ++k) {
+      const FwdUnit f = fwd_unit(prm, u);
+      if (t >= f.nt) {
+        unit_done(sched, k);
+        continue;
+      }
+      const uint16_t* list = lists + (k & 1) * kMaxList;
       int pos, head;
       bool valid;
       if (prm.packed) {
         const int r = row / p.G;
-        pos = (t ? pos1 : pos0) + r;
-        head = (t ? head1 : head0) + row - r * p.G;
-        valid = r < ppt && pos < p.sq;
+        pos = (t ? f.pos[1] : f.pos[0]) + r;
+        head = f.head[0] + row - r * p.G;
+        valid = r < prm.pos_per_tile && pos < p.sq;
       } else {
-        pos = (t ? pos1 : pos0) + row;
-        head = t ? head1 : head0;
+        pos = (t ? f.pos[1] : f.pos[0]) + row;
+        head = t ? f.head[1] : f.head[0];
         valid = pos < p.sq;
       }
-      int lim = valid ? row_limit(p, pos, pre) : 0;
-      const int qd = (valid && p.has_docs) ? __ldg(p.qdoc + (size_t)b * p.sq + pos) : -1;
-      if (p.has_docs && qd < 0) lim = 0;
+      int lim = valid ? row_limit(p, pos, f.pre) : 0;
+      const int qd = (valid && p.has_docs) ? __ldg(p.qdoc + (size_t)f.b * p.sq + pos) : -1;
       const bool any_valid = __any_sync(0xffffffffu, valid);   // warps of padding rows only pass barriers
-      const float slope2 = (p.slopes && valid) ? __ldg(p.slopes + head) * kLog2e : 0.f;
-      const bool raw = !CAP && !p.slopes;                      // raw scores scaled inside the exponent
-      const float c = raw ? p.scale_log2 : 1.f;
-      const float grow = 8.f / c;
-      const int* kdoc = p.has_docs ? p.kdoc + (size_t)b * p.skv : nullptr;
-      int* ids = reinterpret_cast<int*>(smem + C::OFF_DOC) + warp * TILE;
+      const float slope2 = (biased && valid) ? __ldg(p.slopes + head) * kLog2e : 0.f;
 
       float mref = -INFINITY;   // reference maximum (raw or log2 units)
       float l = 0.f;
       bool ok = true;
-      for (int i = 0; i < n; ++i) {
-        ok = warp_wait(&s_full[t], i & 1, abort_flag, err, 0x2301);
+      for (int i = 0; i < f.n; ++i) {
+        const uint32_t ent = p.has_docs ? list[i] : 0u;
+        const int j0 = (f.t0 + (p.has_docs ? int(ent & kEntTile) : i)) * TILE;
+        const bool masked = p.has_docs ? (ent & kEntMask) != 0 : j0 + TILE > f.lim0;
+        int ids[4];
+        if (masked && p.has_docs) {
+          const int* kdoc = p.kdoc + (size_t)f.b * p.skv;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int j = j0 + g * 32 + int(lane);
+            ids[g] = j < p.skv ? __ldg(kdoc + j) : -1;
+          }
+        }
+        ok = warp_wait(&s_full[t], (cnt + i) & 1, abort_flag, err, 0x2301);
         if (!ok) break;
         tc_fence_after();
         if (any_valid) {
-          const uint32_t ent = list[i];
-          const int j0 = (t0 + int(ent & kEntTile)) * TILE;
           uint32_t s[4][32];
 #pragma unroll
           for (int g = 0; g < 4; ++g) tmem_ld32(t_s + g * 32, s[g]);
           tmem_wait_ld();
-          if (!raw) transform_row<CAP>(p, s, slope2, float(pos + p.off - j0));
-          if (ent & kEntMask) {
-            if (p.has_docs) {
-              __syncwarp();
+          if (CAP) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int j = j0 + k * 32 + int(lane);
-                ids[k * 32 + lane] = j < p.skv ? __ldg(kdoc + j) : -1;
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                float z[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) z[y] = __uint_as_float(s[g][e + y]) * p.cap_in;
+                cap_r4(z);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) s[g][e + y] = __float_as_uint(fmaf(-2.f * p.cap_out, z[y], p.cap_out));
               }
-              __syncwarp();
+          }
+          if (biased) {
+            const float d0 = float(pos + p.off - j0), sl = CAP ? 1.f : p.scale_log2;
+            if (__all_sync(0xffffffffu, pos + p.off >= j0 + TILE - 1)) {   // |i - j| = i - j: linear in the column
+              const uint64_t sl2 = f2(sl, sl), a2 = f2(-slope2 * d0, -slope2 * d0), b2 = f2(slope2, slope2);
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                  float x0, x1;
+                  f2_split(f2_fma(f2(s[g][e], s[g][e + 1]), sl2,
+                                  f2_fma(b2, f2(float(g * 32 + e), float(g * 32 + e + 1)), a2)), x0, x1);
+                  s[g][e] = __float_as_uint(x0);
+                  s[g][e + 1] = __float_as_uint(x1);
+                }
+            } else {
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  s[g][e] = __float_as_uint(
+                      fmaf(__uint_as_float(s[g][e]), sl, -slope2 * fabsf(d0 - float(g * 32 + e))));
             }
+          }
+          if (masked) {
+            uint32_t see[4];
+            if (p.has_docs) same_ids<4>(ids, qd, see);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              const int m = min(max(lim - j0 - g * 32, 0), 32);
-              uint32_t see = m == 32 ? 0xffffffffu : (1u << m) - 1u;
-              if (p.has_docs) {
-                uint32_t same = 0;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  const int4 d = *reinterpret_cast<const int4*>(ids + g * 32 + k * 4);
-                  same |= (d.x == qd ? 1u : 0u) << (k * 4) | (d.y == qd ? 2u : 0u) << (k * 4) |
-                          (d.z == qd ? 4u : 0u) << (k * 4) | (d.w == qd ? 8u : 0u) << (k * 4);
-                }
-                see &= same;
-              }
+              const uint32_t below = low_bits(lim - j0 - g * 32);
+              see[g] = p.has_docs ? see[g] & below : below;
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (!((see >> e) & 1u)) s[g][e] = 0xff800000u;   // -inf
+                if (!((see[g] >> e) & 1u)) s[g][e] = 0xff800000u;   // -inf
             }
           }
           float mx[4];
@@ -342,11 +410,11 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (__any_sync(0xffffffffu, m > mref + grow)) {
             const float mnew = fmaxf(mref, m);
-            const float f = mref == mnew ? 1.f : ex2((mref - mnew) * c);   // 0 from a reference of -inf
+            const float fac = mref == mnew ? 1.f : ex2((mref - mnew) * c);   // 0 from a reference of -inf
             mref = mnew;
-            l *= f;
+            l *= fac;
             if (i > 0) {
-              ok = warp_wait(&o_done[t], (i - 1) & 1, abort_flag, err, 0x2302);
+              ok = warp_wait(&o_done[t], (cnt + i - 1) & 1, abort_flag, err, 0x2302);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll
@@ -357,8 +425,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
                 tmem_wait_ld();
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                  o[0][e] = __float_as_uint(__uint_as_float(o[0][e]) * f);
-                  o[1][e] = __float_as_uint(__uint_as_float(o[1][e]) * f);
+                  o[0][e] = __float_as_uint(__uint_as_float(o[0][e]) * fac);
+                  o[1][e] = __float_as_uint(__uint_as_float(o[1][e]) * fac);
                 }
                 tmem_st16(t_o + x * 32, o[0]);
                 tmem_st16(t_o + x * 32 + 16, o[1]);
@@ -395,58 +463,46 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
         if (lane == 0) mbar_arrive(&p_ready[t]);
       }
       // ---- epilogue: o / l, and the row statistic
-      if (ok && n > 0) ok = warp_wait(&o_done[t], (n - 1) & 1, abort_flag, err, 0x2303);
-      if (ok && any_valid) {
+      if (ok && f.n > 0) ok = warp_wait(&o_done[t], (cnt + f.n - 1) & 1, abort_flag, err, 0x2303);
+      if (!ok) break;
+      cnt += uint32_t(f.n);
+      if (any_valid) {
         tc_fence_after();
         const bool empty = l == 0.f;
         const float inv = empty ? 0.f : 1.f / l;
         const float lse = empty ? -INFINITY : (mref * c + log2f(l)) * kLn2;
-        const size_t rowi = ((size_t)b * p.H + head) * p.sq + pos;
-        if (p.splits > 1) {
-          const size_t ri = (size_t)split * p.bs * p.H * p.sq + rowi;
-          if (valid) prm.part_lse[ri] = lse;
-#pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            uint32_t o[32];
-            __syncwarp();
-            if (n > 0) {
-              tmem_ld32(t_o + x * 32, o);
-              tmem_wait_ld();
-            }
+        const size_t rowi = ((size_t)f.b * p.H + head) * p.sq + pos;
+        const size_t ri = (size_t)f.split * p.bs * p.H * p.sq + rowi;
+        if (valid) (p.splits > 1 ? prm.part_lse + ri : prm.lse + rowi)[0] = lse;
+        uint8_t* dst = static_cast<uint8_t*>(prm.o) + (((size_t)f.b * p.sq + pos) * p.H + head) * (D * 2);
+#pragma unroll 1
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t o[32];
+          __syncwarp();
+          if (f.n > 0) {
+            tmem_ld32(t_o + x * 32, o);
+            tmem_wait_ld();
+          }
+          if (p.splits > 1) {
             if (valid) {
-              float4* dst = reinterpret_cast<float4*>(prm.part_o + ri * D + x * 32);
+              float4* part = reinterpret_cast<float4*>(prm.part_o + ri * D + x * 32);
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                dst[e] = empty ? make_float4(0.f, 0.f, 0.f, 0.f)
-                               : make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
-                                             __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+                part[e] = empty ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                : make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
+                                              __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
             }
-          }
-        } else {
-          if (valid) prm.lse[rowi] = lse;
-          uint8_t* dst = static_cast<uint8_t*>(prm.o) + (((size_t)b * p.sq + pos) * p.H + head) * (D * 2);
+          } else {
+            uint32_t w[16];
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            uint32_t o[32];
-            __syncwarp();
-            if (n > 0) {
-              tmem_ld32(t_o + x * 32, o);
-              tmem_wait_ld();
-            }
-            if (valid) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint32_t w[4];
-#pragma unroll
-                for (int y = 0; y < 4; ++y)
-                  w[y] = empty ? 0u : pack2<F16>(__uint_as_float(o[8 * e + 2 * y]) * inv,
-                                                 __uint_as_float(o[8 * e + 2 * y + 1]) * inv);
-                *reinterpret_cast<uint4*>(dst + x * 64 + e * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-            }
+            for (int e = 0; e < 16; ++e)
+              w[e] = empty ? 0u : pack2<F16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            write_rows(stage, w, valid ? dst + x * 64 : nullptr, lane);
           }
         }
+        tc_fence_before();   // the next unit's first product overwrites the accumulator
       }
+      unit_done(sched, k);
     }
   }
   tc_fence_before();

@@ -88,7 +88,7 @@ def test_c_entry_refuses_pointers_and_strides_without_device():
         assert lib.attn_bwd_b200_fused_fwd(ctypes.byref(a), 16, 16, 16, 16, 16, 0, 0, 0) == _lib.EALIGN
         getattr(a, f)[2] = 0
         assert lib.attn_bwd_b200_fused_fwd(ctypes.byref(a), 16, 16, 16, 16, 16, 0, 0, 0) == _lib.EALIGN
-    a = _args(seq_q=(8192 << 7) + 1)
+    a = _args(seq_q=(2048 << 7) + 1, q_documents=16, kv_documents=16)   # more tiles than a list of documents holds
     assert lib.attn_bwd_b200_fused_bwd(ctypes.byref(a), *[16] * 9, 0, 0, 0) == _lib.EUNSUPPORTED
     a = _args(bs=0)   # nothing to do
     assert lib.attn_bwd_b200_fused_fwd(ctypes.byref(a), 0, 0, 0, 0, 0, 0, 0, 0) == _lib.OK
