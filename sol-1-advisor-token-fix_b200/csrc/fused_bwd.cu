@@ -122,6 +122,8 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
   f.nlse = ws;
   f.ndelta = ws + l.stat / 4;
   f.n_kt = tiles_of(a->seq_kv);
+  f.divH = fast_div(a->heads);
+  f.divHkv = fast_div(a->kv_heads);
   f.part = ws + l.stat / 2;
   f.c.qrange = reinterpret_cast<const DocRange*>(reinterpret_cast<const uint8_t*>(f.part) + l.part);
   f.c.krange = f.c.qrange + (int64_t)a->bs * f.c.n_tiles;

@@ -23,6 +23,7 @@ struct BwdParams {
   Params c;
   int sq_pad;            // sq rounded up to tiles: row length of nlse and ndelta
   int n_kt;              // key tiles
+  FastDiv divH, divHkv;
   const float* nlse;     // [bs * H, sq_pad]: -lse * log2(e); -inf for rows that see nothing
   const float* ndelta;   // [bs * H, sq_pad]: -sum(do * o)
   void *dq, *dk, *dv;
@@ -113,9 +114,10 @@ __device__ __forceinline__ uint32_t bwd_begin(const BwdShared& s, int st, const 
   tc_fence_after();
   return *s.tmem_slot;
 }
-__device__ __forceinline__ void bwd_end(uint32_t tmem) {
+__device__ __forceinline__ void bwd_end(const BwdShared& s, uint32_t tmem, int* err) {
   tc_fence_before();
   __syncthreads();
+  report_error(s.abort_flag, err);
   if (warp_id() == 9) {
     __syncwarp();
     tc_fence_after();
@@ -191,7 +193,7 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdParams& prm, const Unit& u)
   const Params& p = prm.c;
   DkvUnit f;
   // earlier keys are seen by more queries and come first
-  const int jt = u.x / p.Hkv;
+  const int jt = prm.divHkv.div(u.x);
   f.kvh = u.x - jt * p.Hkv;
   f.b = u.y;
   f.split = u.z;
@@ -228,7 +230,6 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
   const BwdShared sh = bwd_shared<D>(smem_raw);
   const Params& p = prm.c;
   const uint32_t warp = warp_id(), lane = lane_id();
-  int* err = p.err;
   const uint32_t tmem = bwd_begin(sh, ST, &tm_q, &tm_do, &tm_k, &tm_v);
   const uint32_t t_st = tmem, t_dp = tmem + TILE, t_dv = tmem + 2 * TILE, t_dk = t_dv + D;
   Unit u;
@@ -238,12 +239,12 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
     if (warp == 8) {
       // -------------------------------------------------------------- producer
       uint32_t it = 0, ri = 0;   // items and resident pairs loaded so far
-      for (uint32_t k = 0; next_unit(sh.sched, k, u, sh.abort_flag, err, 0x3103); ++k) {
+      for (uint32_t k = 0; next_unit(sh.sched, k, u, sh.abort_flag, 0x3103); ++k) {
         const DkvUnit f = dkv_unit(prm, u);
         const uint16_t* list = sh.lists + (k & 1) * kMaxList;
         bool ok = true;
         if (f.n > 0) {
-          ok = warp_wait(sh.res_empty, (ri & 1) ^ 1, sh.abort_flag, err, 0x3102);
+          ok = wait_for(sh.res_empty, (ri & 1) ^ 1, sh.abort_flag, 0x3102);
           if (!ok) break;
           ++ri;
           if (lane == 0) {
@@ -260,7 +261,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
             const int h = f.kvh * p.G + g;
             for (int m = 0; m < 2; ++m) {
               const uint32_t s = (2 * it + m) % ST;
-              ok = warp_wait(&sh.empty[s], (((2 * it + m) / ST) & 1) ^ 1, sh.abort_flag, err, 0x3101);
+              ok = wait_for(&sh.empty[s], (((2 * it + m) / ST) & 1) ^ 1, sh.abort_flag, 0x3101);
               if (!ok) break;
               if (lane == 0) {
                 mbar_arrive_expect_tx(&sh.full[s], C::TILE_BYTES + (m ? 0 : 2 * TILE * 4));
@@ -283,10 +284,10 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
         unit_done(sh.sched, k);
       }
       if (lane == 0) {
-        if (ri) mbar_drain(sh.res_full, (ri - 1) & 1, err, 0x3111);
+        if (ri) mbar_drain(sh.res_full, (ri - 1) & 1, p.err, 0x3111);
         for (uint32_t k = 0; k < uint32_t(ST) && k < 2 * it; ++k) {
           const uint32_t i = 2 * it - 1 - k;
-          mbar_drain(&sh.full[i % ST], (i / ST) & 1, err, 0x3112);
+          mbar_drain(&sh.full[i % ST], (i / ST) & 1, p.err, 0x3112);
         }
       }
       __syncwarp();
@@ -294,18 +295,19 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
       // -------------------------------------------------------------- tensor cores
       constexpr uint32_t id_s = idesc16(F16, TILE, TILE, false, false);
       constexpr uint32_t id_g = idesc16(F16, TILE, D, false, true);
-      const uint32_t ks = smem_u32(sh.smem + C::OFF_A), vs = ks + C::TILE_BYTES;
+      const bool one = elect_one();
+      const uint64_t ks = desc_k(smem_u32(sh.smem + C::OFF_A)), vs = desc_k(smem_u32(sh.smem + C::OFF_A) + C::TILE_BYTES);
       const uint32_t ring = smem_u32(sh.smem + C::OFF_RING);
       auto stage = [&](uint32_t si) { return ring + (si % ST) * C::TILE_BYTES; };
       uint32_t it = 0, ri = 0;
       bool ok = true;
-      for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, err, 0x3208); ++k) {
+      for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, 0x3208); ++k) {
         const DkvUnit f = dkv_unit(prm, u);
         const uint16_t* list = sh.lists + (k & 1) * kMaxList;
         if (f.n > 0) {
           // waits for slot si (and clears rows of padding: their products with 0 must be 0)
           auto arrived = [&](uint32_t si, int tt, int code) {
-            if (!warp_wait(&sh.full[si % ST], (si / ST) & 1, sh.abort_flag, err, code)) return false;
+            if (!wait_for(&sh.full[si % ST], (si / ST) & 1, sh.abort_flag, code)) return false;
             if (p.has_docs && (list[tt] & kEntScrub)) {
               const int r0 = int(list[tt] & kEntTile) * TILE;
               scrub_rows<D>(stage(si), p.qdoc + (size_t)f.b * p.sq + r0, p.sq - r0, lane);
@@ -313,64 +315,54 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
             return true;
           };
           int t = f.i0 % f.nl;
-          ok = warp_wait(sh.res_full, ri & 1, sh.abort_flag, err, 0x3201) && arrived(2 * it, t, 0x3202) &&
+          ok = wait_for(sh.res_full, ri & 1, sh.abort_flag, 0x3201) && arrived(2 * it, t, 0x3202) &&
                arrived(2 * it + 1, t, 0x3203);
           if (!ok) break;
           ++ri;
           tc_fence_after();
-          if (lane == 0) {
-            mma_kk<D>(t_st, ks, stage(2 * it), id_s);
-            umma_commit(&sh.s_full[0]);
-            mma_kk<D>(t_dp, vs, stage(2 * it + 1), id_s);
-            umma_commit(sh.dp_full);
-            if (f.n == 1) umma_commit(sh.res_empty);
-          }
-          __syncwarp();
+          mma_kk<D>(one, t_st, ks, desc_k(stage(2 * it)), id_s);
+          commit1(one, &sh.s_full[0]);
+          mma_kk<D>(one, t_dp, vs, desc_k(stage(2 * it + 1)), id_s);
+          commit1(one, sh.dp_full);
+          if (f.n == 1) commit1(one, sh.res_empty);
           for (int i = 0; i < f.n; ++i, ++it) {
             const bool more = i + 1 < f.n;
             if (++t == f.nl) t = 0;
             if (more && !(ok = arrived(2 * it + 2, t, 0x3204))) break;
-            if (!(ok = warp_wait(sh.p_ready, it & 1, sh.abort_flag, err, 0x3205))) break;
+            if (!(ok = wait_for(sh.p_ready, it & 1, sh.abort_flag, 0x3205))) break;
             tc_fence_after();
-            if (lane == 0) {
-              mma_tn<D>(t_dv, t_st, t_st + 64, stage(2 * it + 1), id_g, i > 0);
-              umma_commit(&sh.empty[(2 * it + 1) % ST]);
-              if (more) {
-                mma_kk<D>(t_st, ks, stage(2 * it + 2), id_s);
-                umma_commit(&sh.s_full[0]);
-              }
+            mma_tn<D>(one, t_dv, t_st, t_st + 64, desc_mn(stage(2 * it + 1)), id_g, i > 0);
+            commit1(one, &sh.empty[(2 * it + 1) % ST]);
+            if (more) {
+              mma_kk<D>(one, t_st, ks, desc_k(stage(2 * it + 2)), id_s);
+              commit1(one, &sh.s_full[0]);
             }
-            __syncwarp();
             if (more && !(ok = arrived(2 * it + 3, t, 0x3206))) break;
-            if (!(ok = warp_wait(sh.ds_ready, it & 1, sh.abort_flag, err, 0x3207))) break;
+            if (!(ok = wait_for(sh.ds_ready, it & 1, sh.abort_flag, 0x3207))) break;
             tc_fence_after();
-            if (lane == 0) {
-              mma_tn<D>(t_dk, t_dp, t_dp + 64, stage(2 * it), id_g, i > 0);
-              umma_commit(&sh.empty[(2 * it) % ST]);
-              if (more) {
-                mma_kk<D>(t_dp, vs, stage(2 * it + 3), id_s);
-                umma_commit(sh.dp_full);
-                if (i + 2 == f.n) umma_commit(sh.res_empty);
-              } else {
-                umma_commit(sh.done);
-              }
+            mma_tn<D>(one, t_dk, t_dp, t_dp + 64, desc_mn(stage(2 * it)), id_g, i > 0);
+            commit1(one, &sh.empty[(2 * it) % ST]);
+            if (more) {
+              mma_kk<D>(one, t_dp, vs, desc_k(stage(2 * it + 3)), id_s);
+              commit1(one, sh.dp_full);
+              if (i + 2 == f.n) commit1(one, sh.res_empty);
+            } else {
+              commit1(one, sh.done);
             }
-            __syncwarp();
           }
           if (!ok) break;
         }
         unit_done(sh.sched, k);
       }
       // no commit may arrive after the block has left
-      if (lane == 0) umma_commit(sh.all_done);
-      __syncwarp();
-      warp_wait(sh.all_done, 0, sh.abort_flag, err, 0x3209);
+      commit1(one, sh.all_done);
+      wait_for(sh.all_done, 0, sh.abort_flag, 0x3209);
     } else if (warp == 10) {
       // -------------------------------------------------------------- units and their lists
-      run_scheduler(sh.sched, sh.abort_flag, err, 0x3401, [&](int x, int y, int z, uint32_t slot) {
+      run_scheduler(sh.sched, sh.abort_flag, 0x3401, [&](int x, int y, int z, uint32_t slot) {
         if (!p.has_docs) return 0;
         const DkvUnit f = dkv_unit(prm, Unit{x, y, z, 0});
-        const DocRange kd = prm.c.krange[(size_t)f.b * prm.n_kt + x / p.Hkv];
+        const DocRange kd = prm.c.krange[(size_t)f.b * prm.n_kt + f.j0 / TILE];
         int n = 0;
         for (int t = f.t_lo; t < p.n_tiles; t += 32) {
           int st = kStSkip;
@@ -396,7 +388,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
     const bool biased = p.slopes != nullptr;
     uint32_t it = 0, di = 0;
     bool ok = true;
-    for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, err, 0x3305); ++k) {
+    for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, 0x3305); ++k) {
       const DkvUnit f = dkv_unit(prm, u);
       const uint16_t* list = sh.lists + (k & 1) * kMaxList;
       const int j = f.j0 + int(warp & 3) * 32 + int(lane);
@@ -426,8 +418,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
         }
         const float slope2 = biased ? __ldg(p.slopes + f.kvh * p.G + g) * kLog2e : 0.f;
         const float dist0 = float(r0 + p.off - j);
-        ok = warp_wait(&sh.s_full[0], it & 1, sh.abort_flag, err, 0x3301) &&
-             warp_wait(&sh.full[(2 * it) % ST], ((2 * it) / ST) & 1, sh.abort_flag, err, 0x3302);
+        ok = wait_for(&sh.s_full[0], it & 1, sh.abort_flag, 0x3301) &&
+             wait_for(&sh.full[(2 * it) % ST], ((2 * it) / ST) & 1, sh.abort_flag, 0x3302);
         if (!ok) break;
         tc_fence_after();
         uint32_t w[2][32];   // scores, then what ds is multiplied by
@@ -472,7 +464,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
         __syncwarp();
         if (lane == 0) mbar_arrive(sh.p_ready);
 
-        ok = warp_wait(sh.dp_full, it & 1, sh.abort_flag, err, 0x3303);
+        ok = wait_for(sh.dp_full, it & 1, sh.abort_flag, 0x3303);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -505,7 +497,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
       if (!ok) break;
       // ---- epilogue: warps 0-3 write dv, warps 4-7 dk
       if (f.n > 0) {
-        ok = warp_wait(sh.done, di & 1, sh.abort_flag, err, 0x3304);
+        ok = wait_for(sh.done, di & 1, sh.abort_flag, 0x3304);
         if (!ok) break;
         ++di;
       }
@@ -546,7 +538,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
       unit_done(sh.sched, k);
     }
   }
-  bwd_end(tmem);
+  bwd_end(sh, tmem, p.err);
 }
 
 // Sums the splits of dk and dv, in order.  D / 4 lanes a row of one of the two.
@@ -576,10 +568,10 @@ struct DqUnit {
 __device__ __forceinline__ DqUnit dq_unit(const BwdParams& prm, const Unit& u) {
   const Params& p = prm.c;
   DqUnit f;
-  const int qt = p.n_tiles - 1 - u.x / p.H;   // later queries see more: first
-  f.h = u.x % p.H;
+  const int blk = prm.divH.div(u.x), qt = p.n_tiles - 1 - blk;   // later queries see more: first
+  f.h = u.x - blk * p.H;
   f.b = u.y;
-  f.kvh = f.h / p.G;
+  f.kvh = p.divG.div(f.h);
   f.r0 = qt * TILE;
   f.r1 = min(p.sq, f.r0 + TILE) - 1;
   f.pre = p.prefix ? __ldg(p.prefix + f.b) : 0;
@@ -600,7 +592,6 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
   const BwdShared sh = bwd_shared<D>(smem_raw);
   const Params& p = prm.c;
   const uint32_t warp = warp_id(), lane = lane_id();
-  int* err = p.err;
   const uint32_t tmem = bwd_begin(sh, ST, &tm_q, &tm_do, &tm_k, &tm_v);
   const uint32_t t_dp = tmem + 2 * TILE, t_dq = tmem + 3 * TILE;
   Unit u;
@@ -610,12 +601,12 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
     if (warp == 8) {
       // -------------------------------------------------------------- producer
       uint32_t it = 0, ri = 0;
-      for (uint32_t k = 0; next_unit(sh.sched, k, u, sh.abort_flag, err, 0x4103); ++k) {
+      for (uint32_t k = 0; next_unit(sh.sched, k, u, sh.abort_flag, 0x4103); ++k) {
         const DqUnit f = dq_unit(prm, u);
         const uint16_t* list = sh.lists + (k & 1) * kMaxList;
         bool ok = true;
         if (f.n > 0) {
-          ok = warp_wait(sh.res_empty, (ri & 1) ^ 1, sh.abort_flag, err, 0x4102);
+          ok = wait_for(sh.res_empty, (ri & 1) ^ 1, sh.abort_flag, 0x4102);
           if (!ok) break;
           ++ri;
           if (lane == 0) {
@@ -630,7 +621,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
           const int j0 = (p.has_docs ? int(list[i] & kEntTile) : i) * TILE;
           for (int m = 0; m < 2; ++m) {
             const uint32_t s = (2 * it + m) % ST;
-            ok = warp_wait(&sh.empty[s], (((2 * it + m) / ST) & 1) ^ 1, sh.abort_flag, err, 0x4101);
+            ok = wait_for(&sh.empty[s], (((2 * it + m) / ST) & 1) ^ 1, sh.abort_flag, 0x4101);
             if (!ok) break;
             if (lane == 0) {
               mbar_arrive_expect_tx(&sh.full[s], C::TILE_BYTES);
@@ -645,10 +636,10 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         unit_done(sh.sched, k);
       }
       if (lane == 0) {
-        if (ri) mbar_drain(sh.res_full, (ri - 1) & 1, err, 0x4111);
+        if (ri) mbar_drain(sh.res_full, (ri - 1) & 1, p.err, 0x4111);
         for (uint32_t k = 0; k < uint32_t(ST) && k < 2 * it; ++k) {
           const uint32_t i = 2 * it - 1 - k;
-          mbar_drain(&sh.full[i % ST], (i / ST) & 1, err, 0x4112);
+          mbar_drain(&sh.full[i % ST], (i / ST) & 1, p.err, 0x4112);
         }
       }
       __syncwarp();
@@ -656,18 +647,19 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
       // -------------------------------------------------------------- tensor cores
       constexpr uint32_t id_s = idesc16(F16, TILE, TILE, false, false);
       constexpr uint32_t id_g = idesc16(F16, TILE, D, false, true);
-      const uint32_t qs = smem_u32(sh.smem + C::OFF_A), dos = qs + C::TILE_BYTES;
+      const bool one = elect_one();
+      const uint64_t qs = desc_k(smem_u32(sh.smem + C::OFF_A)), dos = desc_k(smem_u32(sh.smem + C::OFF_A) + C::TILE_BYTES);
       const uint32_t ring = smem_u32(sh.smem + C::OFF_RING);
       auto stage = [&](uint32_t si) { return ring + (si % ST) * C::TILE_BYTES; };
       uint32_t it = 0, ri = 0;
       bool ok = true;
-      for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, err, 0x4208); ++k) {
+      for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, 0x4208); ++k) {
         const DqUnit f = dq_unit(prm, u);
         const uint16_t* list = sh.lists + (k & 1) * kMaxList;
         if (f.n > 0) {
           auto arrived = [&](int i, int m, int code) {   // key (m = 0) or value tile of the unit's item i
             const uint32_t si = 2 * (it + i) + m;
-            if (!warp_wait(&sh.full[si % ST], (si / ST) & 1, sh.abort_flag, err, code)) return false;
+            if (!wait_for(&sh.full[si % ST], (si / ST) & 1, sh.abort_flag, code)) return false;
             return true;
           };
           auto scrub = [&](int i, uint32_t si) {
@@ -676,53 +668,44 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
               scrub_rows<D>(stage(si), p.kdoc + (size_t)f.b * p.skv + j0, p.skv - j0, lane);
             }
           };
-          ok = warp_wait(sh.res_full, ri & 1, sh.abort_flag, err, 0x4201) && arrived(0, 0, 0x4202) &&
+          ok = wait_for(sh.res_full, ri & 1, sh.abort_flag, 0x4201) && arrived(0, 0, 0x4202) &&
                arrived(0, 1, 0x4203) && (f.n < 2 || arrived(1, 0, 0x4204));
           if (!ok) break;
           ++ri;
           scrub(0, 2 * it);
           if (f.n > 1) scrub(1, 2 * it + 2);
           tc_fence_after();
-          if (lane == 0) {
-            mma_kk<D>(tmem + (it & 1) * TILE, qs, stage(2 * it), id_s);
-            umma_commit(&sh.s_full[it & 1]);
-            mma_kk<D>(t_dp, dos, stage(2 * it + 1), id_s);
-            umma_commit(sh.dp_full);
-            umma_commit(&sh.empty[(2 * it + 1) % ST]);
-            if (f.n > 1) {
-              mma_kk<D>(tmem + ((it + 1) & 1) * TILE, qs, stage(2 * it + 2), id_s);
-              umma_commit(&sh.s_full[(it + 1) & 1]);
-            } else {
-              umma_commit(sh.res_empty);
-            }
+          mma_kk<D>(one, tmem + (it & 1) * TILE, qs, desc_k(stage(2 * it)), id_s);
+          commit1(one, &sh.s_full[it & 1]);
+          mma_kk<D>(one, t_dp, dos, desc_k(stage(2 * it + 1)), id_s);
+          commit1(one, sh.dp_full);
+          commit1(one, &sh.empty[(2 * it + 1) % ST]);
+          if (f.n > 1) {
+            mma_kk<D>(one, tmem + ((it + 1) & 1) * TILE, qs, desc_k(stage(2 * it + 2)), id_s);
+            commit1(one, &sh.s_full[(it + 1) & 1]);
+          } else {
+            commit1(one, sh.res_empty);
           }
-          __syncwarp();
           for (int i = 0; i < f.n; ++i, ++it) {
             if (i + 1 < f.n && !(ok = arrived(1, 1, 0x4205))) break;
-            if (!(ok = warp_wait(sh.ds_ready, it & 1, sh.abort_flag, err, 0x4206))) break;
+            if (!(ok = wait_for(sh.ds_ready, it & 1, sh.abort_flag, 0x4206))) break;
             tc_fence_after();
             const uint32_t t_s = tmem + (it & 1) * TILE;
-            if (lane == 0) {
-              if (i + 1 < f.n) {
-                mma_kk<D>(t_dp, dos, stage(2 * it + 3), id_s);
-                umma_commit(sh.dp_full);
-                umma_commit(&sh.empty[(2 * it + 3) % ST]);
-                if (i + 2 == f.n) umma_commit(sh.res_empty);   // the last scores were issued before
-              }
-              mma_tn<D>(t_dq, t_s, t_s + 64, stage(2 * it), id_g, i > 0);
-              umma_commit(&sh.empty[(2 * it) % ST]);
-              if (i + 1 == f.n) umma_commit(sh.done);
+            if (i + 1 < f.n) {
+              mma_kk<D>(one, t_dp, dos, desc_k(stage(2 * it + 3)), id_s);
+              commit1(one, sh.dp_full);
+              commit1(one, &sh.empty[(2 * it + 3) % ST]);
+              if (i + 2 == f.n) commit1(one, sh.res_empty);   // the last scores were issued before
             }
-            __syncwarp();
+            mma_tn<D>(one, t_dq, t_s, t_s + 64, desc_mn(stage(2 * it)), id_g, i > 0);
+            commit1(one, &sh.empty[(2 * it) % ST]);
+            if (i + 1 == f.n) commit1(one, sh.done);
             if (i + 2 < f.n) {
               if (!(ok = arrived(2, 0, 0x4207))) break;
               scrub(i + 2, 2 * it + 4);
               tc_fence_after();
-              if (lane == 0) {
-                mma_kk<D>(t_s, qs, stage(2 * it + 4), id_s);
-                umma_commit(&sh.s_full[it & 1]);
-              }
-              __syncwarp();
+              mma_kk<D>(one, t_s, qs, desc_k(stage(2 * it + 4)), id_s);
+              commit1(one, &sh.s_full[it & 1]);
             }
           }
           if (!ok) break;
@@ -730,12 +713,11 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         unit_done(sh.sched, k);
       }
       // no commit may arrive after the block has left
-      if (lane == 0) umma_commit(sh.all_done);
-      __syncwarp();
-      warp_wait(sh.all_done, 0, sh.abort_flag, err, 0x4209);
+      commit1(one, sh.all_done);
+      wait_for(sh.all_done, 0, sh.abort_flag, 0x4209);
     } else if (warp == 10) {
       // -------------------------------------------------------------- units and their lists
-      run_scheduler(sh.sched, sh.abort_flag, err, 0x4401, [&](int x, int y, int z, uint32_t slot) {
+      run_scheduler(sh.sched, sh.abort_flag, 0x4401, [&](int x, int y, int z, uint32_t slot) {
         if (!p.has_docs) return 0;
         const DqUnit f = dq_unit(prm, Unit{x, y, z, 0});
         const DocRange qd = p.qrange[(size_t)f.b * p.n_tiles + f.r0 / TILE];
@@ -765,7 +747,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
     const bool biased = p.slopes != nullptr;
     uint32_t it = 0, di = 0;
     bool ok = true;
-    for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, err, 0x4304); ++k) {
+    for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, 0x4304); ++k) {
       const DqUnit f = dq_unit(prm, u);
       const uint16_t* list = sh.lists + (k & 1) * kMaxList;
       const int row = f.r0 + int(warp & 3) * 32 + int(lane);
@@ -795,7 +777,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
 #pragma unroll
           for (int y = 0; y < 2; ++y) see[y] &= low_bits(lim - j0 - y * 32);
         }
-        ok = warp_wait(&sh.s_full[it & 1], (it >> 1) & 1, sh.abort_flag, err, 0x4301);
+        ok = wait_for(&sh.s_full[it & 1], (it >> 1) & 1, sh.abort_flag, 0x4301);
         if (!ok) break;
         tc_fence_after();
         uint32_t w[2][32];
@@ -823,7 +805,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         // masked scores are taken out of ds below
         if (biased) phase(std::true_type{});
         else phase(std::false_type{});
-        ok = warp_wait(sh.dp_full, it & 1, sh.abort_flag, err, 0x4302);
+        ok = wait_for(sh.dp_full, it & 1, sh.abort_flag, 0x4302);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -851,7 +833,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
       if (!ok) break;
       // ---- epilogue: each half of the warps writes half of the columns
       if (f.n > 0) {
-        ok = warp_wait(sh.done, di & 1, sh.abort_flag, err, 0x4303);
+        ok = wait_for(sh.done, di & 1, sh.abort_flag, 0x4303);
         if (!ok) break;
         ++di;
       }
@@ -877,7 +859,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
       unit_done(sh.sched, k);
     }
   }
-  bwd_end(tmem);
+  bwd_end(sh, tmem, p.err);
 }
 
 }  // namespace fused

@@ -16,6 +16,17 @@ constexpr int kMaxList = 2048;   // documents: tiles of one unit at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// Division by a number known to the host, exact for 0 <= n < 2^31: with 2^shift >= d the
+// multiplier ceil(2^(32 + shift) / d) has 33 bits, of which mul holds the lower 32.
+struct FastDiv {
+  uint32_t mul, shift, d;
+  __device__ __forceinline__ int div(int n) const {
+    if (d == 1) return n;
+    const uint32_t h = __umulhi(uint32_t(n), mul);
+    return int((h + ((uint32_t(n) - h) >> 1)) >> (shift - 1));
+  }
+};
+
 struct DocRange;
 
 struct Params {
@@ -24,7 +35,8 @@ struct Params {
   int causal, has_docs;
   float scale;             // of the scores
   float scale_log2;        // scale * log2(e)
-  float cap_in;            // softcap: 2 * log2(e) * scale / softcap
+  float cap_u;             // softcap: scale / softcap
+  float cap_in;            // 2 * log2(e) * scale / softcap
   float cap_out;           // softcap * log2(e)
   const float* slopes;     // [H] or null
   const int* prefix;       // [bs] or null
@@ -32,8 +44,43 @@ struct Params {
   const DocRange *qrange, *krange;   // of the 128-position tiles, [bs, tiles]
   int n_tiles;             // tiles of the axis a CTA loops over
   int splits, tiles_per_split;
+  FastDiv divG;            // heads of a group
   int* err;
 };
+
+// Bounded wait of a warp on an mbarrier phase, kept small in code: it occurs some twenty times a
+// kernel, and the kernels' units are short enough for instruction fetches to count.  Gives up
+// after kWaitLimitNs (or when another warp of the block has) and leaves its code in the block's
+// flag, which report_error() passes on at the end.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* flag, int code) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P, Q;\n\t.reg .u64 t0, t1;\n\t.reg .u32 f;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "@P bra DONE;\n\t"
+      "mov.u64 t0, %%globaltimer;\n"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+      "@P bra DONE;\n\t"
+      "ld.volatile.shared.u32 f, [%4];\n\t"
+      "setp.ne.u32 Q, f, 0;\n\t"
+      "@Q bra DONE;\n\t"
+      "mov.u64 t1, %%globaltimer;\n\t"
+      "sub.u64 t1, t1, t0;\n\t"
+      "setp.lt.u64 Q, t1, %5;\n\t"
+      "@Q bra AGAIN;\n\t"
+      "st.volatile.shared.u32 [%4], %6;\n"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendHintNs), "r"(smem_u32(const_cast<int*>(flag))), "l"(kWaitLimitNs),
+        "r"(code)
+      : "memory");
+  return __all_sync(0xffffffffu, ok != 0);
+}
+__device__ __forceinline__ void report_error(volatile int* flag, int* err) {
+  if (threadIdx.x == 0 && *flag) raise_error(err, *flag);
+}
 
 // Number of keys (from key 0) that query row `r` of batch row b sees when documents are left
 // out of account: a prefix, then causal.  Never above skv; 0 or less: none.
@@ -148,13 +195,13 @@ __device__ __forceinline__ void scheduler_init(const Scheduler& s) {
 }
 // The scheduler warp.  build(unit, slot) -> n prepares a unit's list (one warp).
 template <typename F>
-__device__ __forceinline__ void run_scheduler(const Scheduler& s, volatile int* abort, int* err, int code, F build) {
+__device__ __forceinline__ void run_scheduler(const Scheduler& s, volatile int* abort, int code, F build) {
   const uint32_t lane = lane_id();
   int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z;
   bool have = true;
   for (uint32_t k = 0;; ++k) {
     const uint32_t i = k & 1;
-    if (!warp_wait(&s.empty[i], ((k >> 1) & 1) ^ 1, abort, err, code)) return;
+    if (!wait_for(&s.empty[i], ((k >> 1) & 1) ^ 1, abort, code)) return;
     const int n = have ? build(x, y, z, i) : 0;
     __syncwarp();
     if (lane == 0) {
@@ -163,21 +210,20 @@ __device__ __forceinline__ void run_scheduler(const Scheduler& s, volatile int* 
     }
     if (!have) return;
     // not earlier: a CTA that took its next unit at once would hold it while others run dry
-    if (!warp_wait(s.ask, k & 1, abort, err, code + 2)) return;
+    if (!wait_for(s.ask, k & 1, abort, code + 2)) return;
     if (lane == 0) {
       mbar_arrive_expect_tx(s.answer, 16);
       ask_next(s);
     }
-    if (!warp_wait(s.answer, k & 1, abort, err, code + 1)) return;
+    if (!wait_for(s.answer, k & 1, abort, code + 1)) return;
     have = read_answer(s, x, y, z);
     fence_proxy_async_smem();   // the next answer is written by the async proxy
     __syncwarp();
   }
 }
 // A reader's next unit; false: none left (or the kernel gives up).
-__device__ __forceinline__ bool next_unit(const Scheduler& s, uint32_t k, Unit& u, volatile int* abort, int* err,
-                                          int code) {
-  if (!warp_wait(&s.full[k & 1], (k >> 1) & 1, abort, err, code)) return false;
+__device__ __forceinline__ bool next_unit(const Scheduler& s, uint32_t k, Unit& u, volatile int* abort, int code) {
+  if (!wait_for(&s.full[k & 1], (k >> 1) & 1, abort, code)) return false;
   u = s.slot[k & 1];
   return u.x >= 0;
 }
@@ -264,6 +310,29 @@ __device__ __forceinline__ void cap_r4(float (&z)[4]) {
   z[3] = icd * a[2];
 }
 
+// tanh of pairs with |u| <= 0.75: u + u^3 (c0 + c1 u^2 + ..), fitted by Remez exchange (largest
+// relative error 3.3e-8).  Capped layers rarely come near their cap, and this needs no special
+// function: the warps of a tile whose scores all stay below take it.
+constexpr float kTanhSmall = 0.75f;
+struct TanhSmall {
+  uint64_t c[5];
+  // kept in registers (a volatile move is not repeated where the constants are used)
+  __device__ __forceinline__ TanhSmall() {
+    const float v[5] = {-0.3333306908607483f, 0.13326521217823029f, -0.0533902570605278f, 0.019664913415908813f,
+                        -0.0047694905661046505f};
+#pragma unroll
+    for (int i = 0; i < 5; ++i) asm volatile("mov.b64 %0, {%1, %1};" : "=l"(c[i]) : "f"(v[i]));
+  }
+  __device__ __forceinline__ uint64_t operator()(uint64_t u) const {
+    const uint64_t u2 = f2_mul(u, u);
+    uint64_t p = f2_fma(c[4], u2, c[3]);
+    p = f2_fma(p, u2, c[2]);
+    p = f2_fma(p, u2, c[1]);
+    p = f2_fma(p, u2, c[0]);
+    return f2_fma(f2_mul(p, u2), u, u);
+  }
+};
+
 // Which of 32 ids per word (this lane holds ids[k * 32 + lane] in v[k]) equal this lane's own id:
 // one ballot a word for each different id of the warp's rows, usually one or two.
 template <int N>
@@ -288,37 +357,61 @@ __host__ __device__ constexpr uint32_t idesc16(bool f16, int M, int N, bool a_mn
   return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
          (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
-// D[tmem] (+)= A[tmem] * B[smem]^T: A holds 16-bit pairs along K, one 32-bit column a pair.
-__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                        uint32_t accumulate) {
+// The products below are called by a whole warp with `one` set in the lane that issues them (always
+// the same one), not from a branch of that lane: descriptors then stay in uniform registers and are
+// stepped by one addition, where a divergent branch moves each of them there and the issue of
+// small products, not the tensor cores, sets the pace (measured: see mma_kk).
+__device__ __forceinline__ void umma_ss1(bool one, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate));
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(uint32_t(one)));
 }
+// D[tmem] (+)= A[tmem] * B[smem]^T: A holds 16-bit pairs along K, one 32-bit column a pair.
+__device__ __forceinline__ void umma_ts1(bool one, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(uint32_t(one)));
+}
+__device__ __forceinline__ void commit1(bool one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(uint32_t(one))
+      : "memory");
+}
+// Descriptor of a tile read along its rows (K-major), and of one read across them (MN-major).
+// An offset of o bytes adds o / 16.
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile) { return sdesc_sw128(tile, 16, 1024); }
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile) { return sdesc_sw128(tile, TILE * 128, 1024); }
 
-// Product of a K-major A tile [128 x D] and a K-major B tile [128 x D]: D[128 x 128].
-// Tiles are D / 64 blocks of [128 rows x 128 bytes], 128-byte swizzled.
+// Product of a K-major A tile [128 x D] and a K-major B tile [128 x D] (or, with idesc for
+// N = 64, its first 64 rows): D[128 x N].  Tiles are D / 64 blocks of [128 rows x 128 bytes],
+// 128-byte swizzled.
 template <int D>
-__device__ __forceinline__ void mma_kk(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_kk(bool one, uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
-    const uint32_t o = (kk >> 2) * (TILE * 128) + (kk & 3) * 32;
-    umma_bf16(d_tmem, sdesc_sw128(a + o, 16, 1024), sdesc_sw128(b + o, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+    const uint32_t o = ((kk >> 2) * (TILE * 128) + (kk & 3) * 32) >> 4;
+    umma_ss1(one, d_tmem, a + o, b + o, idesc, kk > 0 ? 1u : 0u);
   }
 }
 // Product of A [128 x 128] in TMEM (columns a0.. for the first 64 of K, a1.. for the second) and a
-// tile [128 rows x D] whose rows are K: D[128 x D] (+)=.  kk: steps [k0, k1) of 16 rows.
-template <int D>
-__device__ __forceinline__ void mma_tn(uint32_t d_tmem, uint32_t a0, uint32_t a1, uint32_t b, uint32_t idesc,
-                                       bool accumulate, int k0 = 0, int k1 = 8) {
+// tile [128 rows x D] whose rows are K: D[128 x D] (+)=.  Steps [K0, K1) of 16 rows.
+template <int D, int K0 = 0, int K1 = 8>
+__device__ __forceinline__ void mma_tn(bool one, uint32_t d_tmem, uint32_t a0, uint32_t a1, uint64_t b, uint32_t idesc,
+                                       bool accumulate) {
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk) {
-    if (kk < k0 || kk >= k1) continue;
-    const uint32_t at = (kk < 4 ? a0 : a1) + (kk & 3) * 8;
-    umma_ts(d_tmem, at, sdesc_sw128(b + kk * 2048, TILE * 128, 1024), idesc, (accumulate || kk > 0) ? 1u : 0u);
-  }
+  for (int kk = K0; kk < K1; ++kk)
+    umma_ts1(one, d_tmem, (kk < 4 ? a0 : a1) + (kk & 3) * 8, b + kk * (2048 >> 4), idesc, (accumulate || kk > 0) ? 1u : 0u);
 }
 
 // Clears the rows of a [128 x D] tile whose document is negative (or that lie behind the

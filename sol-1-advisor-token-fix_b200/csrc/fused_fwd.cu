@@ -24,6 +24,7 @@ static FwdParams plan_fwd(const attn_bwd_fused_t* a, int sm_count) {
   // nothing at the diagonal; an odd group takes 256 positions of a head instead
   f.pair_heads = !f.packed && p.G % 2 == 0;
   f.head_slots = f.packed ? p.Hkv : f.pair_heads ? p.H / 2 : p.H;
+  f.div_slots = fast_div(f.head_slots);
   const int pos_per_unit = f.packed ? 2 * ppt : f.pair_heads ? TILE : 2 * TILE;
   f.blocks_q = (p.sq + pos_per_unit - 1) / pos_per_unit;
   p.n_tiles = (p.skv + TILE - 1) / TILE;

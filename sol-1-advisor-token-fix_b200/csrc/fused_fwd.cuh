@@ -10,7 +10,8 @@
 // first scores computed while this one's rows are still written.
 // TMEM: two score tiles (128 columns each) and two outputs (D columns each).  The weights go
 // back to TMEM as 16-bit pairs over the scores they came from and are the A operand of the
-// second product, so they never touch shared memory.
+// second product, so they never touch shared memory.  They are handed over in two halves, so
+// the second product starts while the second half is still computed.
 //
 // The running maximum lags: the accumulator is rescaled only where a row's maximum has grown by
 // more than 2^8, so most tiles need no pass over it.  Weights are then at most 2^8 instead of
@@ -32,6 +33,7 @@ struct FwdParams {
   int pair_heads;      // unpacked: the two tiles are two heads of one group, else 256 positions
   int blocks_q;        // position blocks per (batch, head slot)
   int head_slots;      // units along the heads: kv heads, head pairs or heads
+  FastDiv div_slots;
   void* o;             // [bs, sq, H, D]
   float* lse;          // [bs, H, sq]
   float* part_o;       // splits > 1: [split][bs * H * sq][D]
@@ -48,7 +50,7 @@ struct FwdCfg {
   static constexpr int OFF_LIST = OFF_STAGE + 8 * 2048;        // a list for each unit slot
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;            // two slots, the scheduler's answer
-  static constexpr int NBAR = 3 + 2 * ST + 6 + 6;
+  static constexpr int NBAR = 3 + 2 * ST + 8 + 6;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int SMEM_BYTES = OFF_MISC + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024, "forward kernel shared memory");
@@ -66,8 +68,9 @@ __device__ __forceinline__ FwdUnit fwd_unit(const FwdParams& prm, const Unit& u)
   const Params& p = prm.c;
   FwdUnit f;
   // later positions see more keys and come first
-  const int qb = prm.blocks_q - 1 - u.x / prm.head_slots;
-  const int slot = u.x % prm.head_slots;
+  const int blk = prm.div_slots.div(u.x);
+  const int qb = prm.blocks_q - 1 - blk;
+  const int slot = u.x - blk * prm.head_slots;
   f.b = u.y;
   f.split = u.z;
   if (prm.packed) {
@@ -78,11 +81,11 @@ __device__ __forceinline__ FwdUnit fwd_unit(const FwdParams& prm, const Unit& u)
   } else if (prm.pair_heads) {
     f.head[0] = slot * 2;
     f.head[1] = slot * 2 + 1;
-    f.kvh = f.head[0] / p.G;
+    f.kvh = p.divG.div(f.head[0]);
     f.pos[0] = f.pos[1] = qb * TILE;
   } else {
     f.head[0] = f.head[1] = slot;
-    f.kvh = slot / p.G;
+    f.kvh = p.divG.div(slot);
     f.pos[0] = qb * 2 * TILE;
     f.pos[1] = f.pos[0] + TILE;
   }
@@ -110,9 +113,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
   uint64_t* all_done = bars + 2;
   uint64_t* kv_full = bars + 3;
   uint64_t* kv_empty = kv_full + ST;
-  uint64_t* s_full = kv_empty + ST;    // [2] scores ready
-  uint64_t* p_ready = s_full + 2;      // [2] weights written
-  uint64_t* o_done = p_ready + 2;      // [2] second product done
+  uint64_t* s_full = kv_empty + ST;    // [tile] scores ready
+  uint64_t* p_ready = s_full + 2;      // [tile][half] weights written
+  uint64_t* o_done = p_ready + 4;      // [tile] second product done
   Scheduler sched;
   sched.slot = reinterpret_cast<Unit*>(smem + C::OFF_UNIT);
   sched.handle = smem_u32(smem + C::OFF_UNIT + 32);
@@ -126,13 +129,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
 
   const Params& p = prm.c;
   const uint32_t warp = warp_id(), lane = lane_id();
-  int* err = p.err;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     mbar_init(all_done, 1);
     for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_done[i], 1); }
+    for (int i = 0; i < 4; ++i) mbar_init(&p_ready[i], 4);
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&o_done[i], 1); }
     scheduler_init(sched);
     *abort_flag = 0;
     fence_barrier_init();
@@ -154,12 +157,12 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     if (warp == 8) {
       // -------------------------------------------------------------- producer
       uint32_t si = 0, qi = 0;   // key / value tiles, query tiles loaded so far
-      for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, err, 0x2103); ++k) {
+      for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, 0x2103); ++k) {
         const FwdUnit f = fwd_unit(prm, u);
         const uint16_t* list = lists + (k & 1) * kMaxList;
         bool ok = true;
         if (f.n > 0) {
-          ok = warp_wait(q_empty, (qi & 1) ^ 1, abort_flag, err, 0x2102);
+          ok = wait_for(q_empty, (qi & 1) ^ 1, abort_flag, 0x2102);
           if (!ok) break;
           ++qi;
           if (lane == 0) {
@@ -176,7 +179,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           const int j0 = (f.t0 + (p.has_docs ? int(list[i] & kEntTile) : i)) * TILE;
           for (int m = 0; m < 2; ++m) {
             const uint32_t s = si % ST;
-            ok = warp_wait(&kv_empty[s], ((si / ST) & 1) ^ 1, abort_flag, err, 0x2101);
+            ok = wait_for(&kv_empty[s], ((si / ST) & 1) ^ 1, abort_flag, 0x2101);
             if (!ok) break;
             if (lane == 0) {
               mbar_arrive_expect_tx(&kv_full[s], C::TILE_BYTES);
@@ -192,39 +195,37 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
         unit_done(sched, k);
       }
       if (lane == 0) {
-        if (qi) mbar_drain(q_full, (qi - 1) & 1, err, 0x2111);
+        if (qi) mbar_drain(q_full, (qi - 1) & 1, p.err, 0x2111);
         for (uint32_t k = 0; k < uint32_t(ST) && k < si; ++k) {
           const uint32_t i = si - 1 - k;
-          mbar_drain(&kv_full[i % ST], (i / ST) & 1, err, 0x2112);
+          mbar_drain(&kv_full[i % ST], (i / ST) & 1, p.err, 0x2112);
         }
       }
       __syncwarp();
     } else if (warp == 9) {
       // -------------------------------------------------------------- tensor cores
+      const bool one = elect_one();
       constexpr uint32_t id_s = idesc16(F16, TILE, TILE, false, false);
       constexpr uint32_t id_o = idesc16(F16, TILE, D, false, true);
       const uint32_t qs = smem_u32(smem + C::OFF_Q), kvs = smem_u32(smem + C::OFF_KV);
       auto stage = [&](uint32_t si) { return kvs + (si % ST) * C::TILE_BYTES; };
       auto full = [&](uint32_t si, int code) {
-        return warp_wait(&kv_full[si % ST], (si / ST) & 1, abort_flag, err, code);
+        return wait_for(&kv_full[si % ST], (si / ST) & 1, abort_flag, code);
       };
       uint32_t si = 0, qi = 0, cnt[2] = {0, 0};
-      for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, err, 0x2206); ++k) {
+      for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, 0x2200); ++k) {
         const FwdUnit f = fwd_unit(prm, u);
         const uint16_t* list = lists + (k & 1) * kMaxList;
         if (f.n > 0) {
-          if (!warp_wait(q_full, qi & 1, abort_flag, err, 0x2201) || !full(si, 0x2202)) break;
+          if (!wait_for(q_full, qi & 1, abort_flag, 0x2201) || !full(si, 0x2202)) break;
           ++qi;
           tc_fence_after();
-          if (lane == 0) {
-            for (int t = 0; t < f.nt; ++t) {
-              mma_kk<D>(tmem + t * TILE, qs + t * C::TILE_BYTES, stage(si), id_s);
-              umma_commit(&s_full[t]);
-            }
-            umma_commit(&kv_empty[si % ST]);
-            if (f.n == 1) umma_commit(q_empty);
+          for (int t = 0; t < f.nt; ++t) {
+            mma_kk<D>(one, tmem + t * TILE, desc_k(qs + t * C::TILE_BYTES), desc_k(stage(si)), id_s);
+            commit1(one, &s_full[t]);
           }
-          __syncwarp();
+          commit1(one, &kv_empty[si % ST]);
+          if (f.n == 1) commit1(one, q_empty);
           bool ok = true;
           for (int i = 0; i < f.n; ++i) {
             const uint32_t vi = si + 1, kn = si + 2;
@@ -236,39 +237,40 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             }
             if (more && !(ok = full(kn, 0x2204))) break;
             for (int t = 0; t < f.nt && ok; ++t) {
-              ok = warp_wait(&p_ready[t], cnt[t] & 1, abort_flag, err, 0x2205);
+              const uint32_t t_s = tmem + t * TILE, t_o = tmem + 2 * TILE + t * D;
+              ok = wait_for(&p_ready[2 * t], (cnt[t] + i) & 1, abort_flag, 0x2205);
               if (!ok) break;
-              ++cnt[t];
               tc_fence_after();
-              if (lane == 0) {
-                mma_tn<D>(tmem + 2 * TILE + t * D, tmem + t * TILE, tmem + t * TILE + 32, stage(vi), id_o, i > 0);
-                umma_commit(&o_done[t]);
-                if (t == f.nt - 1) umma_commit(&kv_empty[vi % ST]);
-                if (more) {
-                  mma_kk<D>(tmem + t * TILE, qs + t * C::TILE_BYTES, stage(kn), id_s);
-                  umma_commit(&s_full[t]);
-                  if (t == f.nt - 1) {
-                    umma_commit(&kv_empty[kn % ST]);
-                    if (i + 2 == f.n) umma_commit(q_empty);
-                  }
+              mma_tn<D, 0, 4>(one, t_o, t_s, t_s + 32, desc_mn(stage(vi)), id_o, i > 0);
+              ok = wait_for(&p_ready[2 * t + 1], (cnt[t] + i) & 1, abort_flag, 0x2206);
+              if (!ok) break;
+              tc_fence_after();
+              mma_tn<D, 4, 8>(one, t_o, t_s, t_s + 32, desc_mn(stage(vi)), id_o, true);
+              commit1(one, &o_done[t]);
+              if (t == f.nt - 1) commit1(one, &kv_empty[vi % ST]);
+              if (more) {
+                mma_kk<D>(one, t_s, desc_k(qs + t * C::TILE_BYTES), desc_k(stage(kn)), id_s);
+                commit1(one, &s_full[t]);
+                if (t == f.nt - 1) {
+                  commit1(one, &kv_empty[kn % ST]);
+                  if (i + 2 == f.n) commit1(one, q_empty);
                 }
               }
-              __syncwarp();
             }
             if (!ok) break;
             si += 2;
           }
           if (!ok) break;
+          for (int t = 0; t < f.nt; ++t) cnt[t] += uint32_t(f.n);
         }
         unit_done(sched, k);
       }
       // no commit may arrive after the block has left
-      if (lane == 0) umma_commit(all_done);
-      __syncwarp();
-      warp_wait(all_done, 0, abort_flag, err, 0x2207);
+      commit1(one, all_done);
+      wait_for(all_done, 0, abort_flag, 0x2207);
     } else if (warp == 10) {
       // -------------------------------------------------------------- units and their lists
-      run_scheduler(sched, abort_flag, err, 0x2401, [&](int x, int y, int z, uint32_t slot) {
+      run_scheduler(sched, abort_flag, 0x2401, [&](int x, int y, int z, uint32_t slot) {
         if (!p.has_docs) return 0;
         const FwdUnit f = fwd_unit(prm, Unit{x, y, z, 0});
         const DocRange qd = warp_doc_range(p.qdoc + (size_t)f.b * p.sq + f.pos[0], f.last_pos - f.pos[0] + 1, lane);
@@ -299,11 +301,12 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     const int row = int(warp & 3) * 32 + int(lane);
     const uint32_t stage = smem_u32(smem + C::OFF_STAGE) + warp * 2048;
     const bool biased = p.slopes != nullptr;
-    const bool raw = !CAP && !biased;                      // raw scores scaled inside the exponent
-    const float c = raw ? p.scale_log2 : 1.f;
+    // without a bias scores stay raw (or a tanh) and are scaled inside the exponent
+    const float c = biased ? 1.f : CAP ? p.cap_out : p.scale_log2;
     const float grow = 8.f / c;
-    uint32_t cnt = 0;
-    for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, err, 0x2304); ++k) {
+    const TanhSmall tanh_small;
+    uint32_t cnt = 0;   // tiles so far
+    for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, 0x2304); ++k) {
       const FwdUnit f = fwd_unit(prm, u);
       if (t >= f.nt) {
         unit_done(sched, k);
@@ -313,7 +316,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
       int pos, head;
       bool valid;
       if (prm.packed) {
-        const int r = row / p.G;
+        const int r = p.divG.div(row);
         pos = (t ? f.pos[1] : f.pos[0]) + r;
         head = f.head[0] + row - r * p.G;
         valid = r < prm.pos_per_tile && pos < p.sq;
@@ -322,12 +325,12 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
         head = t ? f.head[1] : f.head[0];
         valid = pos < p.sq;
       }
-      int lim = valid ? row_limit(p, pos, f.pre) : 0;
+      const int lim = valid ? row_limit(p, pos, f.pre) : 0;
       const int qd = (valid && p.has_docs) ? __ldg(p.qdoc + (size_t)f.b * p.sq + pos) : -1;
       const bool any_valid = __any_sync(0xffffffffu, valid);   // warps of padding rows only pass barriers
       const float slope2 = (biased && valid) ? __ldg(p.slopes + head) * kLog2e : 0.f;
 
-      float mref = -INFINITY;   // reference maximum (raw or log2 units)
+      float mref = -INFINITY;   // reference maximum, in units of 1 / c
       float l = 0.f;
       bool ok = true;
       for (int i = 0; i < f.n; ++i) {
@@ -343,41 +346,57 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             ids[g] = j < p.skv ? __ldg(kdoc + j) : -1;
           }
         }
-        ok = warp_wait(&s_full[t], (cnt + i) & 1, abort_flag, err, 0x2301);
+        ok = wait_for(&s_full[t], (cnt + i) & 1, abort_flag, 0x2301);
         if (!ok) break;
         tc_fence_after();
+        // every completion of o_done is waited for once, so its parity cannot be mistaken
+        bool o_seen = i == 0;
         if (any_valid) {
           uint32_t s[4][32];
 #pragma unroll
           for (int g = 0; g < 4; ++g) tmem_ld32(t_s + g * 32, s[g]);
           tmem_wait_ld();
           if (CAP) {
+            float big = 0.f;
 #pragma unroll
             for (int g = 0; g < 4; ++g)
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                float z[4];
-#pragma unroll
-                for (int y = 0; y < 4; ++y) z[y] = __uint_as_float(s[g][e + y]) * p.cap_in;
-                cap_r4(z);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) s[g][e + y] = __float_as_uint(fmaf(-2.f * p.cap_out, z[y], p.cap_out));
-              }
-          }
-          if (biased) {
-            const float d0 = float(pos + p.off - j0), sl = CAP ? 1.f : p.scale_log2;
-            if (__all_sync(0xffffffffu, pos + p.off >= j0 + TILE - 1)) {   // |i - j| = i - j: linear in the column
-              const uint64_t sl2 = f2(sl, sl), a2 = f2(-slope2 * d0, -slope2 * d0), b2 = f2(slope2, slope2);
+              for (int e = 0; e < 32; e += 2)
+                big = fmaxf(big, fmaxf(fabsf(__uint_as_float(s[g][e])), fabsf(__uint_as_float(s[g][e + 1]))));
+            if (__all_sync(0xffffffffu, big * p.cap_u <= kTanhSmall)) {
+              const uint64_t cu = f2(p.cap_u, p.cap_u);
 #pragma unroll
               for (int g = 0; g < 4; ++g)
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                   float x0, x1;
-                  f2_split(f2_fma(f2(s[g][e], s[g][e + 1]), sl2,
-                                  f2_fma(b2, f2(float(g * 32 + e), float(g * 32 + e + 1)), a2)), x0, x1);
+                  f2_split(tanh_small(f2_mul(f2(s[g][e], s[g][e + 1]), cu)), x0, x1);
                   s[g][e] = __float_as_uint(x0);
                   s[g][e + 1] = __float_as_uint(x1);
                 }
+            } else {
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                  float z[4];
+#pragma unroll
+                  for (int y = 0; y < 4; ++y) z[y] = __uint_as_float(s[g][e + y]) * p.cap_in;
+                  cap_r4(z);
+#pragma unroll
+                  for (int y = 0; y < 4; ++y) s[g][e + y] = __float_as_uint(fmaf(-2.f, z[y], 1.f));
+                }
+            }
+          }
+          if (biased) {
+            const float d0 = float(pos + p.off - j0), sl = CAP ? p.cap_out : p.scale_log2;
+            if (__all_sync(0xffffffffu, pos + p.off >= j0 + TILE - 1)) {   // |i - j| = i - j: linear in the column
+              const float a = -slope2 * d0;
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  s[g][e] = __float_as_uint(fmaf(__uint_as_float(s[g][e]), sl, fmaf(slope2, float(g * 32 + e), a)));
             } else {
 #pragma unroll
               for (int g = 0; g < 4; ++g)
@@ -402,10 +421,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           float mx[4];
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            float x = fmaxf(__uint_as_float(s[g][0]), __uint_as_float(s[g][1]));
+            float y = fmaxf(__uint_as_float(s[g][0]), __uint_as_float(s[g][1]));
 #pragma unroll
-            for (int e = 2; e < 32; e += 2) x = fmaxf(x, fmaxf(__uint_as_float(s[g][e]), __uint_as_float(s[g][e + 1])));
-            mx[g] = x;
+            for (int e = 2; e < 32; e += 2) y = fmaxf(y, fmaxf(__uint_as_float(s[g][e]), __uint_as_float(s[g][e + 1])));
+            mx[g] = y;
           }
           const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (__any_sync(0xffffffffu, m > mref + grow)) {
@@ -414,10 +433,11 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             mref = mnew;
             l *= fac;
             if (i > 0) {
-              ok = warp_wait(&o_done[t], (cnt + i - 1) & 1, abort_flag, err, 0x2302);
+              ok = wait_for(&o_done[t], (cnt + i - 1) & 1, abort_flag, 0x2302);
               if (!ok) break;
+              o_seen = true;
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int x = 0; x < D / 32; ++x) {
                 uint32_t o[2][16];
                 tmem_ld16(t_o + x * 32, o[0]);
@@ -431,6 +451,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
                 tmem_st16(t_o + x * 32, o[0]);
                 tmem_st16(t_o + x * 32 + 16, o[1]);
               }
+              tmem_wait_st();
             }
           }
           const float nm = mref == -INFINITY ? 0.f : -mref * c;
@@ -451,19 +472,31 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
               w[e / 2 + 1] = pack2<F16>(b0, b1);
             }
             tmem_st16(t_s + g * 16, w);
+            if (g == 1) {
+              tmem_wait_st();
+              tc_fence_before();
+              if (!o_seen) ok = wait_for(&o_done[t], (cnt + i - 1) & 1, abort_flag, 0x2305);
+              __syncwarp();
+              if (lane == 0 && ok) mbar_arrive(&p_ready[2 * t]);
+            }
           }
+          if (!ok) break;
           float x0, x1, y0, y1;
           f2_split(sum0, x0, x1);
           f2_split(sum1, y0, y1);
           l += (x0 + x1) + (y0 + y1);
           tmem_wait_st();
+        } else {
+          if (!o_seen) ok = wait_for(&o_done[t], (cnt + i - 1) & 1, abort_flag, 0x2306);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(&p_ready[2 * t]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[t]);
+        if (lane == 0) mbar_arrive(&p_ready[2 * t + 1]);
       }
       // ---- epilogue: o / l, and the row statistic
-      if (ok && f.n > 0) ok = warp_wait(&o_done[t], (cnt + f.n - 1) & 1, abort_flag, err, 0x2303);
+      if (ok && f.n > 0) ok = wait_for(&o_done[t], (cnt + f.n - 1) & 1, abort_flag, 0x2303);
       if (!ok) break;
       cnt += uint32_t(f.n);
       if (any_valid) {
@@ -507,6 +540,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
   }
   tc_fence_before();
   __syncthreads();
+  report_error(abort_flag, p.err);
   if (warp == 9) {
     __syncwarp();
     tc_fence_after();

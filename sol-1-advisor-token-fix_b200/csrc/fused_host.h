@@ -36,6 +36,15 @@ inline int check_args(const attn_bwd_fused_t* a) {
   return ATTN_BWD_OK;
 }
 
+inline FastDiv fast_div(int d) {   // d >= 1
+  FastDiv f;
+  f.d = uint32_t(d);
+  f.shift = 1;
+  while ((1u << f.shift) < uint32_t(d)) ++f.shift;
+  f.mul = uint32_t((((1ull << f.shift) - uint64_t(d)) << 32) / uint64_t(d) + 1);
+  return f;
+}
+
 inline Params base_params(const attn_bwd_fused_t* a) {
   Params p;
   std::memset(&p, 0, sizeof(p));
@@ -50,12 +59,14 @@ inline Params base_params(const attn_bwd_fused_t* a) {
   p.has_docs = a->q_documents ? 1 : 0;
   p.scale = a->scale;
   p.scale_log2 = a->scale * kLog2e;
+  p.cap_u = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
   p.cap_in = a->softcap > 0.f ? 2.f * kLog2e * a->scale / a->softcap : 0.f;
   p.cap_out = a->softcap * kLog2e;
   p.slopes = a->slopes;
   p.prefix = a->prefix_lens;
   p.qdoc = a->q_documents;
   p.kdoc = a->kv_documents;
+  p.divG = fast_div(p.G);
   p.splits = 1;
   return p;
 }
