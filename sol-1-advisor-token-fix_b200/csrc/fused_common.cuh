@@ -333,6 +333,33 @@ struct TanhSmall {
   }
 };
 
+// 32 raw scores to tanh(scale x / softcap), in place, the shorter way if the whole warp's allow it.
+__device__ __forceinline__ void cap32(const Params& p, const TanhSmall& ts, uint32_t (&x)[32]) {
+  float big = 0.f;
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1]))));
+  if (__all_sync(0xffffffffu, big * p.cap_u <= kTanhSmall)) {
+    const uint64_t cu = f2(p.cap_u, p.cap_u);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      float a, b;
+      f2_split(ts(f2_mul(f2(x[e], x[e + 1]), cu)), a, b);
+      x[e] = __float_as_uint(a);
+      x[e + 1] = __float_as_uint(b);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      float z[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = __uint_as_float(x[e + i]) * p.cap_in;
+      cap_r4(z);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[e + i] = __float_as_uint(fmaf(-2.f, z[i], 1.f));
+    }
+  }
+}
+
 // Which of 32 ids per word (this lane holds ids[k * 32 + lane] in v[k]) equal this lane's own id:
 // one ballot a word for each different id of the warp's rows, usually one or two.
 template <int N>
@@ -349,6 +376,12 @@ __device__ __forceinline__ void same_ids(const int (&v)[N], int id, uint32_t (&s
     }
     todo &= ~__ballot_sync(0xffffffffu, id == cur);
   }
+}
+__device__ __forceinline__ uint32_t same_id(int v, int id) {
+  uint32_t same[1];
+  const int w[1] = {v};
+  same_ids<1>(w, id, same);
+  return same[0];
 }
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 

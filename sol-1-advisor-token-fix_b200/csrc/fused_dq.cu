@@ -1,0 +1,329 @@
+// fused_dq.cu — gradient of the queries (see fused_bwd.cuh).
+#include "fused_bwd.cuh"
+#include "fused_host.h"
+
+namespace attn_bwd {
+namespace fused {
+
+struct DqUnit {
+  int b, h, kvh, r0, r1, pre, lim0, n;
+};
+__device__ __forceinline__ DqUnit dq_unit(const BwdParams& prm, const Unit& u) {
+  const Params& p = prm.c;
+  DqUnit f;
+  const int blk = prm.divH.div(u.x), qt = p.n_tiles - 1 - blk;   // later queries see more: first
+  f.h = u.x - blk * p.H;
+  f.b = u.y;
+  f.kvh = p.divG.div(f.h);
+  f.r0 = qt * TILE;
+  f.r1 = min(p.sq, f.r0 + TILE) - 1;
+  f.pre = p.prefix ? __ldg(p.prefix + f.b) : 0;
+  f.lim0 = row_limit(p, f.r0, f.pre);
+  f.n = p.has_docs ? u.n : max(0, row_limit(p, f.r1, f.pre) + TILE - 1) / TILE;
+  return f;
+}
+
+// TMEM: two score tiles (the next one is computed while this one is worked on; ds is written
+// over the scores it came from), dp, and the accumulator.
+template <int D, bool F16, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+          const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const BwdParams prm) {
+  using C = BwdCfg<D>;
+  constexpr int ST = C::ST;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const BwdShared sh = bwd_shared<D>(smem_raw);
+  const Params& p = prm.c;
+  const uint32_t warp = warp_id(), lane = lane_id();
+  const uint32_t tmem = bwd_begin(sh, ST, &tm_q, &tm_do, &tm_k, &tm_v);
+  const uint32_t t_dp = tmem + 2 * TILE, t_dq = tmem + 3 * TILE;
+  Unit u;
+
+  if (warp >= 8) {
+    regs_shrink();
+    if (warp == 8) {
+      // -------------------------------------------------------------- producer
+      uint32_t it = 0, ri = 0;
+      for (uint32_t k = 0; next_unit(sh.sched, k, u, sh.abort_flag, 0x4103); ++k) {
+        const DqUnit f = dq_unit(prm, u);
+        const uint16_t* list = sh.lists + (k & 1) * kMaxList;
+        bool ok = true;
+        if (f.n > 0) {
+          ok = wait_for(sh.res_empty, (ri & 1) ^ 1, sh.abort_flag, 0x4102);
+          if (!ok) break;
+          ++ri;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(sh.res_full, 2 * C::TILE_BYTES);
+            for (int m = 0; m < 2; ++m)
+              for (int x = 0; x < D / 64; ++x)
+                tma_load_4d(sh.smem + C::OFF_A + m * C::TILE_BYTES + x * (TILE * 128), m ? &tm_do : &tm_q, sh.res_full,
+                            x * 64, f.r0, f.h, f.b);
+          }
+        }
+        for (int i = 0; i < f.n && ok; ++i, ++it) {
+          const int j0 = (p.has_docs ? int(list[i] & kEntTile) : i) * TILE;
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t s = (2 * it + m) % ST;
+            ok = wait_for(&sh.empty[s], (((2 * it + m) / ST) & 1) ^ 1, sh.abort_flag, 0x4101);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&sh.full[s], C::TILE_BYTES);
+              for (int x = 0; x < D / 64; ++x)
+                tma_load_4d(sh.smem + C::OFF_RING + s * C::TILE_BYTES + x * (TILE * 128), m ? &tm_v : &tm_k,
+                            &sh.full[s], x * 64, j0, f.kvh, f.b);
+            }
+          }
+        }
+        if (!ok) break;
+        ask_for_unit(sh.sched);
+        unit_done(sh.sched, k);
+      }
+      if (lane == 0) {
+        if (ri) mbar_drain(sh.res_full, (ri - 1) & 1, p.err, 0x4111);
+        for (uint32_t k = 0; k < uint32_t(ST) && k < 2 * it; ++k) {
+          const uint32_t i = 2 * it - 1 - k;
+          mbar_drain(&sh.full[i % ST], (i / ST) & 1, p.err, 0x4112);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      // -------------------------------------------------------------- tensor cores
+      constexpr uint32_t id_s = idesc16(F16, TILE, TILE, false, false);
+      constexpr uint32_t id_g = idesc16(F16, TILE, D, false, true);
+      const bool one = elect_one();
+      const uint64_t qs = desc_k(smem_u32(sh.smem + C::OFF_A)), dos = desc_k(smem_u32(sh.smem + C::OFF_A) + C::TILE_BYTES);
+      const uint32_t ring = smem_u32(sh.smem + C::OFF_RING);
+      auto stage = [&](uint32_t si) { return ring + (si % ST) * C::TILE_BYTES; };
+      uint32_t it = 0, ri = 0;
+      bool ok = true;
+      for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, 0x4208); ++k) {
+        const DqUnit f = dq_unit(prm, u);
+        const uint16_t* list = sh.lists + (k & 1) * kMaxList;
+        if (f.n > 0) {
+          auto arrived = [&](int i, int m, int code) {   // key (m = 0) or value tile of the unit's item i
+            const uint32_t si = 2 * (it + i) + m;
+            if (!wait_for(&sh.full[si % ST], (si / ST) & 1, sh.abort_flag, code)) return false;
+            return true;
+          };
+          auto scrub = [&](int i, uint32_t si) {
+            if (p.has_docs && (list[i] & kEntScrub)) {
+              const int j0 = int(list[i] & kEntTile) * TILE;
+              scrub_rows<D>(stage(si), p.kdoc + (size_t)f.b * p.skv + j0, p.skv - j0, lane);
+            }
+          };
+          ok = wait_for(sh.res_full, ri & 1, sh.abort_flag, 0x4201) && arrived(0, 0, 0x4202) &&
+               arrived(0, 1, 0x4203) && (f.n < 2 || arrived(1, 0, 0x4204));
+          if (!ok) break;
+          ++ri;
+          scrub(0, 2 * it);
+          if (f.n > 1) scrub(1, 2 * it + 2);
+          tc_fence_after();
+          mma_kk<D>(one, tmem + (it & 1) * TILE, qs, desc_k(stage(2 * it)), id_s);
+          commit1(one, &sh.s_full[it & 1]);
+          mma_kk<D>(one, t_dp, dos, desc_k(stage(2 * it + 1)), id_s);
+          commit1(one, sh.dp_full);
+          commit1(one, &sh.empty[(2 * it + 1) % ST]);
+          if (f.n > 1) {
+            mma_kk<D>(one, tmem + ((it + 1) & 1) * TILE, qs, desc_k(stage(2 * it + 2)), id_s);
+            commit1(one, &sh.s_full[(it + 1) & 1]);
+          } else {
+            commit1(one, sh.res_empty);
+          }
+          for (int i = 0; i < f.n; ++i, ++it) {
+            if (i + 1 < f.n && !(ok = arrived(1, 1, 0x4205))) break;
+            if (!(ok = wait_for(sh.ds_ready, it & 1, sh.abort_flag, 0x4206))) break;
+            tc_fence_after();
+            const uint32_t t_s = tmem + (it & 1) * TILE;
+            if (i + 1 < f.n) {
+              mma_kk<D>(one, t_dp, dos, desc_k(stage(2 * it + 3)), id_s);
+              commit1(one, sh.dp_full);
+              commit1(one, &sh.empty[(2 * it + 3) % ST]);
+              if (i + 2 == f.n) commit1(one, sh.res_empty);   // the last scores were issued before
+            }
+            mma_tn<D>(one, t_dq, t_s, t_s + 64, desc_mn(stage(2 * it)), id_g, i > 0);
+            commit1(one, &sh.empty[(2 * it) % ST]);
+            if (i + 1 == f.n) commit1(one, sh.done);
+            if (i + 2 < f.n) {
+              if (!(ok = arrived(2, 0, 0x4207))) break;
+              scrub(i + 2, 2 * it + 4);
+              tc_fence_after();
+              mma_kk<D>(one, t_s, qs, desc_k(stage(2 * it + 4)), id_s);
+              commit1(one, &sh.s_full[it & 1]);
+            }
+          }
+          if (!ok) break;
+        }
+        unit_done(sh.sched, k);
+      }
+      // no commit may arrive after the block has left
+      commit1(one, sh.all_done);
+      wait_for(sh.all_done, 0, sh.abort_flag, 0x4209);
+    } else if (warp == 10) {
+      // -------------------------------------------------------------- units and their lists
+      run_scheduler(sh.sched, sh.abort_flag, 0x4401, [&](int x, int y, int z, uint32_t slot) {
+        if (!p.has_docs) return 0;
+        const DqUnit f = dq_unit(prm, Unit{x, y, z, 0});
+        const DocRange qd = p.qrange[(size_t)f.b * p.n_tiles + f.r0 / TILE];
+        const int t1 = max(0, row_limit(p, f.r1, f.pre) + TILE - 1) / TILE;
+        int n = 0;
+        for (int t = 0; t < t1; t += 32) {
+          int st = kStSkip;
+          bool scrub = false;
+          if (t + int(lane) < t1) {
+            const int j0 = (t + int(lane)) * TILE;
+            const DocRange kd = p.krange[(size_t)f.b * prm.n_kt + t + lane];
+            st = pair_state(p, f.pre, f.r0, f.r1, j0, j0 + TILE - 1, qd, kd);
+            scrub = kd.neg != 0;
+          }
+          n = list_append(sh.lists + slot * kMaxList, n, t + int(lane), st, scrub, lane);
+        }
+        return n;
+      });
+    }
+  } else {
+    // ---------------------------------------------------------------- weights: one query a thread, 64 keys
+    regs_grow();
+    const int half = int(warp) >> 2;
+    const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t dp = t_dp + t_lane + half * 64;
+    const uint32_t stage = smem_u32(sh.smem + C::OFF_STAGE) + warp * 2048;
+    uint32_t it = 0, di = 0;
+    bool ok = true;
+    for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, 0x4304); ++k) {
+      const DqUnit f = dq_unit(prm, u);
+      const uint16_t* list = sh.lists + (k & 1) * kMaxList;
+      const int row = f.r0 + int(warp & 3) * 32 + int(lane);
+      const bool valid = row < p.sq;
+      const size_t ri = ((size_t)f.b * p.H + f.h) * prm.sq_pad + row;
+      const float nlse = prm.nlse[ri], nd = prm.ndelta[ri];   // padded to whole tiles
+      const int lim = valid ? row_limit(p, row, f.pre) : 0;
+      const int qd = (valid && p.has_docs) ? __ldg(p.qdoc + (size_t)f.b * p.sq + row) : -1;
+      const float slope2 = BIAS ? __ldg(p.slopes + f.h) * kLog2e : 0.f;
+      const uint64_t nd2 = f2(nd, nd);
+      for (int i = 0; i < f.n; ++i, ++it) {
+        const uint32_t ent = p.has_docs ? list[i] : 0u;
+        const int t0 = (p.has_docs ? int(ent & kEntTile) : i) * TILE, j0 = t0 + half * 64;
+        const bool masked = p.has_docs ? (ent & kEntMask) != 0 : t0 + TILE > f.lim0;
+        const uint32_t st = tmem + (it & 1) * TILE + t_lane + half * 64;
+        uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+        if (masked) {
+          if (p.has_docs) {
+            int ids[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const int j = j0 + y * 32 + int(lane);
+              ids[y] = j < p.skv ? __ldg(p.kdoc + (size_t)f.b * p.skv + j) : -1;
+            }
+            same_ids<2>(ids, qd, see);
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y) see[y] &= low_bits(lim - j0 - y * 32);
+        }
+        ok = wait_for(&sh.s_full[it & 1], (it >> 1) & 1, sh.abort_flag, 0x4301);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t w[2][32];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) tmem_ld32(st + y * 32, w[y]);
+        tmem_wait_ld();
+        const float dist0 = float(row + p.off - j0);
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              float add[4], x[4], m[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) {
+                x[z] = __uint_as_float(w[y][e + z]);
+                add[z] = BIAS ? fmaf(-slope2, fabsf(dist0 - float(y * 32 + e + z)), nlse) : nlse;
+              }
+              weights4<CAP>(p, x, add, m);
+#pragma unroll
+              for (int z = 0; z < 4; ++z) w[y][e + z] = __float_as_uint(m[z]);
+            }
+        // masked scores are taken out of ds below
+        ok = wait_for(sh.dp_full, it & 1, sh.abort_flag, 0x4302);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          uint32_t d[32], pk[16];
+          tmem_ld32(dp + y * 32, d);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float a0, a1;
+            f2_split(f2_mul(f2(w[y][e], w[y][e + 1]), f2_add(f2(d[e], d[e + 1]), nd2)), a0, a1);
+            if (masked) {
+              if (!((see[y] >> e) & 1u)) a0 = 0.f;
+              if (!((see[y] >> (e + 1)) & 1u)) a1 = 0.f;
+            }
+            pk[e / 2] = pack2<F16>(a0, a1);
+          }
+          tmem_st16(st + y * 16, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sh.ds_ready);
+      }
+      if (!ok) break;
+      // ---- epilogue: each half of the warps writes half of the columns
+      if (f.n > 0) {
+        ok = wait_for(sh.done, di & 1, sh.abort_flag, 0x4303);
+        if (!ok) break;
+        ++di;
+      }
+      tc_fence_after();
+      uint8_t* out = static_cast<uint8_t*>(prm.dq) + 2 * (f.b * prm.dqs[0] + f.h * prm.dqs[1] + row * prm.dqs[2]) +
+                     half * D;
+#pragma unroll 1
+      for (int x = 0; x < D / 64; ++x) {
+        uint32_t v[32], o[16];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0u;
+        __syncwarp();
+        if (f.n > 0) {
+          tmem_ld32(t_dq + t_lane + half * (D / 2) + x * 32, v);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          o[e] = pack2<F16>(__uint_as_float(v[2 * e]) * p.scale, __uint_as_float(v[2 * e + 1]) * p.scale);
+        write_rows(stage, o, valid ? out + x * 64 : nullptr, lane);
+      }
+      tc_fence_before();   // the next unit's first product overwrites the accumulator
+      unit_done(sh.sched, k);
+    }
+  }
+  bwd_end(sh, tmem, p.err);
+}
+
+template <int D, bool F16, bool CAP, bool BIAS>
+static int launch(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& go, const CUtensorMap& k,
+                  const CUtensorMap& v, cudaStream_t s) {
+  using C = BwdCfg<D>;
+  const auto kern = dq_kernel<D, F16, CAP, BIAS>;
+  const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
+  if (rc) return rc;
+  kern<<<dim3(unsigned(f.c.n_tiles) * f.c.H, f.c.bs), kThreads, C::SMEM_BYTES, s>>>(q, go, k, v, f);
+  return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;
+}
+
+int launch_dq(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& go, const CUtensorMap& k,
+              const CUtensorMap& v, int d, bool f16, bool cap, cudaStream_t s) {
+  const bool bias = f.c.slopes != nullptr;
+#define ATTN_BWD_PICK(DD, FF)                                                                                   \
+  if (d == DD && f16 == FF)                                                                                     \
+    return cap ? (bias ? launch<DD, FF, true, true>(f, q, go, k, v, s) : launch<DD, FF, true, false>(f, q, go, k, v, s)) \
+               : (bias ? launch<DD, FF, false, true>(f, q, go, k, v, s) : launch<DD, FF, false, false>(f, q, go, k, v, s));
+  ATTN_BWD_PICK(128, false)
+  ATTN_BWD_PICK(128, true)
+  ATTN_BWD_PICK(64, false)
+  ATTN_BWD_PICK(64, true)
+#undef ATTN_BWD_PICK
+  return ATTN_BWD_EUNSUPPORTED;
+}
+
+}  // namespace fused
+}  // namespace attn_bwd

@@ -54,11 +54,11 @@ int64_t fwd_workspace(const attn_bwd_fused_t* a, int sm_count) {
   return range_bytes(f.c) + part_rows(f.c) * (a->head_dim + 1) * 4;
 }
 
-template <int D, bool F16, bool CAP>
+template <int D, bool F16, bool CAP, bool BIAS>
 static int launch(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                   cudaStream_t stream) {
   using C = FwdCfg<D>;
-  auto kern = fwd_kernel<D, F16, CAP>;
+  auto kern = fwd_kernel<D, F16, CAP, BIAS>;
   const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
   if (rc) return rc;
   if (f.c.has_docs && f.c.n_tiles > 0) {
@@ -116,17 +116,15 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
     return ATTN_BWD_ETMAP;
   if (p.skv == 0) mk = mv = mq;   // never loaded from, only prefetched
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_);
-  const bool cap = a->softcap > 0.f;
-#define ATTN_BWD_FWD(DD, FF, CC) \
-  if (a->head_dim == DD && f16 == FF && cap == CC) return launch<DD, FF, CC>(f, mq, mk, mv, s);
-  ATTN_BWD_FWD(128, false, false)
-  ATTN_BWD_FWD(128, false, true)
-  ATTN_BWD_FWD(128, true, false)
-  ATTN_BWD_FWD(128, true, true)
-  ATTN_BWD_FWD(64, false, false)
-  ATTN_BWD_FWD(64, false, true)
-  ATTN_BWD_FWD(64, true, false)
-  ATTN_BWD_FWD(64, true, true)
+  const bool cap = a->softcap > 0.f, bias = a->slopes != nullptr;
+#define ATTN_BWD_FWD(DD, FF)                                                                          \
+  if (a->head_dim == DD && f16 == FF)                                                                \
+    return cap ? (bias ? launch<DD, FF, true, true>(f, mq, mk, mv, s) : launch<DD, FF, true, false>(f, mq, mk, mv, s)) \
+               : (bias ? launch<DD, FF, false, true>(f, mq, mk, mv, s) : launch<DD, FF, false, false>(f, mq, mk, mv, s));
+  ATTN_BWD_FWD(128, false)
+  ATTN_BWD_FWD(128, true)
+  ATTN_BWD_FWD(64, false)
+  ATTN_BWD_FWD(64, true)
 #undef ATTN_BWD_FWD
   return ATTN_BWD_EUNSUPPORTED;
 }

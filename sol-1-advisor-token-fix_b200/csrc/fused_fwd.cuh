@@ -98,7 +98,7 @@ __device__ __forceinline__ FwdUnit fwd_unit(const FwdParams& prm, const Unit& u)
   f.n = p.has_docs ? u.n : max(0, min(min(p.n_tiles, f.t0 + p.tiles_per_split), hi) - f.t0);
   return f;
 }
-template <int D, bool F16, bool CAP>
+template <int D, bool F16, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64, heads of a row, positions, 1)
            const __grid_constant__ CUtensorMap tm_k,   // (d, s, h, b), box (64, 128, 1, 1)
@@ -300,9 +300,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     const uint32_t t_s = tmem + t_lane + t * TILE, t_o = tmem + t_lane + 2 * TILE + t * D;
     const int row = int(warp & 3) * 32 + int(lane);
     const uint32_t stage = smem_u32(smem + C::OFF_STAGE) + warp * 2048;
-    const bool biased = p.slopes != nullptr;
     // without a bias scores stay raw (or a tanh) and are scaled inside the exponent
-    const float c = biased ? 1.f : CAP ? p.cap_out : p.scale_log2;
+    const float c = BIAS ? 1.f : CAP ? p.cap_out : p.scale_log2;
     const float grow = 8.f / c;
     const TanhSmall tanh_small;
     uint32_t cnt = 0;   // tiles so far
@@ -328,7 +327,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
       const int lim = valid ? row_limit(p, pos, f.pre) : 0;
       const int qd = (valid && p.has_docs) ? __ldg(p.qdoc + (size_t)f.b * p.sq + pos) : -1;
       const bool any_valid = __any_sync(0xffffffffu, valid);   // warps of padding rows only pass barriers
-      const float slope2 = (biased && valid) ? __ldg(p.slopes + head) * kLog2e : 0.f;
+      const float slope2 = (BIAS && valid) ? __ldg(p.slopes + head) * kLog2e : 0.f;
 
       float mref = -INFINITY;   // reference maximum, in units of 1 / c
       float l = 0.f;
@@ -337,97 +336,97 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
         const uint32_t ent = p.has_docs ? list[i] : 0u;
         const int j0 = (f.t0 + (p.has_docs ? int(ent & kEntTile) : i)) * TILE;
         const bool masked = p.has_docs ? (ent & kEntMask) != 0 : j0 + TILE > f.lim0;
-        int ids[4];
-        if (masked && p.has_docs) {
-          const int* kdoc = p.kdoc + (size_t)f.b * p.skv;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int j = j0 + g * 32 + int(lane);
-            ids[g] = j < p.skv ? __ldg(kdoc + j) : -1;
-          }
-        }
         ok = wait_for(&s_full[t], (cnt + i) & 1, abort_flag, 0x2301);
         if (!ok) break;
         tc_fence_after();
         // every completion of o_done is waited for once, so its parity cannot be mistaken
         bool o_seen = i == 0;
-        if (any_valid) {
-          uint32_t s[4][32];
-#pragma unroll
-          for (int g = 0; g < 4; ++g) tmem_ld32(t_s + g * 32, s[g]);
-          tmem_wait_ld();
-          if (CAP) {
-            float big = 0.f;
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll
-              for (int e = 0; e < 32; e += 2)
-                big = fmaxf(big, fmaxf(fabsf(__uint_as_float(s[g][e])), fabsf(__uint_as_float(s[g][e + 1]))));
-            if (__all_sync(0xffffffffu, big * p.cap_u <= kTanhSmall)) {
-              const uint64_t cu = f2(p.cap_u, p.cap_u);
-#pragma unroll
-              for (int g = 0; g < 4; ++g)
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                  float x0, x1;
-                  f2_split(tanh_small(f2_mul(f2(s[g][e], s[g][e + 1]), cu)), x0, x1);
-                  s[g][e] = __float_as_uint(x0);
-                  s[g][e + 1] = __float_as_uint(x1);
-                }
-            } else {
-#pragma unroll
-              for (int g = 0; g < 4; ++g)
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                  float z[4];
-#pragma unroll
-                  for (int y = 0; y < 4; ++y) z[y] = __uint_as_float(s[g][e + y]) * p.cap_in;
-                  cap_r4(z);
-#pragma unroll
-                  for (int y = 0; y < 4; ++y) s[g][e + y] = __float_as_uint(fmaf(-2.f, z[y], 1.f));
-                }
-            }
-          }
-          if (biased) {
-            const float d0 = float(pos + p.off - j0), sl = CAP ? p.cap_out : p.scale_log2;
-            if (__all_sync(0xffffffffu, pos + p.off >= j0 + TILE - 1)) {   // |i - j| = i - j: linear in the column
-              const float a = -slope2 * d0;
-#pragma unroll
-              for (int g = 0; g < 4; ++g)
+        if (__builtin_expect(any_valid, 1)) {
+          // Three ways through a row, by what has to be done to its scores:
+          //   nothing but a mask, or a bias that is linear along it: 128 scores stay in registers;
+          //   cap alone: the maximum is the tanh of the raw scores' maximum, and the tanh is
+          //     taken next to the exponentials, which use other units;
+          //   anything else: scores are rewritten in TMEM, 32 at a time, then read again.
+          // (All of it on 128 scores in registers spilled, and a row read twice cost the plain
+          // case 10 % of the 4096x4096 prompt.)
+          // 32 scores from column 32 g on: cap, bias, mask (log2 units / c, -inf where not seen)
+          auto modify = [&](uint32_t (&x)[32], int g) {
+            if (CAP) cap32(p, tanh_small, x);
+            if (BIAS) {
+              const float d0 = float(pos + p.off - j0 - g * 32), sl = CAP ? p.cap_out : p.scale_log2;
+              if (__all_sync(0xffffffffu, d0 >= 31.f)) {   // |i - j| = i - j: linear in the column
+                const float a = -slope2 * d0;
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
-                  s[g][e] = __float_as_uint(fmaf(__uint_as_float(s[g][e]), sl, fmaf(slope2, float(g * 32 + e), a)));
-            } else {
-#pragma unroll
-              for (int g = 0; g < 4; ++g)
+                  x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), sl, fmaf(slope2, float(e), a)));
+              } else {
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
-                  s[g][e] = __float_as_uint(
-                      fmaf(__uint_as_float(s[g][e]), sl, -slope2 * fabsf(d0 - float(g * 32 + e))));
+                  x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), sl, -slope2 * fabsf(d0 - float(e))));
+              }
             }
-          }
-          if (masked) {
-            uint32_t see[4];
-            if (p.has_docs) same_ids<4>(ids, qd, see);
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const uint32_t below = low_bits(lim - j0 - g * 32);
-              see[g] = p.has_docs ? see[g] & below : below;
+            if (__builtin_expect(masked, 0)) {
+              uint32_t see = low_bits(lim - j0 - g * 32);
+              if (p.has_docs) {
+                const int j = j0 + g * 32 + int(lane);
+                see &= same_id(j < p.skv ? __ldg(p.kdoc + (size_t)f.b * p.skv + j) : -1, qd);
+              }
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (!((see[g] >> e) & 1u)) s[g][e] = 0xff800000u;   // -inf
+                if (!((see >> e) & 1u)) x[e] = 0xff800000u;   // -inf
             }
-          }
-          float mx[4];
+          };
+          auto highest = [](const uint32_t (&x)[32]) {
+            float y[2];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float y = fmaxf(__uint_as_float(s[g][0]), __uint_as_float(s[g][1]));
+            for (int h = 0; h < 2; ++h) {
+              y[h] = fmaxf(__uint_as_float(x[16 * h]), __uint_as_float(x[16 * h + 1]));
 #pragma unroll
-            for (int e = 2; e < 32; e += 2) y = fmaxf(y, fmaxf(__uint_as_float(s[g][e]), __uint_as_float(s[g][e + 1])));
-            mx[g] = y;
+              for (int e = 2; e < 16; e += 2)
+                y[h] = fmaxf(y[h], fmaxf(__uint_as_float(x[16 * h + e]), __uint_as_float(x[16 * h + e + 1])));
+            }
+            return fmaxf(y[0], y[1]);
+          };
+          const bool linear = BIAS && __all_sync(0xffffffffu, pos + p.off >= j0 + TILE - 1);
+          const bool in_regs = !CAP && (!BIAS || (!masked && linear));
+          const bool late_cap = CAP && !BIAS && !masked;
+          uint32_t x[4][32];
+          float m;
+          if (in_regs || late_cap) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) tmem_ld32(t_s + g * 32, x[g]);
+            tmem_wait_ld();
+            if (BIAS) {
+              const float a = -slope2 * float(pos + p.off - j0);
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  x[g][e] = __float_as_uint(
+                      fmaf(__uint_as_float(x[g][e]), p.scale_log2, fmaf(slope2, float(g * 32 + e), a)));
+            }
+            if (!CAP && !BIAS && __builtin_expect(masked, 0)) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) modify(x[g], g);
+            }
+            m = fmaxf(fmaxf(highest(x[0]), highest(x[1])), fmaxf(highest(x[2]), highest(x[3])));
+            if (CAP) m = fmaf(-2.f, rcp(1.f + ex2(m * p.cap_in)), 1.f);   // the tanh grows with its argument
+          } else if constexpr (CAP || BIAS) {
+            m = -INFINITY;
+#pragma unroll 1
+            for (int g = 0; g < 4; ++g) {
+              uint32_t y[32];
+              __syncwarp();
+              tmem_ld32(t_s + g * 32, y);
+              tmem_wait_ld();
+              modify(y, g);
+              m = fmaxf(m, highest(y));
+              tmem_st16(t_s + g * 32, *reinterpret_cast<uint32_t (*)[16]>(&y[0]));
+              tmem_st16(t_s + g * 32 + 16, *reinterpret_cast<uint32_t (*)[16]>(&y[16]));
+            }
+            tmem_wait_st();
           }
-          const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          if (__any_sync(0xffffffffu, m > mref + grow)) {
+          if (__builtin_expect(__any_sync(0xffffffffu, m > mref + grow), 0)) {
             const float mnew = fmaxf(mref, m);
             const float fac = mref == mnew ? 1.f : ex2((mref - mnew) * c);   // 0 from a reference of -inf
             mref = mnew;
@@ -438,18 +437,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
               o_seen = true;
               tc_fence_after();
 #pragma unroll 1
-              for (int x = 0; x < D / 32; ++x) {
-                uint32_t o[2][16];
-                tmem_ld16(t_o + x * 32, o[0]);
-                tmem_ld16(t_o + x * 32 + 16, o[1]);
+              for (int x = 0; x < D / 16; ++x) {
+                uint32_t o[16];
+                tmem_ld16(t_o + x * 16, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  o[0][e] = __float_as_uint(__uint_as_float(o[0][e]) * fac);
-                  o[1][e] = __float_as_uint(__uint_as_float(o[1][e]) * fac);
-                }
-                tmem_st16(t_o + x * 32, o[0]);
-                tmem_st16(t_o + x * 32 + 16, o[1]);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
+                tmem_st16(t_o + x * 16, o);
               }
               tmem_wait_st();
             }
@@ -457,27 +451,52 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           const float nm = mref == -INFINITY ? 0.f : -mref * c;
           const uint64_t c2 = f2(c, c), nm2 = f2(nm, nm);
           uint64_t sum0 = 0, sum1 = 0;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
+          // weights of 32 keys, to 16 columns
+          auto weigh = [&](const uint32_t (&y)[32], uint32_t column) {
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
               float a0, a1, b0, b1;
-              f2_split(f2_fma(f2(s[g][e], s[g][e + 1]), c2, nm2), a0, a1);
-              f2_split(f2_fma(f2(s[g][e + 2], s[g][e + 3]), c2, nm2), b0, b1);
+              f2_split(f2_fma(f2(y[e], y[e + 1]), c2, nm2), a0, a1);
+              f2_split(f2_fma(f2(y[e + 2], y[e + 3]), c2, nm2), b0, b1);
               a0 = ex2(a0); a1 = ex2(a1); b0 = ex2(b0); b1 = ex2(b1);
               sum0 = f2_add(sum0, f2(a0, a1));
               sum1 = f2_add(sum1, f2(b0, b1));
               w[e / 2] = pack2<F16>(a0, a1);
               w[e / 2 + 1] = pack2<F16>(b0, b1);
             }
-            tmem_st16(t_s + g * 16, w);
-            if (g == 1) {
-              tmem_wait_st();
-              tc_fence_before();
-              if (!o_seen) ok = wait_for(&o_done[t], (cnt + i - 1) & 1, abort_flag, 0x2305);
-              __syncwarp();
-              if (lane == 0 && ok) mbar_arrive(&p_ready[2 * t]);
+            tmem_st16(t_s + column, w);
+          };
+          // the weights of 64 keys are written: the second product may take them
+          auto hand_over = [&](int h) {
+            tmem_wait_st();
+            tc_fence_before();
+            if (!o_seen) {
+              ok = wait_for(&o_done[t], (cnt + i - 1) & 1, abort_flag, 0x2305);
+              o_seen = true;
+            }
+            __syncwarp();
+            if (lane == 0 && ok) mbar_arrive(&p_ready[2 * t + h]);
+          };
+          if (in_regs) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              weigh(x[g], g * 16);
+              if (g & 1) hand_over(g >> 1);
+            }
+          } else if constexpr (CAP || BIAS) {
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+              for (int g = 2 * h; g < 2 * h + 2; ++g) {
+                uint32_t y[32];
+                __syncwarp();
+                tmem_ld32(t_s + g * 32, y);
+                tmem_wait_ld();
+                if (CAP && late_cap) cap32(p, tanh_small, y);
+                weigh(y, g * 16);
+              }
+              hand_over(h);
             }
           }
           if (!ok) break;
@@ -485,15 +504,15 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           f2_split(sum0, x0, x1);
           f2_split(sum1, y0, y1);
           l += (x0 + x1) + (y0 + y1);
-          tmem_wait_st();
         } else {
           if (!o_seen) ok = wait_for(&o_done[t], (cnt + i - 1) & 1, abort_flag, 0x2306);
           if (!ok) break;
-          if (lane == 0) mbar_arrive(&p_ready[2 * t]);
+          tc_fence_before();
+          if (lane == 0) {
+            mbar_arrive(&p_ready[2 * t]);
+            mbar_arrive(&p_ready[2 * t + 1]);
+          }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[2 * t + 1]);
       }
       // ---- epilogue: o / l, and the row statistic
       if (ok && f.n > 0) ok = wait_for(&o_done[t], (cnt + f.n - 1) & 1, abort_flag, 0x2303);
