@@ -125,25 +125,18 @@ __device__ __forceinline__ void bwd_end(const BwdShared& s, uint32_t tmem, int* 
   }
 }
 
-// Weights of four scores.  x: raw scores in, p out; m: what ds is multiplied by (p, or p tanh').
-// add: bias - lse in log2 units.
+// Weights of four scores (CAP: of their tanh).  x: in, p out; m: what ds is multiplied by (p, or
+// p tanh').  add: bias - lse in log2 units.
 template <bool CAP>
 __device__ __forceinline__ void weights4(const Params& p, float (&x)[4], const float (&add)[4], float (&m)[4]) {
+  const float c = CAP ? p.cap_out : p.scale_log2;
+  const uint64_t c2 = f2(c, c);
   if (CAP) {
-    float r[4];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) r[y] = x[y] * p.cap_in;
-    cap_r4(r);
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      x[y] = fmaf(-2.f * p.cap_out, r[y], p.cap_out) + add[y];
-      m[y] = 4.f * r[y] * (1.f - r[y]);
-    }
-  } else {
-    const uint64_t c2 = f2(p.scale_log2, p.scale_log2);
-    f2_split(f2_fma(f2(x[0], x[1]), c2, f2(add[0], add[1])), x[0], x[1]);
-    f2_split(f2_fma(f2(x[2], x[3]), c2, f2(add[2], add[3])), x[2], x[3]);
+    for (int y = 0; y < 4; ++y) m[y] = fmaf(-x[y], x[y], 1.f);
   }
+  f2_split(f2_fma(f2(x[0], x[1]), c2, f2(add[0], add[1])), x[0], x[1]);
+  f2_split(f2_fma(f2(x[2], x[3]), c2, f2(add[2], add[3])), x[2], x[3]);
 #pragma unroll
   for (int y = 0; y < 4; ++y) {
     x[y] = ex2(x[y]);

@@ -202,6 +202,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
   } else {
     // ---------------------------------------------------------------- weights: one key a thread, 64 queries
     regs_grow();
+    const TanhSmall tanh_small;
     const int half = int(warp) >> 2;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t st = t_st + t_lane + half * 64, dp = t_dp + t_lane + half * 64;
@@ -251,6 +252,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             uint32_t pk[16];
+            if (CAP) cap32(p, tanh_small, w[y]);
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
               const float4 nl4 = *reinterpret_cast<const float4*>(stat + y * 32 + e);

@@ -183,6 +183,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
   } else {
     // ---------------------------------------------------------------- weights: one query a thread, 64 keys
     regs_grow();
+    const TanhSmall tanh_small;
     const int half = int(warp) >> 2;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t dp = t_dp + t_lane + half * 64;
@@ -228,9 +229,10 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         tmem_wait_ld();
         const float dist0 = float(row + p.off - j0);
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < 2; ++y) {
+          if (CAP) cap32(p, tanh_small, w[y]);
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
+          for (int e = 0; e < 32; e += 4) {
               float add[4], x[4], m[4];
 #pragma unroll
               for (int z = 0; z < 4; ++z) {
@@ -240,7 +242,8 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
               weights4<CAP>(p, x, add, m);
 #pragma unroll
               for (int z = 0; z < 4; ++z) w[y][e + z] = __float_as_uint(m[z]);
-            }
+          }
+        }
         // masked scores are taken out of ds below
         ok = wait_for(sh.dp_full, it & 1, sh.abort_flag, 0x4302);
         if (!ok) break;
