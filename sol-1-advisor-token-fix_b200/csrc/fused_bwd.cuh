@@ -42,7 +42,7 @@ struct BwdCfg {
   static constexpr int OFF_LIST = OFF_STAGE + 8 * 2048;
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;
-  static constexpr int NBAR = 3 + 2 * ST + 6 + 6;
+  static constexpr int NBAR = 3 + 2 * ST + 8 + 6;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int SMEM_BYTES = OFF_MISC + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024, "backward kernel shared memory");
@@ -69,9 +69,9 @@ __device__ __forceinline__ BwdShared bwd_shared(uint8_t* raw) {
   s.empty = s.full + C::ST;
   s.s_full = s.empty + C::ST;
   s.p_ready = s.s_full + 2;   // dq: one s_full a score tile
-  s.dp_full = s.p_ready + 1;
+  s.dp_full = s.p_ready + 2;  // p_ready, ds_ready: one for each 32 of a thread's 64 columns
   s.ds_ready = s.dp_full + 1;
-  s.done = s.ds_ready + 1;
+  s.done = s.ds_ready + 2;
   s.sched.slot = reinterpret_cast<Unit*>(s.smem + C::OFF_UNIT);
   s.sched.handle = smem_u32(s.smem + C::OFF_UNIT + 32);
   s.sched.full = s.done + 1;
@@ -94,9 +94,8 @@ __device__ __forceinline__ uint32_t bwd_begin(const BwdShared& s, int st, const 
     for (int i = 0; i < st; ++i) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 1); }
     mbar_init(&s.s_full[0], 1);
     mbar_init(&s.s_full[1], 1);
-    mbar_init(s.p_ready, 8);
+    for (int i = 0; i < 2; ++i) { mbar_init(&s.p_ready[i], 8); mbar_init(&s.ds_ready[i], 8); }
     mbar_init(s.dp_full, 1);
-    mbar_init(s.ds_ready, 8);
     mbar_init(s.done, 1);
     scheduler_init(s.sched);
     *s.abort_flag = 0;

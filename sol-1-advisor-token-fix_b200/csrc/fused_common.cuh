@@ -275,6 +275,10 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float4 lds_f4(uint32_t saddr) {
+  const uint4 v = lds128(saddr);
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
 __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -445,6 +449,15 @@ __device__ __forceinline__ void mma_tn(bool one, uint32_t d_tmem, uint32_t a0, u
 #pragma unroll
   for (int kk = K0; kk < K1; ++kk)
     umma_ts1(one, d_tmem, (kk < 4 ? a0 : a1) + (kk & 3) * 8, b + kk * (2048 >> 4), idesc, (accumulate || kk > 0) ? 1u : 0u);
+}
+
+// The steps of such a product whose A columns the weight warps hand over together: 32 of every
+// thread's 64 columns (Y = 0 or 1).
+template <int D, int Y>
+__device__ __forceinline__ void mma_tn_part(bool one, uint32_t d_tmem, uint32_t a0, uint32_t a1, uint64_t b,
+                                            uint32_t idesc, bool accumulate) {
+  mma_tn<D, 2 * Y, 2 * Y + 2>(one, d_tmem, a0, a1, b, idesc, accumulate);
+  mma_tn<D, 2 * Y + 4, 2 * Y + 6>(one, d_tmem, a0, a1, b, idesc, true);
 }
 
 // Clears the rows of a [128 x D] tile whose document is negative (or that lie behind the

@@ -150,18 +150,24 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
             const bool more = i + 1 < f.n;
             if (++t == f.nl) t = 0;
             if (more && !(ok = arrived(2 * it + 2, t, 0x3204))) break;
-            if (!(ok = wait_for(sh.p_ready, it & 1, sh.abort_flag, 0x3205))) break;
+            if (!(ok = wait_for(&sh.p_ready[0], it & 1, sh.abort_flag, 0x3205))) break;
             tc_fence_after();
-            mma_tn<D>(one, t_dv, t_st, t_st + 64, desc_mn(stage(2 * it + 1)), id_g, i > 0);
+            mma_tn_part<D, 0>(one, t_dv, t_st, t_st + 64, desc_mn(stage(2 * it + 1)), id_g, i > 0);
+            if (!(ok = wait_for(&sh.p_ready[1], it & 1, sh.abort_flag, 0x3200))) break;
+            tc_fence_after();
+            mma_tn_part<D, 1>(one, t_dv, t_st, t_st + 64, desc_mn(stage(2 * it + 1)), id_g, true);
             commit1(one, &sh.empty[(2 * it + 1) % ST]);
             if (more) {
               mma_kk<D>(one, t_st, ks, desc_k(stage(2 * it + 2)), id_s);
               commit1(one, &sh.s_full[0]);
             }
             if (more && !(ok = arrived(2 * it + 3, t, 0x3206))) break;
-            if (!(ok = wait_for(sh.ds_ready, it & 1, sh.abort_flag, 0x3207))) break;
+            if (!(ok = wait_for(&sh.ds_ready[0], it & 1, sh.abort_flag, 0x3207))) break;
             tc_fence_after();
-            mma_tn<D>(one, t_dk, t_dp, t_dp + 64, desc_mn(stage(2 * it)), id_g, i > 0);
+            mma_tn_part<D, 0>(one, t_dk, t_dp, t_dp + 64, desc_mn(stage(2 * it)), id_g, i > 0);
+            if (!(ok = wait_for(&sh.ds_ready[1], it & 1, sh.abort_flag, 0x320a))) break;
+            tc_fence_after();
+            mma_tn_part<D, 1>(one, t_dk, t_dp, t_dp + 64, desc_mn(stage(2 * it)), id_g, true);
             commit1(one, &sh.empty[(2 * it) % ST]);
             if (more) {
               mma_kk<D>(one, t_dp, vs, desc_k(stage(2 * it + 3)), id_s);
@@ -220,7 +226,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
         const uint32_t ent = dkv_entry(p, f, list, t, r0);
         const bool masked = (ent & kEntMask) != 0;
         r0 += half * 64;   // first of this thread's query rows
-        const float* stat = reinterpret_cast<const float*>(sh.smem + C::OFF_STAT + (it & 1) * (2 * TILE * 4)) + half * 64;
+        const uint32_t stat = smem_u32(sh.smem + C::OFF_STAT + (it & 1) * (2 * TILE * 4) + half * 256);
         uint32_t see[2] = {0xffffffffu, 0xffffffffu};
         if (masked) {
           // seen by row r if j < prefix or j <= r + off: rows from j - off on
@@ -255,7 +261,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
             if (CAP) cap32(p, tanh_small, w[y]);
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              const float4 nl4 = *reinterpret_cast<const float4*>(stat + y * 32 + e);
+              const float4 nl4 = lds_f4(stat + (y * 32 + e) * 4);
               float add[4] = {nl4.x, nl4.y, nl4.z, nl4.w}, x[4], m[4];
 #pragma unroll
               for (int z = 0; z < 4; ++z) {
@@ -272,14 +278,14 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
               pk[e / 2 + 1] = pack2<F16>(x[2], x[3]);
             }
             tmem_st16(st + y * 16, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.p_ready[y]);
           }
         };
         if (__builtin_expect(masked, 0)) phase(std::true_type{});
         else phase(std::false_type{});
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sh.p_ready);
 
         ok = wait_for(sh.dp_full, it & 1, sh.abort_flag, 0x3303);
         if (!ok) break;
@@ -291,7 +297,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
           tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            const float4 nd = *reinterpret_cast<const float4*>(stat + TILE + y * 32 + e);
+            const float4 nd = lds_f4(stat + (TILE + y * 32 + e) * 4);
             float a[4];
             f2_split(f2_mul(f2(w[y][e], w[y][e + 1]), f2_add(f2(d[e], d[e + 1]), f2(nd.x, nd.y))), a[0], a[1]);
             f2_split(f2_mul(f2(w[y][e + 2], w[y][e + 3]), f2_add(f2(d[e + 2], d[e + 3]), f2(nd.z, nd.w))), a[2], a[3]);
@@ -304,11 +310,11 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
             pk[e / 2 + 1] = pack2<F16>(a[2], a[3]);
           }
           tmem_st16(dp + y * 16, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.ds_ready[y]);
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sh.ds_ready);
         if (++t == f.nl) { t = 0; ++g; }
       }
       if (!ok) break;

@@ -131,18 +131,22 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
           }
           for (int i = 0; i < f.n; ++i, ++it) {
             if (i + 1 < f.n && !(ok = arrived(1, 1, 0x4205))) break;
-            if (!(ok = wait_for(sh.ds_ready, it & 1, sh.abort_flag, 0x4206))) break;
-            tc_fence_after();
             const uint32_t t_s = tmem + (it & 1) * TILE;
+            if (!(ok = wait_for(&sh.ds_ready[0], it & 1, sh.abort_flag, 0x4206))) break;
+            tc_fence_after();
+            mma_tn_part<D, 0>(one, t_dq, t_s, t_s + 64, desc_mn(stage(2 * it)), id_g, i > 0);
+            if (!(ok = wait_for(&sh.ds_ready[1], it & 1, sh.abort_flag, 0x420a))) break;
+            tc_fence_after();
+            // first, since the next load of keys waits for their tile
+            mma_tn_part<D, 1>(one, t_dq, t_s, t_s + 64, desc_mn(stage(2 * it)), id_g, true);
+            commit1(one, &sh.empty[(2 * it) % ST]);
+            if (i + 1 == f.n) commit1(one, sh.done);
             if (i + 1 < f.n) {
               mma_kk<D>(one, t_dp, dos, desc_k(stage(2 * it + 3)), id_s);
               commit1(one, sh.dp_full);
               commit1(one, &sh.empty[(2 * it + 3) % ST]);
               if (i + 2 == f.n) commit1(one, sh.res_empty);   // the last scores were issued before
             }
-            mma_tn<D>(one, t_dq, t_s, t_s + 64, desc_mn(stage(2 * it)), id_g, i > 0);
-            commit1(one, &sh.empty[(2 * it) % ST]);
-            if (i + 1 == f.n) commit1(one, sh.done);
             if (i + 2 < f.n) {
               if (!(ok = arrived(2, 0, 0x4207))) break;
               scrub(i + 2, 2 * it + 4);
@@ -264,11 +268,11 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
             pk[e / 2] = pack2<F16>(a0, a1);
           }
           tmem_st16(st + y * 16, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.ds_ready[y]);
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sh.ds_ready);
       }
       if (!ok) break;
       // ---- epilogue: each half of the warps writes half of the columns
