@@ -222,21 +222,7 @@ def _stream_handle(device_index):
     return torch.cuda.current_stream(device_index).cuda_stream
 
 
-def _load_torch_fast():
-    """The C++ host binding (csrc/torch_fast.cpp), or None when it is not built or when
-    ATTN_BWD_B200_LIB selects another build of the library (the binding links the
-    in-tree one)."""
-    import os
-    if os.environ.get("ATTN_BWD_B200_LIB") or os.environ.get("ATTN_BWD_NO_TORCH_BINDING"):
-        return None
-    try:
-        from . import _torch_fast
-    except ImportError:
-        return None
-    return _torch_fast.fast
-
-
-_torch_fast_fn = _load_torch_fast()
+_torch_fast_fn = getattr(_lib.binding(), "fast", None)   # csrc/torch_fast.cpp
 
 
 def attn_bwd(data, out=None):

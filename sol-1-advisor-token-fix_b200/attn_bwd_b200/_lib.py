@@ -113,3 +113,36 @@ def call(name, *args):
     rc = getattr(load(), name)(*args)
     if rc != OK:
         raise AttnBwdError(name, rc)
+
+
+_binding = []
+
+
+def binding():
+    """The C++ host binding (csrc/torch_fast.cpp), or None when it is not built or when
+    ATTN_BWD_B200_LIB selects another build of the library (the binding links the in-tree
+    one) or ATTN_BWD_NO_TORCH_BINDING is set."""
+    if not _binding:
+        mod = None
+        if not (os.environ.get("ATTN_BWD_B200_LIB") or os.environ.get("ATTN_BWD_NO_TORCH_BINDING")):
+            try:
+                from . import _torch_fast as mod
+            except ImportError:
+                mod = None
+        _binding.append(mod)
+    return _binding[0]
+
+
+def bound(name, *args):
+    """Calls a function of the C++ binding; None where it declines (the general path then looks
+    at the arguments), AttnBwdError where the library refuses the call."""
+    mod = binding()
+    if mod is None:
+        return None
+    try:
+        r = getattr(mod, name)(*args)
+    except TypeError:   # not what it takes: the general path reports it
+        return None
+    if isinstance(r, int):
+        raise AttnBwdError("attn_bwd_b200_" + name, r)
+    return r

@@ -49,6 +49,22 @@ def _aux(t, name, dtype, shape, dev):
     return t.contiguous()
 
 
+def _bound(name, tensors, q, k, v, scale, softcap, slopes, causal, prefix_lens, documents):
+    """The call through the C++ binding, or None where the general path has to look at it."""
+    qd = kd = documents
+    if isinstance(documents, (tuple, list)):
+        if len(documents) != 2:
+            return None
+        qd, kd = documents
+    if scale is None:
+        if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[3] == 0:
+            return None
+        scale = 1.0 / math.sqrt(q.shape[3])
+    if not (0 < scale < math.inf and 0 <= softcap < math.inf):
+        return None
+    return _lib.bound(name, *tensors, scale, softcap, slopes, bool(causal), prefix_lens, qd, kd)
+
+
 class _Call:
     """Checked arguments of one call: the C structure and the tensors that it points into."""
 
@@ -125,7 +141,12 @@ def fused_attn_fwd(query_states, key_states, value_states, scale=None, softcap=0
         what they hold (NaN included) reaches no result.
     A query that sees no key has output 0 and lse -inf.  A NaN or infinity in a key or value of
     a document (or without documents) may reach all queries near it, seen or not."""
-    c = _Call(query_states, key_states, value_states, scale, softcap, slopes, causal, prefix_lens, documents)
+    softcap = softcap or 0.0
+    mods = (query_states, key_states, value_states, scale, softcap, slopes, causal, prefix_lens, documents)
+    r = _bound("fused_fwd", (query_states, key_states, value_states), *mods)
+    if r is not None:
+        return r
+    c = _Call(*mods)
     bs, h, sq, d = query_states.shape
     with torch.cuda.device(c.device):
         o = torch.empty((bs, sq, h, d), dtype=query_states.dtype, device=c.device)
@@ -143,7 +164,12 @@ def fused_attn_bwd(grad_attn_output, query_states, key_states, value_states, att
     arguments as they were given there.  The gradients have the shapes of the states (keys' and
     values' summed over the heads that share them) and their order in memory.  Equal inputs
     give equal bits."""
-    c = _Call(query_states, key_states, value_states, scale, softcap, slopes, causal, prefix_lens, documents)
+    softcap = softcap or 0.0
+    mods = (query_states, key_states, value_states, scale, softcap, slopes, causal, prefix_lens, documents)
+    r = _bound("fused_bwd", (grad_attn_output, query_states, key_states, value_states, attn_output, lse), *mods)
+    if r is not None:
+        return r
+    c = _Call(*mods)
     bs, h, sq, d = query_states.shape
     _check(grad_attn_output, "grad_attn_output", query_states)
     _check(attn_output, "attn_output", query_states)
@@ -157,6 +183,8 @@ def fused_attn_bwd(grad_attn_output, query_states, key_states, value_states, att
         grads = []
         for t, dst in ((c.q, c.args.dq_stride), (c.k, c.args.dk_stride), (c.v, c.args.dv_stride)):
             g = torch.empty_like(t)
+            if g.stride(3) != 1:
+                g = torch.empty(t.shape, dtype=t.dtype, device=t.device)
             dst[:] = g.stride()[:3]
             grads.append(g)
         dq, dk, dv = grads

@@ -87,6 +87,10 @@ def _overlaps_itself(t):
 
 
 def _rotate(q, k, position_ids, table, interleaved, inverse, out):
+    if out is None and isinstance(table, RopeTable):
+        r = _lib.bound("rope", q, k, position_ids, table.turns, table.rotary_dim, table.factor, bool(interleaved), inverse)
+        if r is not None:
+            return r
     if not isinstance(table, RopeTable):
         raise TypeError(f"table: expected a RopeTable (rope_table(...)), got {type(table).__name__}")
     names = ("query", "key")
