@@ -5,6 +5,7 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include "fast_div.h"
 #include "sm100.cuh"
 
 namespace attn_bwd {
@@ -15,17 +16,6 @@ constexpr int TILE = 128;        // rows of a query tile, keys of a key tile
 constexpr int kMaxList = 2048;   // documents: tiles of one unit at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-
-// Division by a number known to the host, exact for 0 <= n < 2^31: with 2^shift >= d the
-// multiplier ceil(2^(32 + shift) / d) has 33 bits, of which mul holds the lower 32.
-struct FastDiv {
-  uint32_t mul, shift, d;
-  __device__ __forceinline__ int div(int n) const {
-    if (d == 1) return n;
-    const uint32_t h = __umulhi(uint32_t(n), mul);
-    return int((h + ((uint32_t(n) - h) >> 1)) >> (shift - 1));
-  }
-};
 
 struct DocRange;
 

@@ -36,15 +36,6 @@ inline int check_args(const attn_bwd_fused_t* a) {
   return ATTN_BWD_OK;
 }
 
-inline FastDiv fast_div(int d) {   // d >= 1
-  FastDiv f;
-  f.d = uint32_t(d);
-  f.shift = 1;
-  while ((1u << f.shift) < uint32_t(d)) ++f.shift;
-  f.mul = uint32_t((((1ull << f.shift) - uint64_t(d)) << 32) / uint64_t(d) + 1);
-  return f;
-}
-
 inline Params base_params(const attn_bwd_fused_t* a) {
   Params p;
   std::memset(&p, 0, sizeof(p));
