@@ -38,8 +38,7 @@ struct BwdCfg {
   static constexpr int OFF_A = 0;                               // two resident tiles
   static constexpr int OFF_RING = 2 * TILE_BYTES;
   static constexpr int OFF_STAT = OFF_RING + ST * TILE_BYTES;   // dkv: 2 x (nlse, ndelta) of 128 rows
-  static constexpr int OFF_STAGE = OFF_STAT + 2 * 2 * TILE * 4;
-  static constexpr int OFF_LIST = OFF_STAGE + 8 * 2048;
+  static constexpr int OFF_LIST = OFF_STAT + 2 * 2 * TILE * 4;
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;
   static constexpr int NBAR = 3 + 2 * ST + 8 + 6;
@@ -124,18 +123,23 @@ __device__ __forceinline__ void bwd_end(const BwdShared& s, uint32_t tmem, int* 
   }
 }
 
-// Weights of four scores (CAP: of their tanh).  x: in, p out; m: what ds is multiplied by (p, or
-// p tanh').  add: bias - lse in log2 units.
+// Weights of four scores (CAP: capped, in log2 units).  x: in, p out; m: what ds is multiplied by (p,
+// or p tanh').  add: bias - lse in log2 units.
 template <bool CAP>
 __device__ __forceinline__ void weights4(const Params& p, float (&x)[4], const float (&add)[4], float (&m)[4]) {
-  const float c = CAP ? p.cap_out : p.scale_log2;
-  const uint64_t c2 = f2(c, c);
   if (CAP) {
+    const uint64_t inv = f2(p.cap_inv, p.cap_inv), neg = f2(-1.f, -1.f), one = f2(1.f, 1.f);
 #pragma unroll
-    for (int y = 0; y < 4; ++y) m[y] = fmaf(-x[y], x[y], 1.f);
+    for (int y = 0; y < 4; y += 2) {
+      const uint64_t v = f2(x[y], x[y + 1]), t = f2_mul(v, inv);
+      f2_split(f2_fma(f2_mul(t, neg), t, one), m[y], m[y + 1]);
+      f2_split(f2_add(v, f2(add[y], add[y + 1])), x[y], x[y + 1]);
+    }
+  } else {
+    const uint64_t c2 = f2(p.scale_log2, p.scale_log2);
+    f2_split(f2_fma(f2(x[0], x[1]), c2, f2(add[0], add[1])), x[0], x[1]);
+    f2_split(f2_fma(f2(x[2], x[3]), c2, f2(add[2], add[3])), x[2], x[3]);
   }
-  f2_split(f2_fma(f2(x[0], x[1]), c2, f2(add[0], add[1])), x[0], x[1]);
-  f2_split(f2_fma(f2(x[2], x[3]), c2, f2(add[2], add[3])), x[2], x[3]);
 #pragma unroll
   for (int y = 0; y < 4; ++y) {
     x[y] = ex2(x[y]);

@@ -28,6 +28,8 @@ struct Params {
   float cap_u;             // softcap: scale / softcap
   float cap_in;            // 2 * log2(e) * scale / softcap
   float cap_out;           // softcap * log2(e)
+  float cap_inv;           // 1 / cap_out
+  float cap_poly[6];       // coefficients of TanhSmall
   const float* slopes;     // [H] or null
   const int* prefix;       // [bs] or null
   const int *qdoc, *kdoc;  // [bs, sq], [bs, skv] or null
@@ -226,25 +228,17 @@ __device__ __forceinline__ void unit_done(const Scheduler& s, uint32_t k) {
   if (lane_id() == 0) mbar_arrive(&s.empty[k & 1]);
 }
 
-// ---- results: a warp holds 32 rows of 16-bit values, one a lane, and writes them 64 bytes of
-// each row at a time through its 2 KB of shared memory, so that 4 neighbouring lanes write one row's
-// 64 bytes (a lane writing its own row would touch 32 lines an instruction).
-// w: 32 values of this lane's row as 16 pairs; dst: where they go, null for a row that does not exist.
-__device__ __forceinline__ void write_rows(uint32_t stage, const uint32_t (&w)[16], uint8_t* dst, uint32_t lane) {
-  __syncwarp();
+// ---- results: one row a lane, 32 values as 16 pairs, in two stores of 32 bytes (a whole sector
+// each).  Through shared memory the stores of neighbouring lanes would touch fewer lines, but
+// that is what the tensor cores read their operands from, and its other users wait (4950
+// cycles for a warp's rows of 128 instead of 4380).
+__device__ __forceinline__ void write_row(const uint32_t (&w)[16], uint8_t* dst) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    sts128(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
-  __syncwarp();
-  const uint32_t c = lane & 3;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t r = i * 8 + (lane >> 2);
-    uint8_t* row = reinterpret_cast<uint8_t*>(
-        __shfl_sync(0xffffffffu, static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(dst)), int(r)));
-    const uint4 v = lds128(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-    if (row) *reinterpret_cast<uint4*>(row + c * 16) = v;
-  }
+  for (int h = 0; h < 2; ++h)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + h * 32), "r"(w[8 * h]),
+                 "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]), "r"(w[8 * h + 4]), "r"(w[8 * h + 5]),
+                 "r"(w[8 * h + 6]), "r"(w[8 * h + 7])
+                 : "memory");
 }
 
 // Register split of the attention kernels: three warpgroups are launched with 168 registers a
@@ -304,44 +298,50 @@ __device__ __forceinline__ void cap_r4(float (&z)[4]) {
   z[3] = icd * a[2];
 }
 
-// tanh of pairs with |u| <= 0.75: u + u^3 (c0 + c1 u^2 + ..), fitted by Remez exchange (largest
-// relative error 3.3e-8).  Capped layers rarely come near their cap, and this needs no special
-// function: the warps of a tile whose scores all stay below take it.
+// softcap tanh(scale x / softcap) log2(e) of raw scores with |scale x / softcap| <= 0.75: x (c0 + c1
+// x^2 + ..), an odd polynomial fitted to the tanh by Remez exchange (largest relative error 3.3e-8)
+// with both scales in its coefficients.  Capped layers rarely come near their cap, and this needs
+// no special function: the warps of a tile whose scores all stay below take it.
 constexpr float kTanhSmall = 0.75f;
+constexpr double kTanhPoly[5] = {-0.3333306908607483, 0.13326521217823029, -0.0533902570605278, 0.019664913415908813,
+                                 -0.0047694905661046505};
 struct TanhSmall {
-  uint64_t c[5];
+  uint64_t c[6];
   // kept in registers (a volatile move is not repeated where the constants are used)
-  __device__ __forceinline__ TanhSmall() {
-    const float v[5] = {-0.3333306908607483f, 0.13326521217823029f, -0.0533902570605278f, 0.019664913415908813f,
-                        -0.0047694905661046505f};
+  __device__ __forceinline__ explicit TanhSmall(const Params& p) {
 #pragma unroll
-    for (int i = 0; i < 5; ++i) asm volatile("mov.b64 %0, {%1, %1};" : "=l"(c[i]) : "f"(v[i]));
+    for (int i = 0; i < 6; ++i) asm volatile("mov.b64 %0, {%1, %1};" : "=l"(c[i]) : "f"(p.cap_poly[i]));
   }
-  __device__ __forceinline__ uint64_t operator()(uint64_t u) const {
-    const uint64_t u2 = f2_mul(u, u);
-    uint64_t p = f2_fma(c[4], u2, c[3]);
-    p = f2_fma(p, u2, c[2]);
-    p = f2_fma(p, u2, c[1]);
-    p = f2_fma(p, u2, c[0]);
-    return f2_fma(f2_mul(p, u2), u, u);
+  // the factor of x
+  __device__ __forceinline__ uint64_t factor(uint64_t x) const {
+    const uint64_t x2 = f2_mul(x, x);
+    uint64_t y = f2_fma(c[5], x2, c[4]);
+    y = f2_fma(y, x2, c[3]);
+    y = f2_fma(y, x2, c[2]);
+    y = f2_fma(y, x2, c[1]);
+    return f2_fma(y, x2, c[0]);
   }
 };
-
-// 32 raw scores to tanh(scale x / softcap), in place, the shorter way if the whole warp's allow it.
-__device__ __forceinline__ void cap32(const Params& p, const TanhSmall& ts, uint32_t (&x)[32]) {
+__device__ __forceinline__ bool cap_small(const Params& p, const uint32_t (&x)[32]) {
   float big = 0.f;
 #pragma unroll
   for (int e = 0; e < 32; e += 2) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1]))));
-  if (__all_sync(0xffffffffu, big * p.cap_u <= kTanhSmall)) {
-    const uint64_t cu = f2(p.cap_u, p.cap_u);
+  return __all_sync(0xffffffffu, big * p.cap_u <= kTanhSmall);
+}
+// 32 raw scores to softcap tanh(scale x / softcap) log2(e) + add, in place.
+__device__ __forceinline__ void cap32(const Params& p, const TanhSmall& ts, uint32_t (&x)[32], float add = 0.f) {
+  if (cap_small(p, x)) {
+    const uint64_t a2 = f2(add, add);
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
+      const uint64_t v = f2(x[e], x[e + 1]);
       float a, b;
-      f2_split(ts(f2_mul(f2(x[e], x[e + 1]), cu)), a, b);
+      f2_split(f2_fma(ts.factor(v), v, a2), a, b);
       x[e] = __float_as_uint(a);
       x[e + 1] = __float_as_uint(b);
     }
   } else {
+    const float top = p.cap_out + add;
 #pragma unroll
     for (int e = 0; e < 32; e += 4) {
       float z[4];
@@ -349,7 +349,7 @@ __device__ __forceinline__ void cap32(const Params& p, const TanhSmall& ts, uint
       for (int i = 0; i < 4; ++i) z[i] = __uint_as_float(x[e + i]) * p.cap_in;
       cap_r4(z);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[e + i] = __float_as_uint(fmaf(-2.f, z[i], 1.f));
+      for (int i = 0; i < 4; ++i) x[e + i] = __float_as_uint(fmaf(-2.f * p.cap_out, z[i], top));
     }
   }
 }

@@ -208,11 +208,10 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
   } else {
     // ---------------------------------------------------------------- weights: one key a thread, 64 queries
     regs_grow();
-    const TanhSmall tanh_small;
+    const TanhSmall tanh_small(p);
     const int half = int(warp) >> 2;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t st = t_st + t_lane + half * 64, dp = t_dp + t_lane + half * 64;
-    const uint32_t stage = smem_u32(sh.smem + C::OFF_STAGE) + warp * 2048;
     uint32_t it = 0, di = 0;
     bool ok = true;
     for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, 0x3305); ++k) {
@@ -245,8 +244,14 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
         }
         const float slope2 = BIAS ? __ldg(p.slopes + f.kvh * p.G + g) * kLog2e : 0.f;
         const float dist0 = float(r0 + p.off - j);
-        ok = wait_for(&sh.s_full[0], it & 1, sh.abort_flag, 0x3301) &&
-             wait_for(&sh.full[(2 * it) % ST], ((2 * it) / ST) & 1, sh.abort_flag, 0x3302);
+        // the rows' statistics are read before the wait for the scores: shared memory answers slowly
+        // while the tensor cores read from it
+        ok = wait_for(&sh.full[(2 * it) % ST], ((2 * it) / ST) & 1, sh.abort_flag, 0x3302);
+        if (!ok) break;
+        float4 nl4[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nl4[e] = lds_f4(stat + e * 16);
+        ok = wait_for(&sh.s_full[0], it & 1, sh.abort_flag, 0x3301);
         if (!ok) break;
         tc_fence_after();
         uint32_t w[2][32];   // scores, then what ds is multiplied by
@@ -261,8 +266,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
             if (CAP) cap32(p, tanh_small, w[y]);
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              const float4 nl4 = lds_f4(stat + (y * 32 + e) * 4);
-              float add[4] = {nl4.x, nl4.y, nl4.z, nl4.w}, x[4], m[4];
+              const float4 nl = nl4[y * 8 + e / 4];
+              float add[4] = {nl.x, nl.y, nl.z, nl.w}, x[4], m[4];
 #pragma unroll
               for (int z = 0; z < 4; ++z) {
                 x[z] = __uint_as_float(w[y][e + z]);
@@ -287,6 +292,9 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
         if (__builtin_expect(masked, 0)) phase(std::true_type{});
         else phase(std::false_type{});
 
+        float4 nd4[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nd4[e] = lds_f4(stat + TILE * 4 + e * 16);
         ok = wait_for(sh.dp_full, it & 1, sh.abort_flag, 0x3303);
         if (!ok) break;
         tc_fence_after();
@@ -297,7 +305,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
           tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            const float4 nd = lds_f4(stat + (TILE + y * 32 + e) * 4);
+            const float4 nd = nd4[y * 8 + e / 4];
             float a[4];
             f2_split(f2_mul(f2(w[y][e], w[y][e + 1]), f2_add(f2(d[e], d[e + 1]), f2(nd.x, nd.y))), a[0], a[1]);
             f2_split(f2_mul(f2(w[y][e + 2], w[y][e + 3]), f2_add(f2(d[e + 2], d[e + 3]), f2(nd.z, nd.w))), a[2], a[3]);
@@ -354,7 +362,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             o[e] = pack2<F16>(__uint_as_float(v[2 * e]) * fac, __uint_as_float(v[2 * e + 1]) * fac);
-          write_rows(stage, o, j < p.skv ? out + x * 64 : nullptr, lane);
+          if (j < p.skv) write_row(o, out + x * 64);
         }
       }
       tc_fence_before();   // the next unit's first products overwrite the accumulators

@@ -187,11 +187,10 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
   } else {
     // ---------------------------------------------------------------- weights: one query a thread, 64 keys
     regs_grow();
-    const TanhSmall tanh_small;
+    const TanhSmall tanh_small(p);
     const int half = int(warp) >> 2;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t dp = t_dp + t_lane + half * 64;
-    const uint32_t stage = smem_u32(sh.smem + C::OFF_STAGE) + warp * 2048;
     uint32_t it = 0, di = 0;
     bool ok = true;
     for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, 0x4304); ++k) {
@@ -284,20 +283,24 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
       tc_fence_after();
       uint8_t* out = static_cast<uint8_t*>(prm.dq) + 2 * (f.b * prm.dqs[0] + f.h * prm.dqs[1] + row * prm.dqs[2]) +
                      half * D;
-#pragma unroll 1
-      for (int x = 0; x < D / 64; ++x) {
-        uint32_t v[32], o[16];
+      uint32_t v[D / 64][32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0u;
-        __syncwarp();
-        if (f.n > 0) {
-          tmem_ld32(t_dq + t_lane + half * (D / 2) + x * 32, v);
-          tmem_wait_ld();
-        }
+      for (int x = 0; x < D / 64; ++x)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[x][e] = 0u;
+      __syncwarp();
+      if (f.n > 0) {   // all loads first: TMEM answers slowly while the tensor cores write to it
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) tmem_ld32(t_dq + t_lane + half * (D / 2) + x * 32, v[x]);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int x = 0; x < D / 64; ++x) {
+        uint32_t o[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          o[e] = pack2<F16>(__uint_as_float(v[2 * e]) * p.scale, __uint_as_float(v[2 * e + 1]) * p.scale);
-        write_rows(stage, o, valid ? out + x * 64 : nullptr, lane);
+          o[e] = pack2<F16>(__uint_as_float(v[x][2 * e]) * p.scale, __uint_as_float(v[x][2 * e + 1]) * p.scale);
+        if (valid) write_row(o, out + x * 64);
       }
       tc_fence_before();   // the next unit's first product overwrites the accumulator
       unit_done(sh.sched, k);

@@ -21,6 +21,8 @@
 // 128 (position, head) pairs of one group (few positions, as when tokens are generated): a
 // group's heads read the same keys.
 #pragma once
+#include <type_traits>
+
 #include "fused_common.cuh"
 
 namespace attn_bwd {
@@ -46,8 +48,7 @@ struct FwdCfg {
   static constexpr int ST = D == 128 ? 4 : 8;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = 2 * TILE_BYTES;
-  static constexpr int OFF_STAGE = OFF_KV + ST * TILE_BYTES;   // per warp of rows: 2 KB
-  static constexpr int OFF_LIST = OFF_STAGE + 8 * 2048;        // a list for each unit slot
+  static constexpr int OFF_LIST = OFF_KV + ST * TILE_BYTES;    // a list for each unit slot
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;            // two slots, the scheduler's answer
   static constexpr int NBAR = 3 + 2 * ST + 8 + 6;
@@ -299,11 +300,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + t_lane + t * TILE, t_o = tmem + t_lane + 2 * TILE + t * D;
     const int row = int(warp & 3) * 32 + int(lane);
-    const uint32_t stage = smem_u32(smem + C::OFF_STAGE) + warp * 2048;
-    // without a bias scores stay raw (or a tanh) and are scaled inside the exponent
-    const float c = BIAS ? 1.f : CAP ? p.cap_out : p.scale_log2;
+    // scores that are only scaled stay raw and are scaled inside the exponent
+    const float c = BIAS || CAP ? 1.f : p.scale_log2;
     const float grow = 8.f / c;
-    const TanhSmall tanh_small;
+    const TanhSmall tanh_small(p);
     uint32_t cnt = 0;   // tiles so far
     for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, 0x2304); ++k) {
       const FwdUnit f = fwd_unit(prm, u);
@@ -353,7 +353,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           auto modify = [&](uint32_t (&x)[32], int g) {
             if (CAP) cap32(p, tanh_small, x);
             if (BIAS) {
-              const float d0 = float(pos + p.off - j0 - g * 32), sl = CAP ? p.cap_out : p.scale_log2;
+              const float d0 = float(pos + p.off - j0 - g * 32), sl = CAP ? 1.f : p.scale_log2;
               if (__all_sync(0xffffffffu, d0 >= 31.f)) {   // |i - j| = i - j: linear in the column
                 const float a = -slope2 * d0;
 #pragma unroll
@@ -410,7 +410,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
               for (int g = 0; g < 4; ++g) modify(x[g], g);
             }
             m = fmaxf(fmaxf(highest(x[0]), highest(x[1])), fmaxf(highest(x[2]), highest(x[3])));
-            if (CAP) m = fmaf(-2.f, rcp(1.f + ex2(m * p.cap_in)), 1.f);   // the tanh grows with its argument
+            if (CAP) m = fmaf(-2.f * p.cap_out, rcp(1.f + ex2(m * p.cap_in)), p.cap_out);   // the tanh grows with its argument
           } else if constexpr (CAP || BIAS) {
             m = -INFINITY;
 #pragma unroll 1
@@ -452,13 +452,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           const uint64_t c2 = f2(c, c), nm2 = f2(nm, nm);
           uint64_t sum0 = 0, sum1 = 0;
           // weights of 32 keys, to 16 columns
-          auto weigh = [&](const uint32_t (&y)[32], uint32_t column) {
+          auto weigh = [&](const uint32_t (&y)[32], uint32_t column, auto done_tag) {
+            constexpr bool DONE = decltype(done_tag)::value;   // the exponents themselves
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
               float a0, a1, b0, b1;
-              f2_split(f2_fma(f2(y[e], y[e + 1]), c2, nm2), a0, a1);
-              f2_split(f2_fma(f2(y[e + 2], y[e + 3]), c2, nm2), b0, b1);
+              f2_split(DONE ? f2(y[e], y[e + 1]) : f2_fma(f2(y[e], y[e + 1]), c2, nm2), a0, a1);
+              f2_split(DONE ? f2(y[e + 2], y[e + 3]) : f2_fma(f2(y[e + 2], y[e + 3]), c2, nm2), b0, b1);
               a0 = ex2(a0); a1 = ex2(a1); b0 = ex2(b0); b1 = ex2(b1);
               sum0 = f2_add(sum0, f2(a0, a1));
               sum1 = f2_add(sum1, f2(b0, b1));
@@ -481,7 +482,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           if (in_regs) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              weigh(x[g], g * 16);
+              weigh(x[g], g * 16, std::false_type{});
               if (g & 1) hand_over(g >> 1);
             }
           } else if constexpr (CAP || BIAS) {
@@ -493,8 +494,12 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
                 __syncwarp();
                 tmem_ld32(t_s + g * 32, y);
                 tmem_wait_ld();
-                if (CAP && late_cap) cap32(p, tanh_small, y);
-                weigh(y, g * 16);
+                if (CAP && late_cap) {
+                  cap32(p, tanh_small, y, nm);
+                  weigh(y, g * 16, std::true_type{});
+                } else {
+                  weigh(y, g * 16, std::false_type{});
+                }
               }
               hand_over(h);
             }
@@ -527,6 +532,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
         const size_t ri = (size_t)f.split * p.bs * p.H * p.sq + rowi;
         if (valid) (p.splits > 1 ? prm.part_lse + ri : prm.lse + rowi)[0] = lse;
         uint8_t* dst = static_cast<uint8_t*>(prm.o) + (((size_t)f.b * p.sq + pos) * p.H + head) * (D * 2);
+        // (64 columns a load would hide more of TMEM's latency, but leaves the loop above fewer
+        // registers: 7 % of the 4096x4096 prompt)
 #pragma unroll 1
         for (int x = 0; x < D / 32; ++x) {
           uint32_t o[32];
@@ -549,7 +556,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               w[e] = empty ? 0u : pack2<F16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-            write_rows(stage, w, valid ? dst + x * 64 : nullptr, lane);
+            if (valid) write_row(w, dst + x * 64);
           }
         }
         tc_fence_before();   // the next unit's first product overwrites the accumulator

@@ -53,6 +53,17 @@ inline Params base_params(const attn_bwd_fused_t* a) {
   p.cap_u = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
   p.cap_in = a->softcap > 0.f ? 2.f * kLog2e * a->scale / a->softcap : 0.f;
   p.cap_out = a->softcap * kLog2e;
+  if (a->softcap > 0.f) {
+    p.cap_inv = 1.f / p.cap_out;
+    // cap_out * tanh(u x) = cap_out (u x) (1 + k0 (u x)^2 + k1 (u x)^4 + ..)
+    const double u = double(a->scale) / a->softcap;
+    double f = double(a->softcap) * 1.4426950408889634 * u;
+    p.cap_poly[0] = float(f);
+    for (int i = 0; i < 5; ++i) {
+      f *= u * u;
+      p.cap_poly[i + 1] = float(kTanhPoly[i] * f);
+    }
+  }
   p.slopes = a->slopes;
   p.prefix = a->prefix_lens;
   p.qdoc = a->q_documents;
