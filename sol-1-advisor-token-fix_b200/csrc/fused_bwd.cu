@@ -39,49 +39,6 @@ static BwdLayout layout_bwd(const attn_bwd_fused_t* a, int sm_count) {
   return l;
 }
 
-// nlse and ndelta of every row (rows of padding get -inf and 0).  16 lanes a row.
-template <int D, bool F16>
-__global__ void __launch_bounds__(256) bwd_stats_kernel(const uint8_t* __restrict__ go, const uint8_t* __restrict__ o,
-                                                        const float* __restrict__ lse, float* __restrict__ nlse,
-                                                        float* __restrict__ ndelta, int bs, int sq, int sq_pad, int H) {
-  constexpr int L = D / 8;   // lanes a row: 16 bytes each
-  const long long idx = ((long long)blockIdx.x * 256 + threadIdx.x) / L;   // (b, position, head)
-  const int lane = threadIdx.x % L;
-  const long long total = (long long)bs * sq_pad * H;
-  const long long bp = idx / H, h = idx - bp * H, b = bp / sq_pad, pos = bp - b * sq_pad;
-  const bool in = idx < total;
-  float d = 0.f;
-  if (in && pos < sq) {
-    const long long at = ((b * sq + pos) * H + h) * (D * 2) + lane * 16;
-    const uint4 x = *reinterpret_cast<const uint4*>(go + at), y = *reinterpret_cast<const uint4*>(o + at);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 u = unpack2<F16>(xs[i]), v = unpack2<F16>(ys[i]);
-      d = fmaf(u.x, v.x, d);
-      d = fmaf(u.y, v.y, d);
-    }
-  }
-#pragma unroll
-  for (int k = L / 2; k; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
-  if (in && lane == 0) {
-    const float l = pos < sq ? lse[(b * H + h) * sq + pos] : -INFINITY;
-    const bool none = l == -INFINITY;
-    nlse[(b * H + h) * sq_pad + pos] = none ? -INFINITY : -l * kLog2e;
-    ndelta[(b * H + h) * sq_pad + pos] = none ? 0.f : -d;
-  }
-}
-
-template <int D, bool F16>
-static int launch_stats(const BwdParams& f, const void* go, const void* o, const float* lse, cudaStream_t s) {
-  const Params& p = f.c;
-  const long long threads = (long long)p.bs * f.sq_pad * p.H * (D / 8);
-  bwd_stats_kernel<D, F16><<<unsigned((threads + 255) / 256), 256, 0, s>>>(
-      static_cast<const uint8_t*>(go), static_cast<const uint8_t*>(o), lse, const_cast<float*>(f.nlse),
-      const_cast<float*>(f.ndelta), p.bs, p.sq, f.sq_pad, p.H);
-  return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;
-}
-
 }  // namespace fused
 }  // namespace attn_bwd
 
@@ -123,6 +80,8 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
   f.c.splits = l.splits;
   f.sq_pad = l.sq_pad;
   float* ws = static_cast<float*>(workspace);
+  f.o = static_cast<const uint8_t*>(o);
+  f.lse = lse;
   f.nlse = ws;
   f.ndelta = ws + l.stat / 4;
   f.n_kt = tiles_of(a->seq_kv);
@@ -163,11 +122,6 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_);
   const bool cap = a->softcap > 0.f;
   const int d = a->head_dim;
-  if (a->seq_q) {
-    rc = d == 128 ? (f16 ? launch_stats<128, true>(f, go, o, lse, s) : launch_stats<128, false>(f, go, o, lse, s))
-                  : (f16 ? launch_stats<64, true>(f, go, o, lse, s) : launch_stats<64, false>(f, go, o, lse, s));
-    if (rc) return rc;
-  }
   if (f.c.has_docs) {
     const long long tiles = (long long)a->bs * (f.c.n_tiles + f.n_kt);
     doc_ranges_kernel<<<unsigned((tiles + 7) / 8), 256, 0, s>>>(f.c.kdoc, a->seq_kv, f.c.qdoc, a->seq_q, a->bs,
@@ -175,7 +129,7 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
                                                                 const_cast<DocRange*>(f.c.qrange));
     if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
   }
-  if (a->seq_kv && (rc = launch_dkv(f, mq, md, mk, mv, d, f16, cap, s))) return rc;
   if (a->seq_q && (rc = launch_dq(f, mq, md, mk, mv, d, f16, cap, s))) return rc;
+  if (a->seq_kv && (rc = launch_dkv(f, mq, md, mk, mv, d, f16, cap, s))) return rc;
   return ATTN_BWD_OK;
 }

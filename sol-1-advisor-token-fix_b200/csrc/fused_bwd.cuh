@@ -7,7 +7,8 @@
 //   dkv: one key tile a CTA, streams the query tiles of all heads of the group.  It computes the
 //        transposed scores (keys are rows), so p^T and ds^T are A operands in TMEM and the sum over
 //        the group's heads happens in the accumulators.
-//   dq:  one query tile of one head a CTA, streams the key tiles.
+//   dq:  one query tile of one head a CTA, streams the key tiles.  It runs first and leaves the
+//        rows' statistics (delta from the resident do and a read of o) to dkv.
 // In both, warp 8 is the TMA producer, warp 9 issues tcgen05, warp 10 fetches units (and makes their
 // lists of tiles), and warps 0-7 turn scores into weights: TMEM lane quadrant warp % 4, columns
 // 64 * (warp / 4).. of each tile.
@@ -24,8 +25,10 @@ struct BwdParams {
   int sq_pad;            // sq rounded up to tiles: row length of nlse and ndelta
   int n_kt;              // key tiles
   FastDiv divH, divHkv;
-  const float* nlse;     // [bs * H, sq_pad]: -lse * log2(e); -inf for rows that see nothing
-  const float* ndelta;   // [bs * H, sq_pad]: -sum(do * o)
+  const uint8_t* o;      // [bs, sq, H, D]
+  const float* lse;      // [bs, H, sq]
+  float* nlse;           // [bs * H, sq_pad]: -lse * log2(e); -inf for rows that see nothing
+  float* ndelta;         // [bs * H, sq_pad]: -sum(do * o); dq writes both, dkv reads them
   void *dq, *dk, *dv;
   long long dqs[3], dks[3], dvs[3];   // element strides: batch, head, position
   float* part;           // dkv, splits > 1: [split][bs * Hkv * skv][2][D], dk first
@@ -37,7 +40,8 @@ struct BwdCfg {
   static constexpr int ST = 4;
   static constexpr int OFF_A = 0;                               // two resident tiles
   static constexpr int OFF_RING = 2 * TILE_BYTES;
-  static constexpr int OFF_STAT = OFF_RING + ST * TILE_BYTES;   // dkv: 2 x (nlse, ndelta) of 128 rows
+  // dkv: 2 x (nlse, ndelta) of 128 rows; dq: 2 x (halves of 128 rows' delta)
+  static constexpr int OFF_STAT = OFF_RING + ST * TILE_BYTES;
   static constexpr int OFF_LIST = OFF_STAT + 2 * 2 * TILE * 4;
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;
@@ -82,13 +86,14 @@ __device__ __forceinline__ BwdShared bwd_shared(uint8_t* raw) {
   s.lists = reinterpret_cast<uint16_t*>(s.smem + C::OFF_LIST);
   return s;
 }
-// Barriers, descriptors and TMEM; returns the TMEM base.
-__device__ __forceinline__ uint32_t bwd_begin(const BwdShared& s, int st, const CUtensorMap* q, const CUtensorMap* go,
+// Barriers, descriptors and TMEM; returns the TMEM base.  res_users: arrivals that free the resident
+// tiles.
+__device__ __forceinline__ uint32_t bwd_begin(const BwdShared& s, int st, int res_users, const CUtensorMap* q, const CUtensorMap* go,
                                               const CUtensorMap* k, const CUtensorMap* v) {
   const uint32_t warp = warp_id(), lane = lane_id();
   if (threadIdx.x == 0) {
     mbar_init(s.res_full, 1);
-    mbar_init(s.res_empty, 1);
+    mbar_init(s.res_empty, res_users);
     mbar_init(s.all_done, 1);
     for (int i = 0; i < st; ++i) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 1); }
     mbar_init(&s.s_full[0], 1);

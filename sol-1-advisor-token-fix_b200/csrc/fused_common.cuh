@@ -179,6 +179,16 @@ __device__ __forceinline__ bool read_answer(const Scheduler& s, int& x, int& y, 
       : "memory");
   return ok != 0;
 }
+// L2 prefetches for the unit that comes next, by the scheduler warp: its resident tiles are asked
+// for only when this unit has done with their place.
+__device__ __forceinline__ void prefetch_l2_4d(const CUtensorMap* m, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory"); }
+
 constexpr int kUnitReaders = 10;   // producer, tensor cores, 8 warps of rows
 __device__ __forceinline__ void scheduler_init(const Scheduler& s) {
   for (int i = 0; i < 2; ++i) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], kUnitReaders); }

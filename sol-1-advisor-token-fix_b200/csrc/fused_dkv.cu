@@ -51,7 +51,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
   const BwdShared sh = bwd_shared<D>(smem_raw);
   const Params& p = prm.c;
   const uint32_t warp = warp_id(), lane = lane_id();
-  const uint32_t tmem = bwd_begin(sh, ST, &tm_q, &tm_do, &tm_k, &tm_v);
+  const uint32_t tmem = bwd_begin(sh, ST, 1, &tm_q, &tm_do, &tm_k, &tm_v);
   const uint32_t t_st = tmem, t_dp = tmem + TILE, t_dv = tmem + 2 * TILE, t_dk = t_dv + D;
   Unit u;
 
@@ -187,8 +187,10 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
     } else if (warp == 10) {
       // -------------------------------------------------------------- units and their lists
       run_scheduler(sh.sched, sh.abort_flag, 0x3401, [&](int x, int y, int z, uint32_t slot) {
-        if (!p.has_docs) return 0;
         const DkvUnit f = dkv_unit(prm, Unit{x, y, z, 0});
+        if (int(lane) < 2 * (D / 64))
+          prefetch_l2_4d(int(lane) & 1 ? &tm_v : &tm_k, (int(lane) >> 1) * 64, f.j0, f.kvh, f.b);
+        if (!p.has_docs) return 0;
         const DocRange kd = prm.c.krange[(size_t)f.b * prm.n_kt + f.j0 / TILE];
         int n = 0;
         for (int t = f.t_lo; t < p.n_tiles; t += 32) {
@@ -298,31 +300,36 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
         ok = wait_for(sh.dp_full, it & 1, sh.abort_flag, 0x3303);
         if (!ok) break;
         tc_fence_after();
+        auto gradients = [&](auto mask_tag) {
+          constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          uint32_t d[32], pk[16];
-          tmem_ld32(dp + y * 32, d);
-          tmem_wait_ld();
+          for (int y = 0; y < 2; ++y) {
+            uint32_t d[32], pk[16];
+            tmem_ld32(dp + y * 32, d);
+            tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 nd = nd4[y * 8 + e / 4];
-            float a[4];
-            f2_split(f2_mul(f2(w[y][e], w[y][e + 1]), f2_add(f2(d[e], d[e + 1]), f2(nd.x, nd.y))), a[0], a[1]);
-            f2_split(f2_mul(f2(w[y][e + 2], w[y][e + 3]), f2_add(f2(d[e + 2], d[e + 3]), f2(nd.z, nd.w))), a[2], a[3]);
-            if (masked) {   // p is 0 there already, but dp of padding may be NaN
+            for (int e = 0; e < 32; e += 4) {
+              const float4 nd = nd4[y * 8 + e / 4];
+              float a[4];
+              f2_split(f2_mul(f2(w[y][e], w[y][e + 1]), f2_add(f2(d[e], d[e + 1]), f2(nd.x, nd.y))), a[0], a[1]);
+              f2_split(f2_mul(f2(w[y][e + 2], w[y][e + 3]), f2_add(f2(d[e + 2], d[e + 3]), f2(nd.z, nd.w))), a[2], a[3]);
+              if (MASK) {   // p is 0 there already, but dp of padding may be NaN
 #pragma unroll
-              for (int z = 0; z < 4; ++z)
-                if (!((see[y] >> (e + z)) & 1u)) a[z] = 0.f;
+                for (int z = 0; z < 4; ++z)
+                  if (!((see[y] >> (e + z)) & 1u)) a[z] = 0.f;
+              }
+              pk[e / 2] = pack2<F16>(a[0], a[1]);
+              pk[e / 2 + 1] = pack2<F16>(a[2], a[3]);
             }
-            pk[e / 2] = pack2<F16>(a[0], a[1]);
-            pk[e / 2 + 1] = pack2<F16>(a[2], a[3]);
+            tmem_st16(dp + y * 16, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.ds_ready[y]);
           }
-          tmem_st16(dp + y * 16, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.ds_ready[y]);
-        }
+        };
+        if (__builtin_expect(masked, 0)) gradients(std::true_type{});
+        else gradients(std::false_type{});
         if (++t == f.nl) { t = 0; ++g; }
       }
       if (!ok) break;

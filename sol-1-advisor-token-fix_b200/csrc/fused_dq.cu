@@ -35,7 +35,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
   const BwdShared sh = bwd_shared<D>(smem_raw);
   const Params& p = prm.c;
   const uint32_t warp = warp_id(), lane = lane_id();
-  const uint32_t tmem = bwd_begin(sh, ST, &tm_q, &tm_do, &tm_k, &tm_v);
+  const uint32_t tmem = bwd_begin(sh, ST, 9, &tm_q, &tm_do, &tm_k, &tm_v);
   const uint32_t t_dp = tmem + 2 * TILE, t_dq = tmem + 3 * TILE;
   Unit u;
 
@@ -165,8 +165,13 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
     } else if (warp == 10) {
       // -------------------------------------------------------------- units and their lists
       run_scheduler(sh.sched, sh.abort_flag, 0x4401, [&](int x, int y, int z, uint32_t slot) {
-        if (!p.has_docs) return 0;
         const DqUnit f = dq_unit(prm, Unit{x, y, z, 0});
+        if (int(lane) < 2 * (D / 64))
+          prefetch_l2_4d(int(lane) & 1 ? &tm_do : &tm_q, (int(lane) >> 1) * 64, f.r0, f.h, f.b);
+        for (int r = f.r0 + int(lane); r <= f.r1; r += 32)
+          for (int c = 0; c < D * 2; c += 128)
+            prefetch_l2(prm.o + (((size_t)f.b * p.sq + r) * p.H + f.h) * (D * 2) + c);
+        if (!p.has_docs) return 0;
         const DocRange qd = p.qrange[(size_t)f.b * p.n_tiles + f.r0 / TILE];
         const int t1 = max(0, row_limit(p, f.r1, f.pre) + TILE - 1) / TILE;
         int n = 0;
@@ -187,6 +192,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
   } else {
     // ---------------------------------------------------------------- weights: one query a thread, 64 keys
     regs_grow();
+    constexpr int NC = D / 16;   // 16-byte words of half a row
     const TanhSmall tanh_small(p);
     const int half = int(warp) >> 2;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
@@ -198,12 +204,22 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
       const uint16_t* list = sh.lists + (k & 1) * kMaxList;
       const int row = f.r0 + int(warp & 3) * 32 + int(lane);
       const bool valid = row < p.sq;
-      const size_t ri = ((size_t)f.b * p.H + f.h) * prm.sq_pad + row;
-      const float nlse = prm.nlse[ri], nd = prm.ndelta[ri];   // padded to whole tiles
+      const size_t ri = ((size_t)f.b * p.H + f.h) * prm.sq_pad + row;   // padded to whole tiles
+      const float lse = valid ? __ldg(prm.lse + ((size_t)f.b * p.H + f.h) * p.sq + row) : -INFINITY;
+      const bool none = lse == -INFINITY;   // the row sees nothing
+      const float nlse = none ? -INFINITY : -lse * kLog2e;
+      uint4 ov[NC];   // this half of the row of o, for delta
+      const uint8_t* orow = prm.o + (((size_t)f.b * p.sq + (valid ? row : f.r0)) * p.H + f.h) * (D * 2) + half * D;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) ov[c] = __ldg(reinterpret_cast<const uint4*>(orow) + c);
+      uint64_t nd2 = 0;
       const int lim = valid ? row_limit(p, row, f.pre) : 0;
       const int qd = (valid && p.has_docs) ? __ldg(p.qdoc + (size_t)f.b * p.sq + row) : -1;
       const float slope2 = BIAS ? __ldg(p.slopes + f.h) * kLog2e : 0.f;
-      const uint64_t nd2 = f2(nd, nd);
+      if (f.n == 0 && half == 0) {   // no tile, so no key tile asks for these
+        prm.nlse[ri] = -INFINITY;
+        prm.ndelta[ri] = 0.f;
+      }
       for (int i = 0; i < f.n; ++i, ++it) {
         const uint32_t ent = p.has_docs ? list[i] : 0u;
         const int t0 = (p.has_docs ? int(ent & kEntTile) : i) * TILE, j0 = t0 + half * 64;
@@ -247,31 +263,68 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
               for (int z = 0; z < 4; ++z) w[y][e + z] = __float_as_uint(m[z]);
           }
         }
+        if (i == 0) {
+          // delta of the row: each half of the warps takes half of the columns
+          ok = wait_for(sh.res_full, di & 1, sh.abort_flag, 0x4305);
+          if (!ok) break;
+          const int r = int(warp & 3) * 32 + int(lane);
+          float d = 0.f;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const int cg = half * NC + c;
+            const uint4 g = lds128(smem_u32(sh.smem + C::OFF_A + C::TILE_BYTES) + (cg >> 3) * (TILE * 128) + r * 128 +
+                                   (((cg & 7) ^ (r & 7)) << 4));
+            const uint32_t gs[4] = {g.x, g.y, g.z, g.w}, os[4] = {ov[c].x, ov[c].y, ov[c].z, ov[c].w};
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const float2 u = unpack2<F16>(gs[z]), v = unpack2<F16>(os[z]);
+              d = fmaf(u.x, v.x, d);
+              d = fmaf(u.y, v.y, d);
+            }
+          }
+          float* part = reinterpret_cast<float*>(sh.smem + C::OFF_STAT) + (k & 1) * (2 * TILE);
+          part[half * TILE + r] = d;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sh.res_empty);
+          named_bar_sync(1 + (warp & 3), 64);   // the two warps of these rows
+          d += part[(half ^ 1) * TILE + r];     // a sum of two: the same in either order
+          const float nd = none ? 0.f : -d;
+          nd2 = f2(nd, nd);
+          if (half == 0) {
+            prm.nlse[ri] = nlse;
+            prm.ndelta[ri] = nd;
+          }
+        }
         // masked scores are taken out of ds below
         ok = wait_for(sh.dp_full, it & 1, sh.abort_flag, 0x4302);
         if (!ok) break;
         tc_fence_after();
+        auto gradients = [&](auto mask_tag) {
+          constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          uint32_t d[32], pk[16];
-          tmem_ld32(dp + y * 32, d);
-          tmem_wait_ld();
+          for (int y = 0; y < 2; ++y) {
+            uint32_t d[32], pk[16];
+            tmem_ld32(dp + y * 32, d);
+            tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float a0, a1;
-            f2_split(f2_mul(f2(w[y][e], w[y][e + 1]), f2_add(f2(d[e], d[e + 1]), nd2)), a0, a1);
-            if (masked) {
-              if (!((see[y] >> e) & 1u)) a0 = 0.f;
-              if (!((see[y] >> (e + 1)) & 1u)) a1 = 0.f;
+            for (int e = 0; e < 32; e += 2) {
+              float a0, a1;
+              f2_split(f2_mul(f2(w[y][e], w[y][e + 1]), f2_add(f2(d[e], d[e + 1]), nd2)), a0, a1);
+              if (MASK) {
+                if (!((see[y] >> e) & 1u)) a0 = 0.f;
+                if (!((see[y] >> (e + 1)) & 1u)) a1 = 0.f;
+              }
+              pk[e / 2] = pack2<F16>(a0, a1);
             }
-            pk[e / 2] = pack2<F16>(a0, a1);
+            tmem_st16(st + y * 16, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.ds_ready[y]);
           }
-          tmem_st16(st + y * 16, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.ds_ready[y]);
-        }
+        };
+        if (__builtin_expect(masked, 0)) gradients(std::true_type{});
+        else gradients(std::false_type{});
       }
       if (!ok) break;
       // ---- epilogue: each half of the warps writes half of the columns

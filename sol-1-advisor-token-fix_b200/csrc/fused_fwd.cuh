@@ -147,6 +147,17 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     prefetch_tmap(&tm_v);
   }
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (prm.packed) {
+    // rows behind the last (position, head) pair of a tile are never loaded; what stood there
+    // would take part in the warps' votes, and results would not be the same bits each time
+    const int r0 = prm.pos_per_tile * p.G, n = (TILE - r0) * (D / 8);
+    for (int i = int(threadIdx.x); i < 2 * n; i += kThreads) {
+      const int t = i >= n ? 1 : 0, j = i - t * n, c = j % (D / 8), r = r0 + j / (D / 8);
+      sts128(smem_u32(smem + C::OFF_Q + t * C::TILE_BYTES + (c >> 3) * (TILE * 128)) + r * 128 + (c & 7) * 16,
+             make_uint4(0, 0, 0, 0));
+    }
+    fence_proxy_async_smem();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -272,8 +283,12 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     } else if (warp == 10) {
       // -------------------------------------------------------------- units and their lists
       run_scheduler(sched, abort_flag, 0x2401, [&](int x, int y, int z, uint32_t slot) {
-        if (!p.has_docs) return 0;
         const FwdUnit f = fwd_unit(prm, Unit{x, y, z, 0});
+        if (int(lane) < f.nt * (D / 64)) {
+          const int t = int(lane) / (D / 64);
+          prefetch_l2_4d(&tm_q, int(lane) % (D / 64) * 64, t ? f.head[1] : f.head[0], t ? f.pos[1] : f.pos[0], f.b);
+        }
+        if (!p.has_docs) return 0;
         const DocRange qd = warp_doc_range(p.qdoc + (size_t)f.b * p.sq + f.pos[0], f.last_pos - f.pos[0] + 1, lane);
         const int hi = max(0, row_limit(p, f.last_pos, f.pre) + TILE - 1) / TILE;
         const int t1 = min(min(p.n_tiles, f.t0 + p.tiles_per_split), hi);
