@@ -369,16 +369,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             if (CAP) cap32(p, tanh_small, x);
             if (BIAS) {
               const float d0 = float(pos + p.off - j0 - g * 32), sl = CAP ? 1.f : p.scale_log2;
-              if (__all_sync(0xffffffffu, d0 >= 31.f)) {   // |i - j| = i - j: linear in the column
-                const float a = -slope2 * d0;
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), sl, fmaf(slope2, float(e), a)));
-              } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), sl, -slope2 * fabsf(d0 - float(e))));
-              }
+              for (int e = 0; e < 32; ++e)
+                x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), sl, -slope2 * fabsf(d0 - float(e))));
             }
             if (__builtin_expect(masked, 0)) {
               uint32_t see = low_bits(lim - j0 - g * 32);
