@@ -364,6 +364,16 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           //   anything else: scores are rewritten in TMEM, 32 at a time, then read again.
           // (All of it on 128 scores in registers spilled, and a row read twice cost the plain
           // case 10 % of the 4096x4096 prompt.)
+          auto hide = [&](uint32_t (&x)[32], int g) {   // -inf to the keys that are not seen
+            uint32_t see = low_bits(lim - j0 - g * 32);
+            if (p.has_docs) {
+              const int j = j0 + g * 32 + int(lane);
+              see &= same_id(j < p.skv ? __ldg(p.kdoc + (size_t)f.b * p.skv + j) : -1, qd);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((see >> e) & 1u)) x[e] = 0xff800000u;
+          };
           // 32 scores from column 32 g on: cap, bias, mask (log2 units / c, -inf where not seen)
           auto modify = [&](uint32_t (&x)[32], int g) {
             if (CAP) cap32(p, tanh_small, x);
@@ -373,16 +383,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
               for (int e = 0; e < 32; ++e)
                 x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), sl, -slope2 * fabsf(d0 - float(e))));
             }
-            if (__builtin_expect(masked, 0)) {
-              uint32_t see = low_bits(lim - j0 - g * 32);
-              if (p.has_docs) {
-                const int j = j0 + g * 32 + int(lane);
-                see &= same_id(j < p.skv ? __ldg(p.kdoc + (size_t)f.b * p.skv + j) : -1, qd);
-              }
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((see >> e) & 1u)) x[e] = 0xff800000u;   // -inf
-            }
+            if (__builtin_expect(masked, 0)) hide(x, g);
           };
           auto highest = [](const uint32_t (&x)[32]) {
             float y[2];
@@ -396,7 +397,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             return fmaxf(y[0], y[1]);
           };
           const bool linear = BIAS && __all_sync(0xffffffffu, pos + p.off >= j0 + TILE - 1);
-          const bool in_regs = !CAP && (!BIAS || (!masked && linear));
+          const bool in_regs = !CAP && (!BIAS || linear);
           const bool late_cap = CAP && !BIAS && !masked;
           uint32_t x[4][32];
           float m;
@@ -413,9 +414,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
                   x[g][e] = __float_as_uint(
                       fmaf(__uint_as_float(x[g][e]), p.scale_log2, fmaf(slope2, float(g * 32 + e), a)));
             }
-            if (!CAP && !BIAS && __builtin_expect(masked, 0)) {
+            if (!CAP && __builtin_expect(masked, 0)) {
 #pragma unroll
-              for (int g = 0; g < 4; ++g) modify(x[g], g);
+              for (int g = 0; g < 4; ++g) hide(x[g], g);
             }
             m = fmaxf(fmaxf(highest(x[0]), highest(x[1])), fmaxf(highest(x[2]), highest(x[3])));
             if (CAP) m = fmaf(-2.f * p.cap_out, rcp(1.f + ex2(m * p.cap_in)), p.cap_out);   // the tanh grows with its argument
