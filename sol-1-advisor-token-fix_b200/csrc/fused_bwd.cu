@@ -20,7 +20,9 @@ static int dkv_splits(const attn_bwd_fused_t* a, int sm_count) {
   if (units == 0) return 1;
   long long s = sm_count / units;
   if (s > items) s = items;
-  return s < 1 ? 1 : int(s);
+  if (s <= 1) return 1;
+  const long long per = (items + s - 1) / s;
+  return int((items + per - 1) / per);   // no split without items
 }
 
 struct BwdLayout {

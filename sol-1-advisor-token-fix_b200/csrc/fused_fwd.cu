@@ -30,6 +30,9 @@ static FwdParams plan_fwd(const attn_bwd_fused_t* a, int sm_count) {
   p.n_tiles = (p.skv + TILE - 1) / TILE;
   // Too few units for the GPU: split the keys, two tiles a split at least (below that the
   // join costs more than it saves), and never more tiles than a unit's list holds.
+  // (two chains in a CTA: the same two tiles for each)
+  f.duo = p.n_tiles > 1 && !f.pair_heads && f.blocks_q == 1 && p.sq <= f.pos_per_tile;
+  const int parts = f.duo ? 2 : 1;
   const long long units = (long long)f.blocks_q * f.head_slots * p.bs;
   long long splits = units > 0 ? sm_count / units : 1;
   if (splits > p.n_tiles / 2) splits = p.n_tiles / 2;
@@ -38,8 +41,9 @@ static FwdParams plan_fwd(const attn_bwd_fused_t* a, int sm_count) {
   if (splits < 1) splits = 1;
   p.tiles_per_split = int((p.n_tiles + splits - 1) / splits);
   if (p.tiles_per_split < 1) p.tiles_per_split = 1;
-  p.splits = (p.n_tiles + p.tiles_per_split - 1) / p.tiles_per_split;
-  if (p.splits < 1) p.splits = 1;
+  f.cta_splits = (p.n_tiles + p.tiles_per_split - 1) / p.tiles_per_split;
+  if (f.cta_splits < 1) f.cta_splits = 1;
+  p.splits = f.cta_splits * parts;
   return f;
 }
 
@@ -54,28 +58,7 @@ int64_t fwd_workspace(const attn_bwd_fused_t* a, int sm_count) {
   return range_bytes(f.c) + part_rows(f.c) * (a->head_dim + 1) * 4;
 }
 
-template <int D, bool F16, bool CAP, bool BIAS>
-static int launch(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
-                  cudaStream_t stream) {
-  using C = FwdCfg<D>;
-  auto kern = fwd_kernel<D, F16, CAP, BIAS>;
-  const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
-  if (rc) return rc;
-  if (f.c.has_docs && f.c.n_tiles > 0) {
-    const long long tiles = (long long)f.c.bs * f.c.n_tiles;
-    doc_ranges_kernel<<<unsigned((tiles + 7) / 8), 256, 0, stream>>>(f.c.kdoc, f.c.skv, nullptr, 0, f.c.bs,
-                                                                    const_cast<DocRange*>(f.c.krange), nullptr);
-    if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
-  }
-  kern<<<dim3(unsigned(f.blocks_q) * f.head_slots, f.c.bs, f.c.splits), kThreads, C::SMEM_BYTES, stream>>>(q, k, v, f);
-  if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
-  if (f.c.splits > 1) {
-    const long long rows = (long long)f.c.bs * f.c.H * f.c.sq;
-    fwd_join_kernel<D, F16><<<unsigned((rows + 7) / 8), 256, 0, stream>>>(f);
-    if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
-  }
-  return ATTN_BWD_OK;
-}
+ATTN_BWD_FWD_LAUNCHER(launch_fwd, false)
 
 }  // namespace fused
 }  // namespace attn_bwd
@@ -95,7 +78,7 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
   p.err = dev.err;
   f.o = o;
   f.lse = lse;
-  if (f.blocks_q > (1 << 30) / f.head_slots || p.splits > 65535) return ATTN_BWD_EINVAL;
+  if (f.blocks_q > (1 << 30) / f.head_slots || f.cta_splits > 65535) return ATTN_BWD_EINVAL;
   const int64_t need = range_bytes(p) + part_rows(p) * (a->head_dim + 1) * 4;
   if (need) {
     if (!workspace || workspace_bytes < need) return ATTN_BWD_EINVAL;
@@ -116,15 +99,23 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
     return ATTN_BWD_ETMAP;
   if (p.skv == 0) mk = mv = mq;   // never loaded from, only prefetched
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_);
-  const bool cap = a->softcap > 0.f, bias = a->slopes != nullptr;
-#define ATTN_BWD_FWD(DD, FF)                                                                          \
-  if (a->head_dim == DD && f16 == FF)                                                                \
-    return cap ? (bias ? launch<DD, FF, true, true>(f, mq, mk, mv, s) : launch<DD, FF, true, false>(f, mq, mk, mv, s)) \
-               : (bias ? launch<DD, FF, false, true>(f, mq, mk, mv, s) : launch<DD, FF, false, false>(f, mq, mk, mv, s));
-  ATTN_BWD_FWD(128, false)
-  ATTN_BWD_FWD(128, true)
-  ATTN_BWD_FWD(64, false)
-  ATTN_BWD_FWD(64, true)
-#undef ATTN_BWD_FWD
-  return ATTN_BWD_EUNSUPPORTED;
+  const bool cap = a->softcap > 0.f;
+  if (p.has_docs && p.n_tiles > 0) {
+    const long long tiles = (long long)p.bs * p.n_tiles;
+    doc_ranges_kernel<<<unsigned((tiles + 7) / 8), 256, 0, s>>>(p.kdoc, p.skv, nullptr, 0, p.bs,
+                                                               const_cast<DocRange*>(p.krange), nullptr);
+    if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
+  }
+  rc = f.duo ? launch_token(f, mq, mk, mv, a->head_dim, f16, cap, s) : launch_fwd(f, mq, mk, mv, a->head_dim, f16, cap, s);
+  if (rc || p.splits == 1) return rc;
+  const long long rows = (long long)p.bs * p.H * p.sq;
+  const dim3 grid(unsigned((rows + 7) / 8));
+  if (a->head_dim == 128) {
+    if (f16) fwd_join_kernel<128, true><<<grid, 256, 0, s>>>(f);
+    else fwd_join_kernel<128, false><<<grid, 256, 0, s>>>(f);
+  } else {
+    if (f16) fwd_join_kernel<64, true><<<grid, 256, 0, s>>>(f);
+    else fwd_join_kernel<64, false><<<grid, 256, 0, s>>>(f);
+  }
+  return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;
 }

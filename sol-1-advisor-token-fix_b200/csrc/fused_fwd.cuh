@@ -17,6 +17,10 @@
 // more than 2^8, so most tiles need no pass over it.  Weights are then at most 2^8 instead of
 // 1, which neither fp32 sums nor 16-bit weights (relative rounding) notice.
 //
+// Where all rows of a unit fit one tile (generated tokens), the two sets of warps take alternate key
+// tiles for the same rows instead (DUO): what bounds such a unit is the chain of scores, softmax and
+// product per tile, and two chains run side by side.  Each leaves its part to be joined.
+//
 // Rows of a query tile are 128 positions of one head or, where that needs fewer tiles, up to
 // 128 (position, head) pairs of one group (few positions, as when tokens are generated): a
 // group's heads read the same keys.
@@ -30,8 +34,10 @@ namespace fused {
 
 struct FwdParams {
   Params c;
+  int cta_splits;      // splits of the grid; DUO leaves two parts each
   int packed;          // rows are (position, head of the group) pairs
   int pos_per_tile;    // positions of a tile: 128, or 128 / G
+  int duo;             // all rows of a unit in one tile: two chains over alternate key tiles
   int pair_heads;      // unpacked: the two tiles are two heads of one group, else 256 positions
   int blocks_q;        // position blocks per (batch, head slot)
   int head_slots;      // units along the heads: kv heads, head pairs or heads
@@ -42,12 +48,13 @@ struct FwdParams {
   float* part_lse;     // splits > 1: [split][bs * H * sq]
 };
 
-template <int D>
+template <int D, bool DUO>
 struct FwdCfg {
   static constexpr int TILE_BYTES = TILE * D * 2;
-  static constexpr int ST = D == 128 ? 4 : 8;
+  static constexpr int QT = DUO ? 1 : 2;                       // query tiles
+  static constexpr int ST = (D == 128 ? 6 : 10) - QT;          // stages of keys or values
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_KV = 2 * TILE_BYTES;
+  static constexpr int OFF_KV = QT * TILE_BYTES;
   static constexpr int OFF_LIST = OFF_KV + ST * TILE_BYTES;    // a list for each unit slot
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;            // two slots, the scheduler's answer
@@ -99,12 +106,12 @@ __device__ __forceinline__ FwdUnit fwd_unit(const FwdParams& prm, const Unit& u)
   f.n = p.has_docs ? u.n : max(0, min(min(p.n_tiles, f.t0 + p.tiles_per_split), hi) - f.t0);
   return f;
 }
-template <int D, bool F16, bool CAP, bool BIAS>
+template <int D, bool F16, bool CAP, bool BIAS, bool DUO>
 __global__ void __launch_bounds__(kThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64, heads of a row, positions, 1)
            const __grid_constant__ CUtensorMap tm_k,   // (d, s, h, b), box (64, 128, 1, 1)
            const __grid_constant__ CUtensorMap tm_v, const FwdParams prm) {
-  using C = FwdCfg<D>;
+  using C = FwdCfg<D, DUO>;
   constexpr int ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -151,7 +158,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     // rows behind the last (position, head) pair of a tile are never loaded; what stood there
     // would take part in the warps' votes, and results would not be the same bits each time
     const int r0 = prm.pos_per_tile * p.G, n = (TILE - r0) * (D / 8);
-    for (int i = int(threadIdx.x); i < 2 * n; i += kThreads) {
+    for (int i = int(threadIdx.x); i < C::QT * n; i += kThreads) {
       const int t = i >= n ? 1 : 0, j = i - t * n, c = j % (D / 8), r = r0 + j / (D / 8);
       sts128(smem_u32(smem + C::OFF_Q + t * C::TILE_BYTES + (c >> 3) * (TILE * 128)) + r * 128 + (c & 7) * 16,
              make_uint4(0, 0, 0, 0));
@@ -168,7 +175,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     regs_shrink();
     if (warp == 8) {
       // -------------------------------------------------------------- producer
-      uint32_t si = 0, qi = 0;   // key / value tiles, query tiles loaded so far
+      uint32_t si = 0, qi = 0, round = 0;   // key / value tiles, query tiles loaded so far; DUO: rounds
       for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, 0x2103); ++k) {
         const FwdUnit f = fwd_unit(prm, u);
         const uint16_t* list = lists + (k & 1) * kMaxList;
@@ -187,25 +194,41 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
                             t ? f.head[1] : f.head[0], t ? f.pos[1] : f.pos[0], f.b);
           }
         }
-        for (int i = 0; i < f.n && ok; ++i) {
+        // a key (m = 0) or value tile into the stage of ring index r
+        auto load = [&](uint32_t r, int i, int m) {
           const int j0 = (f.t0 + (p.has_docs ? int(list[i] & kEntTile) : i)) * TILE;
-          for (int m = 0; m < 2; ++m) {
-            const uint32_t s = si % ST;
-            ok = wait_for(&kv_empty[s], ((si / ST) & 1) ^ 1, abort_flag, 0x2101);
-            if (!ok) break;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&kv_full[s], C::TILE_BYTES);
-              for (int x = 0; x < D / 64; ++x)
-                tma_load_4d(smem + C::OFF_KV + s * C::TILE_BYTES + x * (TILE * 128), m ? &tm_v : &tm_k, &kv_full[s],
-                            x * 64, j0, f.kvh, f.b);
-            }
-            ++si;
+          const uint32_t s = r % ST;
+          if (!wait_for(&kv_empty[s], ((r / ST) & 1) ^ 1, abort_flag, 0x2101)) return false;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&kv_full[s], C::TILE_BYTES);
+            for (int x = 0; x < D / 64; ++x)
+              tma_load_4d(smem + C::OFF_KV + s * C::TILE_BYTES + x * (TILE * 128), m ? &tm_v : &tm_k, &kv_full[s],
+                          x * 64, j0, f.kvh, f.b);
           }
+          return true;
+        };
+        auto pass = [&](uint32_t r) {
+          if (!wait_for(&kv_empty[r % ST], ((r / ST) & 1) ^ 1, abort_flag, 0x2104)) return false;
+          if (lane == 0) mbar_arrive(&kv_full[r % ST]);
+          return true;
+        };
+        if (DUO) {
+          // rounds of four stages: keys of both chains, values of both; after a last odd tile two
+          // stages of its round are passed on as they are
+          for (int i = 0; i < f.n && ok; i += 2, ++round) {
+            const bool two = i + 1 < f.n;
+            ok = load(4 * round, i, 0) && (!two || load(4 * round + 1, i + 1, 0)) && load(4 * round + 2, i, 1) &&
+                 (!two || load(4 * round + 3, i + 1, 1));
+            if (ok && !two) ok = pass(4 * round + 1) && pass(4 * round + 3);
+          }
+        } else {
+          for (int i = 0; i < f.n && ok; ++i, si += 2) ok = load(si, i, 0) && load(si + 1, i, 1);
         }
         if (!ok) break;
         ask_for_unit(sched);
         unit_done(sched, k);
       }
+      if (DUO) si = 4 * round;
       if (lane == 0) {
         if (qi) mbar_drain(q_full, (qi - 1) & 1, p.err, 0x2111);
         for (uint32_t k = 0; k < uint32_t(ST) && k < si; ++k) {
@@ -228,7 +251,48 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
       for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, 0x2200); ++k) {
         const FwdUnit f = fwd_unit(prm, u);
         const uint16_t* list = lists + (k & 1) * kMaxList;
-        if (f.n > 0) {
+        if (DUO && f.n > 0) {
+          if (!wait_for(q_full, qi & 1, abort_flag, 0x2201)) break;
+          ++qi;
+          // scores of tile j (ring index r of its keys), or a stage passed on
+          auto scores = [&](uint32_t r, int j) {
+            if (!full(r, 0x2202)) return false;
+            if (j < f.n) {
+              tc_fence_after();
+              mma_kk<D>(one, tmem + (j & 1) * TILE, desc_k(qs), desc_k(stage(r)), id_s);
+              commit1(one, &s_full[j & 1]);
+            }
+            commit1(one, &kv_empty[r % ST]);
+            return true;
+          };
+          bool ok = scores(si, 0) && scores(si + 1, 1);
+          for (int i = 0; i < f.n && ok; i += 2, si += 4)
+            for (int t = 0; t < 2 && ok; ++t) {
+              const int j = i + t;
+              const uint32_t r = si + 2 + t;
+              if (!(ok = full(r, 0x2203))) break;
+              if (j < f.n) {
+                if (p.has_docs && (list[j] & kEntScrub)) {
+                  const int j0 = (f.t0 + int(list[j] & kEntTile)) * TILE;
+                  scrub_rows<D>(stage(r), p.kdoc + (size_t)f.b * p.skv + j0, p.skv - j0, lane);
+                }
+                const uint32_t t_s = tmem + t * TILE, t_o = tmem + 2 * TILE + t * D;
+                if (!(ok = wait_for(&p_ready[2 * t], cnt[t] & 1, abort_flag, 0x2205))) break;
+                tc_fence_after();
+                mma_tn<D, 0, 4>(one, t_o, t_s, t_s + 32, desc_mn(stage(r)), id_o, i > 0);
+                if (!(ok = wait_for(&p_ready[2 * t + 1], cnt[t] & 1, abort_flag, 0x2206))) break;
+                tc_fence_after();
+                mma_tn<D, 4, 8>(one, t_o, t_s, t_s + 32, desc_mn(stage(r)), id_o, true);
+                commit1(one, &o_done[t]);
+                ++cnt[t];
+              }
+              commit1(one, &kv_empty[r % ST]);
+              if (i + 2 < f.n) ok = scores(si + 4 + t, j + 2);
+            }
+          if (!ok) break;
+          commit1(one, q_empty);
+        }
+        if (!DUO && f.n > 0) {
           if (!wait_for(q_full, qi & 1, abort_flag, 0x2201) || !full(si, 0x2202)) break;
           ++qi;
           tc_fence_after();
@@ -322,7 +386,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     uint32_t cnt = 0;   // tiles so far
     for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, 0x2304); ++k) {
       const FwdUnit f = fwd_unit(prm, u);
-      if (t >= f.nt) {
+      if (!DUO && t >= f.nt) {
         unit_done(sched, k);
         continue;
       }
@@ -331,12 +395,12 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
       bool valid;
       if (prm.packed) {
         const int r = p.divG.div(row);
-        pos = (t ? f.pos[1] : f.pos[0]) + r;
+        pos = (t && !DUO ? f.pos[1] : f.pos[0]) + r;
         head = f.head[0] + row - r * p.G;
         valid = r < prm.pos_per_tile && pos < p.sq;
       } else {
-        pos = (t ? f.pos[1] : f.pos[0]) + row;
-        head = t ? f.head[1] : f.head[0];
+        pos = (t && !DUO ? f.pos[1] : f.pos[0]) + row;
+        head = t && !DUO ? f.head[1] : f.head[0];
         valid = pos < p.sq;
       }
       const int lim = valid ? row_limit(p, pos, f.pre) : 0;
@@ -347,9 +411,11 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
       float mref = -INFINITY;   // reference maximum, in units of 1 / c
       float l = 0.f;
       bool ok = true;
-      for (int i = 0; i < f.n; ++i) {
-        const uint32_t ent = p.has_docs ? list[i] : 0u;
-        const int j0 = (f.t0 + (p.has_docs ? int(ent & kEntTile) : i)) * TILE;
+      const int n = DUO ? (f.n + 1 - t) >> 1 : f.n;   // tiles of these warps
+      for (int i = 0; i < n; ++i) {
+        const int ti = DUO ? 2 * i + t : i;
+        const uint32_t ent = p.has_docs ? list[ti] : 0u;
+        const int j0 = (f.t0 + (p.has_docs ? int(ent & kEntTile) : ti)) * TILE;
         const bool masked = p.has_docs ? (ent & kEntMask) != 0 : j0 + TILE > f.lim0;
         ok = wait_for(&s_full[t], (cnt + i) & 1, abort_flag, 0x2301);
         if (!ok) break;
@@ -529,16 +595,16 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
         }
       }
       // ---- epilogue: o / l, and the row statistic
-      if (ok && f.n > 0) ok = wait_for(&o_done[t], (cnt + f.n - 1) & 1, abort_flag, 0x2303);
+      if (ok && n > 0) ok = wait_for(&o_done[t], (cnt + n - 1) & 1, abort_flag, 0x2303);
       if (!ok) break;
-      cnt += uint32_t(f.n);
+      cnt += uint32_t(n);
       if (any_valid) {
         tc_fence_after();
         const bool empty = l == 0.f;
         const float inv = empty ? 0.f : 1.f / l;
         const float lse = empty ? -INFINITY : (mref * c + log2f(l)) * kLn2;
         const size_t rowi = ((size_t)f.b * p.H + head) * p.sq + pos;
-        const size_t ri = (size_t)f.split * p.bs * p.H * p.sq + rowi;
+        const size_t ri = (size_t)(DUO ? 2 * f.split + t : f.split) * p.bs * p.H * p.sq + rowi;
         if (valid) (p.splits > 1 ? prm.part_lse + ri : prm.lse + rowi)[0] = lse;
         uint8_t* dst = static_cast<uint8_t*>(prm.o) + (((size_t)f.b * p.sq + pos) * p.H + head) * (D * 2);
         // (64 columns a load would hide more of TMEM's latency, but leaves the loop above fewer
@@ -547,7 +613,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
         for (int x = 0; x < D / 32; ++x) {
           uint32_t o[32];
           __syncwarp();
-          if (f.n > 0) {
+          if (n > 0) {
             tmem_ld32(t_o + x * 32, o);
             tmem_wait_ld();
           }
@@ -621,6 +687,37 @@ __global__ void __launch_bounds__(256) fwd_join_kernel(const FwdParams prm) {
   for (int e = 0; e < N / 2; ++e) dst[e] = pack2<F16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
   if (lane == 0) prm.lse[r] = mx == -INFINITY ? -INFINITY : mx + logf(l);
 }
+
+// fused_fwd.cu, fused_token.cu (units of one tile)
+int launch_fwd(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int d, bool f16,
+               bool cap, cudaStream_t s);
+int launch_token(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int d, bool f16,
+                 bool cap, cudaStream_t s);
+
+#define ATTN_BWD_FWD_LAUNCHER(NAME, DUO)                                                                               \
+  template <int D, bool F16, bool CAP, bool BIAS>                                                                      \
+  static int NAME##_one(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,          \
+                        cudaStream_t stream) {                                                                         \
+    using C = FwdCfg<D, DUO>;                                                                                               \
+    const auto kern = fwd_kernel<D, F16, CAP, BIAS, DUO>;                                                              \
+    const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);                                 \
+    if (rc) return rc;                                                                                                 \
+    kern<<<dim3(unsigned(f.blocks_q) * f.head_slots, f.c.bs, f.cta_splits), kThreads, C::SMEM_BYTES, stream>>>(q, k, v, f); \
+    return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;                                        \
+  }                                                                                                                    \
+  int NAME(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int d, bool f16,      \
+           bool cap, cudaStream_t s) {                                                                                 \
+    const bool bias = f.c.slopes != nullptr;                                                                           \
+    if (d == 128)                                                                                                      \
+      return f16 ? (cap ? (bias ? NAME##_one<128, true, true, true>(f, q, k, v, s) : NAME##_one<128, true, true, false>(f, q, k, v, s))     \
+                        : (bias ? NAME##_one<128, true, false, true>(f, q, k, v, s) : NAME##_one<128, true, false, false>(f, q, k, v, s)))  \
+                 : (cap ? (bias ? NAME##_one<128, false, true, true>(f, q, k, v, s) : NAME##_one<128, false, true, false>(f, q, k, v, s))   \
+                        : (bias ? NAME##_one<128, false, false, true>(f, q, k, v, s) : NAME##_one<128, false, false, false>(f, q, k, v, s))); \
+    return f16 ? (cap ? (bias ? NAME##_one<64, true, true, true>(f, q, k, v, s) : NAME##_one<64, true, true, false>(f, q, k, v, s))         \
+                      : (bias ? NAME##_one<64, true, false, true>(f, q, k, v, s) : NAME##_one<64, true, false, false>(f, q, k, v, s)))      \
+               : (cap ? (bias ? NAME##_one<64, false, true, true>(f, q, k, v, s) : NAME##_one<64, false, true, false>(f, q, k, v, s))       \
+                      : (bias ? NAME##_one<64, false, false, true>(f, q, k, v, s) : NAME##_one<64, false, false, false>(f, q, k, v, s)));   \
+  }
 
 }  // namespace fused
 }  // namespace attn_bwd
