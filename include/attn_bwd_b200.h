@@ -165,11 +165,13 @@ int attn_bwd_b200_rope(const attn_bwd_rope_t* args, const void* q, const void* k
  * j is seen if  (!causal || j < max(i + 1, prefix_lens[b]))  and, with documents,
  * q_documents[b, row] == kv_documents[b, j] >= 0.  A row that sees nothing has output 0, row
  * statistic -inf and gradient 0.  Keys and queries whose document is negative are never read
- * into a result, whatever they hold.  slopes, prefix_lens and documents may be null;
+ * into a result, whatever they hold; a NaN or infinity in another key or value may also reach
+ * queries of the same tiles that do not see it.  slopes, prefix_lens and documents may be null;
  * prefix_lens needs causal; both document arrays or neither.
  *   q [bs, heads, seq_q, head_dim], k and v [bs, kv_heads, seq_kv, head_dim]: strides in
  *     elements in the order batch, head, position (positive multiples of 8, head elements
- *     contiguous, 16-byte aligned), heads a multiple of kv_heads, head_dim 64 or 128
+ *     contiguous, 16-byte aligned), heads a multiple of kv_heads, head_dim 64 or 128; bs and
+ *     heads at most 65535; the backward call with documents: at most 262144 positions
  *   o [bs, seq_q, heads, head_dim] contiguous; lse [bs, heads, seq_q] fp32 (natural log)
  *   dq, dk, dv: shaped as q, k, v, strides in dq_stride / dk_stride / dv_stride
  * workspace: at least attn_bwd_b200_fused_workspace() bytes, 256-byte aligned, private to the call until
@@ -178,8 +180,8 @@ typedef struct {
   int bs, seq_q, seq_kv, heads, kv_heads, head_dim;
   int dtype; /* ATTN_BWD_DT_BF16 or ATTN_BWD_DT_FP16 */
   int causal;
-  float scale;   /* > 0 */
-  float softcap; /* 0: none */
+  float scale;   /* > 0, below 1e38 */
+  float softcap; /* 0: none; else above 1e-30, below 1e38, scale / softcap below 1e30 */
   const float* slopes;         /* [heads] */
   const int32_t* prefix_lens;  /* [bs] */
   const int32_t* q_documents;  /* [bs, seq_q] */

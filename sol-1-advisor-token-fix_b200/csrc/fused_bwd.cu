@@ -67,6 +67,7 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
   if (a->seq_kv && (!k || !v || !dk || !dv)) return ATTN_BWD_EINVAL;
   if (!al16(go) || !al16(q) || !al16(k) || !al16(v) || !al16(o) || !al16(dq) || !al16(dk) || !al16(dv))
     return ATTN_BWD_EALIGN;
+  if (tiles_of(a->seq_q) > (1 << 30) / a->heads || tiles_of(a->seq_kv) > (1 << 30) / a->kv_heads) return ATTN_BWD_EINVAL;
   // with documents a unit lists its tiles
   if (a->q_documents && (tiles_of(a->seq_q) > kMaxList || tiles_of(a->seq_kv) > kMaxList)) return ATTN_BWD_EUNSUPPORTED;
   HostDevice dev;

@@ -25,7 +25,7 @@ struct Params {
   int causal, has_docs;
   float scale;             // of the scores
   float scale_log2;        // scale * log2(e)
-  float cap_u;             // softcap: scale / softcap
+  float cap_u;             // softcap: scale / softcap (infinite where TanhSmall's coefficients are)
   float cap_in;            // 2 * log2(e) * scale / softcap
   float cap_out;           // softcap * log2(e)
   float cap_inv;           // 1 / cap_out
@@ -337,6 +337,13 @@ __device__ __forceinline__ bool cap_small(const Params& p, const uint32_t (&x)[3
 #pragma unroll
   for (int e = 0; e < 32; e += 2) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1]))));
   return __all_sync(0xffffffffu, big * p.cap_u <= kTanhSmall);
+}
+// One raw score to softcap tanh(scale x / softcap) log2(e).  (Through the reciprocal alone a high
+// cap would leave nothing of a low score.)
+__device__ __forceinline__ float cap1(const Params& p, const TanhSmall& ts, float x) {
+  float lo, hi;
+  f2_split(f2_mul(ts.factor(f2(x, x)), f2(x, x)), lo, hi);
+  return fabsf(x) * p.cap_u <= kTanhSmall ? lo : fmaf(-2.f * p.cap_out, rcp(1.f + ex2(x * p.cap_in)), p.cap_out);
 }
 // 32 raw scores to softcap tanh(scale x / softcap) log2(e) + add, in place.
 __device__ __forceinline__ void cap32(const Params& p, const TanhSmall& ts, uint32_t (&x)[32], float add = 0.f) {

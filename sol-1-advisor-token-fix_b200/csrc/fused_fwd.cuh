@@ -381,7 +381,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     const int row = int(warp & 3) * 32 + int(lane);
     // scores that are only scaled stay raw and are scaled inside the exponent
     const float c = BIAS || CAP ? 1.f : p.scale_log2;
-    const float grow = 8.f / c;
+    const float grow = fminf(8.f / c, 3e38f);
     const TanhSmall tanh_small(p);
     uint32_t cnt = 0;   // tiles so far
     for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, 0x2304); ++k) {
@@ -485,7 +485,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
               for (int g = 0; g < 4; ++g) hide(x[g], g);
             }
             m = fmaxf(fmaxf(highest(x[0]), highest(x[1])), fmaxf(highest(x[2]), highest(x[3])));
-            if (CAP) m = fmaf(-2.f * p.cap_out, rcp(1.f + ex2(m * p.cap_in)), p.cap_out);   // the tanh grows with its argument
+            if (CAP) m = cap1(p, tanh_small, m);   // the tanh grows with its argument
           } else if constexpr (CAP || BIAS) {
             m = -INFINITY;
 #pragma unroll 1

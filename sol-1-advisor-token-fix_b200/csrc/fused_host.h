@@ -1,5 +1,6 @@
 // fused_host.h — argument checks and parameters that the fused attention entry points share.
 #pragma once
+#include <cmath>
 #include <cstring>
 
 #include "../../include/attn_bwd_b200.h"
@@ -24,7 +25,9 @@ inline int check_args(const attn_bwd_fused_t* a) {
   if (!a || a->bs < 0 || a->seq_q < 0 || a->seq_kv < 0 || a->heads < 1 || a->kv_heads < 1 ||
       a->heads % a->kv_heads || a->bs > 65535 || a->heads > 65535 || a->seq_q >= (1 << 30) || a->seq_kv >= (1 << 30))
     return ATTN_BWD_EINVAL;
-  if (!(a->scale > 0.f) || !(a->scale < 3e38f) || !(a->softcap >= 0.f) || !(a->softcap < 3e38f)) return ATTN_BWD_EINVAL;
+  // scale and softcap in log2 units, and their ratio, have to be finite fp32 numbers
+  if (!(a->scale > 0.f) || !(a->scale < 1e38f) || !(a->softcap >= 0.f) || !(a->softcap < 1e38f)) return ATTN_BWD_EINVAL;
+  if (a->softcap > 0.f && !(a->softcap > 1e-30f && double(a->scale) / a->softcap < 1e30)) return ATTN_BWD_EINVAL;
   if (a->prefix_lens && !a->causal) return ATTN_BWD_EINVAL;
   if ((a->q_documents == nullptr) != (a->kv_documents == nullptr)) return ATTN_BWD_EINVAL;
   if (a->head_dim != 64 && a->head_dim != 128) return ATTN_BWD_EUNSUPPORTED;
@@ -62,6 +65,7 @@ inline Params base_params(const attn_bwd_fused_t* a) {
     for (int i = 0; i < 5; ++i) {
       f *= u * u;
       p.cap_poly[i + 1] = float(kTanhPoly[i] * f);
+      if (!(fabs(p.cap_poly[i + 1]) < 3e38f)) p.cap_u = INFINITY;
     }
   }
   p.slopes = a->slopes;

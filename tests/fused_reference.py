@@ -42,6 +42,10 @@ def attention(q, k, v, do=None, scale=None, softcap=0.0, slopes=None, causal=Fal
     half = HALF_STEP[q.dtype] if half is None else half
     if q.dtype == torch.float16:
         subnormal = 2.0 ** -25
+    elif q.dtype == torch.bfloat16:
+        # the exponent range of fp32: an exponential, a product or a result below its smallest normal
+        # number 2^-126 may be taken as 0, so each is off by at most that much
+        subnormal = 2.0 ** -126
     b, h, sq, d = q.shape
     kv, skv = k.shape[1], k.shape[2]
     grp = h // kv

@@ -64,7 +64,8 @@ def _args(**kw):
     (dict(bs=-1), _lib.EINVAL), (dict(seq_q=-1), _lib.EINVAL), (dict(seq_kv=-4), _lib.EINVAL), (dict(heads=0), _lib.EINVAL),
     (dict(kv_heads=3), _lib.EINVAL), (dict(scale=0.0), _lib.EINVAL), (dict(scale=-1.0), _lib.EINVAL),
     (dict(scale=math.nan), _lib.EINVAL), (dict(scale=math.inf), _lib.EINVAL), (dict(softcap=-1.0), _lib.EINVAL),
-    (dict(softcap=math.nan), _lib.EINVAL), (dict(head_dim=96), _lib.EUNSUPPORTED), (dict(dtype=2), _lib.EUNSUPPORTED),
+    (dict(softcap=math.nan), _lib.EINVAL), (dict(softcap=1e-35), _lib.EINVAL), (dict(scale=3e38), _lib.EINVAL),
+    (dict(scale=1e10, softcap=1e-25), _lib.EINVAL), (dict(head_dim=96), _lib.EUNSUPPORTED), (dict(dtype=2), _lib.EUNSUPPORTED),
     (dict(prefix_lens=16), _lib.EINVAL), (dict(q_documents=16), _lib.EINVAL), (dict(kv_documents=16), _lib.EINVAL),
     (dict(bs=70000), _lib.EINVAL), (dict(seq_q=1 << 30), _lib.EINVAL)])
 def test_c_entry_refuses_without_device(bad, code):
@@ -199,6 +200,37 @@ def test_modified_scores(cuda, mod, bs, sq, skv, dtype, d):
         qd = torch.cat([torch.full((bs, max(0, sq - skv)), -1, dtype=torch.int32), kd], 1)[:, -sq:]
         kw["documents"] = (qd.contiguous().cuda(), kd.cuda())
     _check(q, k, v, do, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("std,kw", [
+    (1.0, dict(softcap=1e-4)), (1.0, dict(softcap=1e8)), (1.0, dict(softcap=1e30)), (8.0, dict(softcap=2.0)),
+    (1.0, dict(scale=1e-30)), (1.0, dict(scale=4.0)), (0.0, dict(softcap=1e-20)), (20.0, dict(softcap=50.0))])
+def test_extreme_caps_and_scales(cuda, std, kw):
+    """Caps far above and below the scores, scores at the cap, scales that leave nothing of them."""
+    q, k, v, do = _inputs(1, 4, 2, 150, 260, 64, BF, std=std)
+    _check(q, k, v, do, causal=True, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 2, 3, 5])
+def test_tokens_over_few_and_odd_tiles(cuda, n):
+    """One tile of rows: two chains over alternate key tiles, the last of them odd; with documents too."""
+    skv = n * 128 - 7
+    q, k, v, do = _inputs(3, 8, 2, 4, skv, 64, HF)
+    _check(q, k, v, do, causal=True)
+    kd = _docs(3, skv, 90, pad=3)
+    _check(q, k, v, do, causal=True, documents=(kd[:, -4:].contiguous().cuda(), kd.cuda()), softcap=3.0)
+
+
+@pytest.mark.gpu
+def test_many_short_units(cuda):
+    """More units than SMs, most of them of one tile, some of none: each CTA takes up several."""
+    q, k, v, do = _inputs(24, 12, 4, 130, 70, 64, BF)
+    _check(q, k, v, do, causal=True)
+    kd = _docs(24, 130, 20, pad=30)
+    q, k, v, do = _inputs(24, 12, 4, 130, 130, 64, BF)
+    _check(q, k, v, do, causal=True, documents=kd.cuda())
 
 
 @pytest.mark.gpu
