@@ -128,11 +128,13 @@ __device__ __forceinline__ void bwd_end(const BwdShared& s, uint32_t tmem, int* 
   }
 }
 
-// Weights of four scores (CAP: capped, in log2 units).  x: in, p out; m: what ds is multiplied by (p,
-// or p tanh').  add: bias - lse in log2 units.
-template <bool CAP>
-__device__ __forceinline__ void weights4(const Params& p, float (&x)[4], const float (&add)[4], float (&m)[4]) {
+// Weights of four raw scores.  x: in, p out; m: what ds is multiplied by (p, or p tanh').  add: bias
+// - lse in log2 units.  SMALL: see TanhSmall.
+template <bool CAP, bool SMALL>
+__device__ __forceinline__ void weights4(const Params& p, const TanhSmall& ts, float (&x)[4], const float (&add)[4],
+                                         float (&m)[4]) {
   if (CAP) {
+    cap4<SMALL>(p, ts, x, 0.f);
     const uint64_t inv = f2(p.cap_inv, p.cap_inv), neg = f2(-1.f, -1.f), one = f2(1.f, 1.f);
 #pragma unroll
     for (int y = 0; y < 4; y += 2) {

@@ -332,10 +332,13 @@ struct TanhSmall {
     return f2_fma(y, x2, c[0]);
   }
 };
-__device__ __forceinline__ bool cap_small(const Params& p, const uint32_t (&x)[32]) {
+__device__ __forceinline__ float highest_abs(const uint32_t (&x)[32]) {
   float big = 0.f;
 #pragma unroll
   for (int e = 0; e < 32; e += 2) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1]))));
+  return big;
+}
+__device__ __forceinline__ bool cap_small(const Params& p, float big) {
   return __all_sync(0xffffffffu, big * p.cap_u <= kTanhSmall);
 }
 // One raw score to softcap tanh(scale x / softcap) log2(e).  (Through the reciprocal alone a high
@@ -345,29 +348,33 @@ __device__ __forceinline__ float cap1(const Params& p, const TanhSmall& ts, floa
   f2_split(f2_mul(ts.factor(f2(x, x)), f2(x, x)), lo, hi);
   return fabsf(x) * p.cap_u <= kTanhSmall ? lo : fmaf(-2.f * p.cap_out, rcp(1.f + ex2(x * p.cap_in)), p.cap_out);
 }
-// 32 raw scores to softcap tanh(scale x / softcap) log2(e) + add, in place.
-__device__ __forceinline__ void cap32(const Params& p, const TanhSmall& ts, uint32_t (&x)[32], float add = 0.f) {
-  if (cap_small(p, x)) {
-    const uint64_t a2 = f2(add, add);
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      const uint64_t v = f2(x[e], x[e + 1]);
-      float a, b;
-      f2_split(f2_fma(ts.factor(v), v, a2), a, b);
-      x[e] = __float_as_uint(a);
-      x[e + 1] = __float_as_uint(b);
-    }
+// Four raw scores to softcap tanh(scale x / softcap) log2(e) + add.  SMALL: all below kTanhSmall.
+template <bool SMALL>
+__device__ __forceinline__ void cap4(const Params& p, const TanhSmall& ts, float (&x)[4], float add) {
+  if (SMALL) {
+    const uint64_t a2 = f2(add, add), v = f2(x[0], x[1]), w = f2(x[2], x[3]);
+    f2_split(f2_fma(ts.factor(v), v, a2), x[0], x[1]);
+    f2_split(f2_fma(ts.factor(w), w, a2), x[2], x[3]);
   } else {
     const float top = p.cap_out + add;
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {
-      float z[4];
+    for (int i = 0; i < 4; ++i) x[i] *= p.cap_in;
+    cap_r4(x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) z[i] = __uint_as_float(x[e + i]) * p.cap_in;
-      cap_r4(z);
+    for (int i = 0; i < 4; ++i) x[i] = fmaf(-2.f * p.cap_out, x[i], top);
+  }
+}
+// 32 of them, in place.
+template <bool SMALL>
+__device__ __forceinline__ void cap32(const Params& p, const TanhSmall& ts, uint32_t (&x)[32]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[e + i] = __float_as_uint(fmaf(-2.f * p.cap_out, z[i], top));
-    }
+  for (int e = 0; e < 32; e += 4) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __uint_as_float(x[e + i]);
+    cap4<SMALL>(p, ts, y, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[e + i] = __float_as_uint(y[i]);
   }
 }
 

@@ -260,12 +260,11 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
 #pragma unroll
         for (int y = 0; y < 2; ++y) tmem_ld32(st + y * 32, w[y]);
         tmem_wait_ld();
-        auto phase = [&](auto mask_tag) {
-          constexpr bool MASK = decltype(mask_tag)::value;
+        auto phase = [&](auto mask_tag, auto small_tag) {
+          constexpr bool MASK = decltype(mask_tag)::value, SMALL = decltype(small_tag)::value;
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             uint32_t pk[16];
-            if (CAP) cap32(p, tanh_small, w[y]);
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
               const float4 nl = nl4[y * 8 + e / 4];
@@ -275,7 +274,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
                 x[z] = __uint_as_float(w[y][e + z]);
                 if (BIAS) add[z] = fmaf(-slope2, fabsf(dist0 + float(y * 32 + e + z)), add[z]);
               }
-              weights4<CAP>(p, x, add, m);
+              weights4<CAP, SMALL>(p, tanh_small, x, add, m);
 #pragma unroll
               for (int z = 0; z < 4; ++z) {
                 if (MASK && !((see[y] >> (e + z)) & 1u)) x[z] = m[z] = 0.f;
@@ -291,8 +290,14 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
             if (lane == 0) mbar_arrive(&sh.p_ready[y]);
           }
         };
-        if (__builtin_expect(masked, 0)) phase(std::true_type{});
-        else phase(std::false_type{});
+        const bool small = CAP && cap_small(p, fmaxf(highest_abs(w[0]), highest_abs(w[1])));
+        if (__builtin_expect(masked, 0)) {
+          if (CAP && small) phase(std::true_type{}, std::true_type{});
+          else phase(std::true_type{}, std::false_type{});
+        } else {
+          if (CAP && small) phase(std::false_type{}, std::true_type{});
+          else phase(std::false_type{}, std::false_type{});
+        }
 
         float4 nd4[16];
 #pragma unroll

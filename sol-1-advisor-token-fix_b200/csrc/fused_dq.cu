@@ -247,22 +247,25 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         for (int y = 0; y < 2; ++y) tmem_ld32(st + y * 32, w[y]);
         tmem_wait_ld();
         const float dist0 = float(row + p.off - j0);
+        auto phase = [&](auto small_tag) {
+          constexpr bool SMALL = decltype(small_tag)::value;
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          if (CAP) cap32(p, tanh_small, w[y]);
+          for (int y = 0; y < 2; ++y)
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
+            for (int e = 0; e < 32; e += 4) {
               float add[4], x[4], m[4];
 #pragma unroll
               for (int z = 0; z < 4; ++z) {
                 x[z] = __uint_as_float(w[y][e + z]);
                 add[z] = BIAS ? fmaf(-slope2, fabsf(dist0 - float(y * 32 + e + z)), nlse) : nlse;
               }
-              weights4<CAP>(p, x, add, m);
+              weights4<CAP, SMALL>(p, tanh_small, x, add, m);
 #pragma unroll
               for (int z = 0; z < 4; ++z) w[y][e + z] = __float_as_uint(m[z]);
-          }
-        }
+            }
+        };
+        if (CAP && cap_small(p, fmaxf(highest_abs(w[0]), highest_abs(w[1])))) phase(std::true_type{});
+        else phase(std::false_type{});
         if (i == 0) {
           // delta of the row: each half of the warps takes half of the columns
           ok = wait_for(sh.res_full, di & 1, sh.abort_flag, 0x4305);

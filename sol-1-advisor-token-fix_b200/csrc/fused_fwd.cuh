@@ -442,7 +442,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           };
           // 32 scores from column 32 g on: cap, bias, mask (log2 units / c, -inf where not seen)
           auto modify = [&](uint32_t (&x)[32], int g) {
-            if (CAP) cap32(p, tanh_small, x);
+            if (CAP) {
+              if (cap_small(p, highest_abs(x))) cap32<true>(p, tanh_small, x);
+              else cap32<false>(p, tanh_small, x);
+            }
             if (BIAS) {
               const float d0 = float(pos + p.off - j0 - g * 32), sl = CAP ? 1.f : p.scale_log2;
 #pragma unroll
@@ -467,6 +470,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           const bool late_cap = CAP && !BIAS && !masked;
           uint32_t x[4][32];
           float m;
+          bool small = false;
           if (in_regs || late_cap) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) tmem_ld32(t_s + g * 32, x[g]);
@@ -485,6 +489,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
               for (int g = 0; g < 4; ++g) hide(x[g], g);
             }
             m = fmaxf(fmaxf(highest(x[0]), highest(x[1])), fmaxf(highest(x[2]), highest(x[3])));
+            if (CAP)
+              small = cap_small(p, fmaxf(fmaxf(highest_abs(x[0]), highest_abs(x[1])),
+                                         fmaxf(highest_abs(x[2]), highest_abs(x[3]))));
             if (CAP) m = cap1(p, tanh_small, m);   // the tanh grows with its argument
           } else if constexpr (CAP || BIAS) {
             m = -INFINITY;
@@ -526,20 +533,27 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           const float nm = mref == -INFINITY ? 0.f : -mref * c;
           const uint64_t c2 = f2(c, c), nm2 = f2(nm, nm);
           uint64_t sum0 = 0, sum1 = 0;
-          // weights of 32 keys, to 16 columns
-          auto weigh = [&](const uint32_t (&y)[32], uint32_t column, auto done_tag) {
-            constexpr bool DONE = decltype(done_tag)::value;   // the exponents themselves
+          // weights of 32 keys, to 16 columns.  TR 0: of scores; 1, 2: of raw scores to be capped
+          auto weigh = [&](const uint32_t (&y)[32], uint32_t column, auto tr_tag) {
+            constexpr int TR = decltype(tr_tag)::value;
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              float a0, a1, b0, b1;
-              f2_split(DONE ? f2(y[e], y[e + 1]) : f2_fma(f2(y[e], y[e + 1]), c2, nm2), a0, a1);
-              f2_split(DONE ? f2(y[e + 2], y[e + 3]) : f2_fma(f2(y[e + 2], y[e + 3]), c2, nm2), b0, b1);
-              a0 = ex2(a0); a1 = ex2(a1); b0 = ex2(b0); b1 = ex2(b1);
-              sum0 = f2_add(sum0, f2(a0, a1));
-              sum1 = f2_add(sum1, f2(b0, b1));
-              w[e / 2] = pack2<F16>(a0, a1);
-              w[e / 2 + 1] = pack2<F16>(b0, b1);
+              float a[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) a[z] = __uint_as_float(y[e + z]);
+              if (TR) {
+                cap4<TR == 1>(p, tanh_small, a, nm);
+              } else {
+                f2_split(f2_fma(f2(a[0], a[1]), c2, nm2), a[0], a[1]);
+                f2_split(f2_fma(f2(a[2], a[3]), c2, nm2), a[2], a[3]);
+              }
+#pragma unroll
+              for (int z = 0; z < 4; ++z) a[z] = ex2(a[z]);
+              sum0 = f2_add(sum0, f2(a[0], a[1]));
+              sum1 = f2_add(sum1, f2(a[2], a[3]));
+              w[e / 2] = pack2<F16>(a[0], a[1]);
+              w[e / 2 + 1] = pack2<F16>(a[2], a[3]);
             }
             tmem_st16(t_s + column, w);
           };
@@ -557,27 +571,27 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           if (in_regs) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              weigh(x[g], g * 16, std::false_type{});
+              weigh(x[g], g * 16, std::integral_constant<int, 0>{});
               if (g & 1) hand_over(g >> 1);
             }
           } else if constexpr (CAP || BIAS) {
+            auto again = [&](auto tr_tag) {
 #pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
+              for (int h = 0; h < 2; ++h) {
 #pragma unroll 1
-              for (int g = 2 * h; g < 2 * h + 2; ++g) {
-                uint32_t y[32];
-                __syncwarp();
-                tmem_ld32(t_s + g * 32, y);
-                tmem_wait_ld();
-                if (CAP && late_cap) {
-                  cap32(p, tanh_small, y, nm);
-                  weigh(y, g * 16, std::true_type{});
-                } else {
-                  weigh(y, g * 16, std::false_type{});
+                for (int g = 2 * h; g < 2 * h + 2; ++g) {
+                  uint32_t y[32];
+                  __syncwarp();
+                  tmem_ld32(t_s + g * 32, y);
+                  tmem_wait_ld();
+                  weigh(y, g * 16, tr_tag);
                 }
+                hand_over(h);
               }
-              hand_over(h);
-            }
+            };
+            if (CAP && late_cap && small) again(std::integral_constant<int, 1>{});
+            else if (CAP && late_cap) again(std::integral_constant<int, 2>{});
+            else again(std::integral_constant<int, 0>{});
           }
           if (!ok) break;
           float x0, x1, y0, y1;
