@@ -192,7 +192,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
   } else {
     // ---------------------------------------------------------------- weights: one query a thread, 64 keys
     regs_grow();
-    constexpr int NC = D / 16;   // 16-byte words of half a row
+    constexpr int LR = D / 16;   // 16-byte words of half a row
     const TanhSmall tanh_small(p);
     const int half = int(warp) >> 2;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
@@ -206,12 +206,18 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
       const bool valid = row < p.sq;
       const size_t ri = ((size_t)f.b * p.H + f.h) * prm.sq_pad + row;   // padded to whole tiles
       const float lse = valid ? __ldg(prm.lse + ((size_t)f.b * p.H + f.h) * p.sq + row) : -INFINITY;
-      const bool none = lse == -INFINITY;   // the row sees nothing
-      const float nlse = none ? -INFINITY : -lse * kLog2e;
-      uint4 ov[NC];   // this half of the row of o, for delta
-      const uint8_t* orow = prm.o + (((size_t)f.b * p.sq + (valid ? row : f.r0)) * p.H + f.h) * (D * 2) + half * D;
+      // o of these rows, this half of the columns, for delta: the lanes of a group of LR read one row's
+      // part together (a lane reading its own row's would touch 32 lines a load).  Used, like
+      // lse, only after the wait for the first scores.
+      uint4 ov[LR];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) ov[c] = __ldg(reinterpret_cast<const uint4*>(orow) + c);
+      for (int c = 0; c < LR; ++c) {
+        const int r = min(f.r1, f.r0 + int(warp & 3) * 32 + c * (32 / LR) + int(lane) / LR);
+        ov[c] = __ldg(reinterpret_cast<const uint4*>(prm.o + (((size_t)f.b * p.sq + r) * p.H + f.h) * (D * 2) + half * D) +
+                      int(lane) % LR);
+      }
+      bool none = false;       // the row sees nothing
+      float nlse = 0.f;
       uint64_t nd2 = 0;
       const int lim = valid ? row_limit(p, row, f.pre) : 0;
       const int qd = (valid && p.has_docs) ? __ldg(p.qdoc + (size_t)f.b * p.sq + row) : -1;
@@ -242,6 +248,10 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         ok = wait_for(&sh.s_full[it & 1], (it >> 1) & 1, sh.abort_flag, 0x4301);
         if (!ok) break;
         tc_fence_after();
+        if (i == 0) {
+          none = lse == -INFINITY;
+          nlse = none ? -INFINITY : -lse * kLog2e;
+        }
         uint32_t w[2][32];
 #pragma unroll
         for (int y = 0; y < 2; ++y) tmem_ld32(st + y * 32, w[y]);
@@ -271,26 +281,28 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
           ok = wait_for(sh.res_full, di & 1, sh.abort_flag, 0x4305);
           if (!ok) break;
           const int r = int(warp & 3) * 32 + int(lane);
-          float d = 0.f;
+          float* part = reinterpret_cast<float*>(sh.smem + C::OFF_STAT) + (k & 1) * (2 * TILE);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const int cg = half * NC + c;
-            const uint4 g = lds128(smem_u32(sh.smem + C::OFF_A + C::TILE_BYTES) + (cg >> 3) * (TILE * 128) + r * 128 +
-                                   (((cg & 7) ^ (r & 7)) << 4));
+          for (int c = 0; c < LR; ++c) {
+            const int rr = int(warp & 3) * 32 + c * (32 / LR) + int(lane) / LR, cg = half * LR + int(lane) % LR;
+            const uint4 g = lds128(smem_u32(sh.smem + C::OFF_A + C::TILE_BYTES) + (cg >> 3) * (TILE * 128) + rr * 128 +
+                                   (((cg & 7) ^ (rr & 7)) << 4));
             const uint32_t gs[4] = {g.x, g.y, g.z, g.w}, os[4] = {ov[c].x, ov[c].y, ov[c].z, ov[c].w};
+            float d = 0.f;
 #pragma unroll
             for (int z = 0; z < 4; ++z) {
               const float2 u = unpack2<F16>(gs[z]), v = unpack2<F16>(os[z]);
               d = fmaf(u.x, v.x, d);
               d = fmaf(u.y, v.y, d);
             }
+#pragma unroll
+            for (int m = LR / 2; m; m >>= 1) d += __shfl_xor_sync(0xffffffffu, d, m);
+            if (int(lane) % LR == 0) part[half * TILE + rr] = d;
           }
-          float* part = reinterpret_cast<float*>(sh.smem + C::OFF_STAT) + (k & 1) * (2 * TILE);
-          part[half * TILE + r] = d;
           __syncwarp();
           if (lane == 0) mbar_arrive(sh.res_empty);
           named_bar_sync(1 + (warp & 3), 64);   // the two warps of these rows
-          d += part[(half ^ 1) * TILE + r];     // a sum of two: the same in either order
+          const float d = part[r] + part[TILE + r];
           const float nd = none ? 0.f : -d;
           nd2 = f2(nd, nd);
           if (half == 0) {
