@@ -423,3 +423,68 @@ def test_workspace_is_checked(cuda):
     assert call(0, 0) == _lib.EINVAL and call(ws.data_ptr(), need - 1) == _lib.EINVAL
     assert call(ws.data_ptr() + 16, need) == _lib.EALIGN
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(cuda):
+    """Calls that overlap on two streams, each with its own workspace, give the bits they give alone."""
+    sets = [_inputs(2, 10, 2, 300, 900, 128, BF, seed=s) for s in (1, 2)]
+    mods = dict(causal=True, softcap=15.0)
+
+    def step(q, k, v, do):
+        o, lse = ab.fused_attn_fwd(q, k, v, **mods)
+        t, tl = ab.fused_attn_fwd(q[:, :, -1:], k, v, **mods)
+        return (o, lse, t, tl) + ab.fused_attn_bwd(do, q, k, v, o, lse, **mods)
+
+    alone = [step(*x) for x in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    for a, runs in zip(alone, got):
+        assert all(torch.equal(x, y) for r in runs for x, y in zip(a, r))
+    assert ab.poll_error() == 0
+
+
+@pytest.mark.gpu
+def test_long_cache(cuda):
+    """17 million keys: element offsets above 2^31.  A few planted keys, the last one among them, take
+    nearly all of the weight; the rest is noise of known size."""
+    n, d = 17_000_003, 128
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k = torch.empty(1, 1, n, d, dtype=BF, device="cuda").normal_(generator=g).mul_(0.01)
+    v = torch.empty(1, 1, n, d, dtype=BF, device="cuda").normal_(generator=g)
+    q = torch.randn(1, 4, 1, d, generator=g, device="cuda").to(BF)
+    at = [5, 8_388_607, 16_777_216, 16_900_000, n - 1]
+    for a, h in zip(at, (0, 1, 2, 3, 0)):
+        k[0, 0, a] = q[0, h, 0] * 3        # score about 3 * 128 / sqrt(128) = 34 for its head
+    o, lse = ab.fused_attn_fwd(q, k, v, causal=True)
+    ref, rl = torch.zeros(4, d, dtype=torch.float64, device="cuda"), torch.full((4, 1), -math.inf, device="cuda").double()
+    for c in range(0, n, 1 << 21):
+        s = q[0, :, 0].double() @ k[0, 0, c:c + (1 << 21)].double().t() / math.sqrt(d)
+        part = torch.logsumexp(s, 1, keepdim=True)
+        new = torch.logaddexp(rl, part)
+        ref = ref * torch.exp(rl - new) + torch.exp(s - new) @ v[0, 0, c:c + (1 << 21)].double()
+        rl = new
+    # weights rounded to bf16 and the result once: 2 half steps of values up to 5, and fp32 sums
+    assert (o[0, 0].double() - ref).abs().max() < 2 * 2 ** -8 * 5
+    assert ref.abs().max() > 0.5           # the planted keys, not the mean of the noise
+    assert (lse[0].double() - rl).abs().max() < 1e-4
+
+
+@pytest.mark.gpu
+def test_cache_slices_far_from_its_start(cuda):
+    """Keys and values that lie above 2^32 bytes in their buffer, gradients in their own."""
+    big = torch.zeros(2, 2, 4_400_000, 128, dtype=BF, device="cuda")    # 4.5 GB a buffer
+    q, k, v, do = _inputs(2, 4, 2, 90, 200, 128, BF)
+    far = big[:, :, -200:]
+    far.copy_(k)
+    o, lse = ab.fused_attn_fwd(q, far, v, causal=True)
+    e, el = ab.fused_attn_fwd(q, k, v, causal=True)
+    assert torch.equal(o, e) and torch.equal(lse, el)
+    for a, b in zip(ab.fused_attn_bwd(do, q, far, v, o, lse, causal=True), ab.fused_attn_bwd(do, q, k, v, e, el, causal=True)):
+        assert torch.equal(a, b)

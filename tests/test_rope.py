@@ -127,6 +127,17 @@ def test_far_positions_and_position_forms(cuda):
 
 
 @pytest.mark.gpu
+def test_offsets_above_32_bits(cuda):
+    """17 million positions of one head: the last rows are what a short call gives for them."""
+    n = 17_000_003
+    k = torch.empty(1, 1, n, 128, dtype=BF, device="cuda").normal_()
+    table, pos = ab.rope_table(128), torch.arange(n, device="cuda")
+    _, got = ab.rope_fwd(None, k, pos, table)
+    for part in (slice(0, 70), slice(8_388_600, 8_388_700), slice(n - 50, n)):
+        assert torch.equal(got[:, :, part], ab.rope_fwd(None, k[:, :, part], pos[part], table)[1])
+
+
+@pytest.mark.gpu
 def test_scaled_table_and_gradient_against_differences(cuda):
     scaling = {"type": "ramp", "factor": 8.0, "original_length": 64, "low": 1.0, "high": 8.0}
     table = ab.rope_table(64, scaling=scaling)
