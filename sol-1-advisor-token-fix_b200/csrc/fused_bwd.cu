@@ -93,7 +93,6 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
   f.part = ws + l.stat / 2;
   f.c.qrange = reinterpret_cast<const DocRange*>(reinterpret_cast<const uint8_t*>(f.part) + l.part);
   f.c.krange = f.c.qrange + (int64_t)a->bs * f.c.n_tiles;
-  f.dq = dq;
   f.dk = dk;
   f.dv = dv;
   // an extent of 1 has no stride that counts
@@ -102,7 +101,6 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
     dst[1] = heads > 1 ? src[1] : 0;
     dst[2] = seq > 1 ? src[2] : 0;
   };
-  set(f.dqs, a->dq_stride, a->heads, a->seq_q);
   set(f.dks, a->dk_stride, a->kv_heads, a->seq_kv);
   set(f.dvs, a->dv_stride, a->kv_heads, a->seq_kv);
   const bool f16 = a->dtype == ATTN_BWD_DT_FP16;
@@ -120,6 +118,10 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
       (!map_bhsd(&mk, k, a->k_stride, a->bs, a->kv_heads, a->seq_kv, a->head_dim, f16, TILE, 1, true) ||
        !map_bhsd(&mv, v, a->v_stride, a->bs, a->kv_heads, a->seq_kv, a->head_dim, f16, TILE, 1, true)))
     return ATTN_BWD_ETMAP;
+  CUtensorMap mdq;
+  std::memset(&mdq, 0, sizeof(mdq));
+  if (a->seq_q && !map_bhsd(&mdq, dq, a->dq_stride, a->bs, a->heads, a->seq_q, a->head_dim, f16, 32, 1, true, true))
+    return ATTN_BWD_ETMAP;
   if (!a->seq_q) mq = md = mk;   // never loaded from, only prefetched
   if (!a->seq_kv) mk = mv = mq;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_);
@@ -132,7 +134,7 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
                                                                 const_cast<DocRange*>(f.c.qrange));
     if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
   }
-  if (a->seq_q && (rc = launch_dq(f, mq, md, mk, mv, d, f16, cap, s))) return rc;
+  if (a->seq_q && (rc = launch_dq(f, mq, md, mk, mv, mdq, d, f16, cap, s))) return rc;
   if (a->seq_kv && (rc = launch_dkv(f, mq, md, mk, mv, d, f16, cap, s))) return rc;
   return ATTN_BWD_OK;
 }

@@ -29,8 +29,8 @@ struct BwdParams {
   const float* lse;      // [bs, H, sq]
   float* nlse;           // [bs * H, sq_pad]: -lse * log2(e); -inf for rows that see nothing
   float* ndelta;         // [bs * H, sq_pad]: -sum(do * o); dq writes both, dkv reads them
-  void *dq, *dk, *dv;
-  long long dqs[3], dks[3], dvs[3];   // element strides: batch, head, position
+  void *dk, *dv;
+  long long dks[3], dvs[3];   // element strides: batch, head, position
   float* part;           // dkv, splits > 1: [split][bs * Hkv * skv][2][D], dk first
 };
 
@@ -42,7 +42,8 @@ struct BwdCfg {
   static constexpr int OFF_RING = 2 * TILE_BYTES;
   // dkv: 2 x (nlse, ndelta) of 128 rows; dq: 2 x (halves of 128 rows' delta)
   static constexpr int OFF_STAT = OFF_RING + ST * TILE_BYTES;
-  static constexpr int OFF_LIST = OFF_STAT + 2 * 2 * TILE * 4;
+  static constexpr int OFF_STAGE = OFF_STAT + 2 * 2 * TILE * 4;   // 2 KB for each warp of rows
+  static constexpr int OFF_LIST = OFF_STAGE + 8 * 2048;
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;
   static constexpr int NBAR = 3 + 2 * ST + 8 + 6;
@@ -158,7 +159,7 @@ __device__ __forceinline__ void weights4(const Params& p, const TanhSmall& ts, f
 int launch_dkv(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& go, const CUtensorMap& k,
                const CUtensorMap& v, int d, bool f16, bool cap, cudaStream_t s);
 int launch_dq(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& go, const CUtensorMap& k,
-              const CUtensorMap& v, int d, bool f16, bool cap, cudaStream_t s);
+              const CUtensorMap& v, const CUtensorMap& dq, int d, bool f16, bool cap, cudaStream_t s);
 
 }  // namespace fused
 }  // namespace attn_bwd

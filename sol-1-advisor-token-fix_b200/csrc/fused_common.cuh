@@ -251,6 +251,27 @@ __device__ __forceinline__ void write_row(const uint32_t (&w)[16], uint8_t* dst)
                  : "memory");
 }
 
+// The same through the warp's 2 KB of shared memory and one tensor store of 32 rows x 64 bytes (a map
+// with a box of 32 x 32 and the 64-byte swizzle): the warp goes on while the rows leave.  Rows behind
+// the end are cut off by the map.
+__device__ __forceinline__ void store_rows(uint32_t stage, const CUtensorMap* m, const uint32_t (&w)[16], int c0, int c1,
+                                           int c2, int c3, uint32_t lane) {
+  if (lane == 0) bulk_wait_read0();   // the store before this one has read the place
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    sts128(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(m)),
+                 "r"(stage), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+                 : "memory");
+    bulk_commit();
+  }
+}
+
 // Register split of the attention kernels: three warpgroups are launched with 168 registers a
 // thread (504 in sum); the two that hold score rows grow to 216, the one that issues copies and
 // products shrinks to 72: 216 + 216 + 72 = 504.  The host launches only kernels that ptxas

@@ -28,7 +28,9 @@ __device__ __forceinline__ DqUnit dq_unit(const BwdParams& prm, const Unit& u) {
 template <int D, bool F16, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
 dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
-          const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const BwdParams prm) {
+          const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+          const __grid_constant__ CUtensorMap tm_dq,   // (d, s, h, b), box (32, 32, 1, 1)
+          const BwdParams prm) {
   using C = BwdCfg<D>;
   constexpr int ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -192,6 +194,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
   } else {
     // ---------------------------------------------------------------- weights: one query a thread, 64 keys
     regs_grow();
+    const uint32_t stage = smem_u32(sh.smem + C::OFF_STAGE) + warp * 2048;
     constexpr int LR = D / 16;   // 16-byte words of half a row
     const TanhSmall tanh_small(p);
     const int half = int(warp) >> 2;
@@ -203,7 +206,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
       const DqUnit f = dq_unit(prm, u);
       const uint16_t* list = sh.lists + (k & 1) * kMaxList;
       const int row = f.r0 + int(warp & 3) * 32 + int(lane);
-      const bool valid = row < p.sq;
+      const bool valid = row < p.sq, any_valid = row - int(lane) < p.sq;
       const size_t ri = ((size_t)f.b * p.H + f.h) * prm.sq_pad + row;   // padded to whole tiles
       const float lse = valid ? __ldg(prm.lse + ((size_t)f.b * p.H + f.h) * p.sq + row) : -INFINITY;
       // o of these rows, this half of the columns, for delta: the lanes of a group of LR read one row's
@@ -349,8 +352,6 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         ++di;
       }
       tc_fence_after();
-      uint8_t* out = static_cast<uint8_t*>(prm.dq) + 2 * (f.b * prm.dqs[0] + f.h * prm.dqs[1] + row * prm.dqs[2]) +
-                     half * D;
       uint32_t v[D / 64][32];
 #pragma unroll
       for (int x = 0; x < D / 64; ++x)
@@ -368,33 +369,35 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           o[e] = pack2<F16>(__uint_as_float(v[x][2 * e]) * p.scale, __uint_as_float(v[x][2 * e + 1]) * p.scale);
-        if (valid) write_row(o, out + x * 64);
+        if (any_valid) store_rows(stage, &tm_dq, o, half * (D / 2) + x * 32, row - int(lane), f.h, f.b, lane);
       }
       tc_fence_before();   // the next unit's first product overwrites the accumulator
       unit_done(sh.sched, k);
     }
+    if (lane == 0) bulk_wait_all0();   // no store may outlive the block
+    __syncwarp();
   }
   bwd_end(sh, tmem, p.err);
 }
 
 template <int D, bool F16, bool CAP, bool BIAS>
 static int launch(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& go, const CUtensorMap& k,
-                  const CUtensorMap& v, cudaStream_t s) {
+                  const CUtensorMap& v, const CUtensorMap& dq, cudaStream_t s) {
   using C = BwdCfg<D>;
   const auto kern = dq_kernel<D, F16, CAP, BIAS>;
   const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
   if (rc) return rc;
-  kern<<<dim3(unsigned(f.c.n_tiles) * f.c.H, f.c.bs), kThreads, C::SMEM_BYTES, s>>>(q, go, k, v, f);
+  kern<<<dim3(unsigned(f.c.n_tiles) * f.c.H, f.c.bs), kThreads, C::SMEM_BYTES, s>>>(q, go, k, v, dq, f);
   return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;
 }
 
 int launch_dq(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& go, const CUtensorMap& k,
-              const CUtensorMap& v, int d, bool f16, bool cap, cudaStream_t s) {
+              const CUtensorMap& v, const CUtensorMap& dq, int d, bool f16, bool cap, cudaStream_t s) {
   const bool bias = f.c.slopes != nullptr;
 #define ATTN_BWD_PICK(DD, FF)                                                                                   \
   if (d == DD && f16 == FF)                                                                                     \
-    return cap ? (bias ? launch<DD, FF, true, true>(f, q, go, k, v, s) : launch<DD, FF, true, false>(f, q, go, k, v, s)) \
-               : (bias ? launch<DD, FF, false, true>(f, q, go, k, v, s) : launch<DD, FF, false, false>(f, q, go, k, v, s));
+    return cap ? (bias ? launch<DD, FF, true, true>(f, q, go, k, v, dq, s) : launch<DD, FF, true, false>(f, q, go, k, v, dq, s)) \
+               : (bias ? launch<DD, FF, false, true>(f, q, go, k, v, dq, s) : launch<DD, FF, false, false>(f, q, go, k, v, dq, s));
   ATTN_BWD_PICK(128, false)
   ATTN_BWD_PICK(128, true)
   ATTN_BWD_PICK(64, false)

@@ -98,6 +98,9 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
        !map_bhsd(&mv, v, a->v_stride, p.bs, p.Hkv, p.skv, a->head_dim, f16, TILE, 1, true)))
     return ATTN_BWD_ETMAP;
   if (p.skv == 0) mk = mv = mq;   // never loaded from, only prefetched
+  const int64_t os[3] = {(int64_t)p.sq * p.H * a->head_dim, a->head_dim, (int64_t)p.H * a->head_dim};
+  CUtensorMap mo;
+  if (!map_bhsd(&mo, o, os, p.bs, p.H, p.sq, a->head_dim, f16, 32, 1, false, true)) return ATTN_BWD_ETMAP;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_);
   const bool cap = a->softcap > 0.f;
   if (p.has_docs && p.n_tiles > 0) {
@@ -106,7 +109,7 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
                                                                const_cast<DocRange*>(p.krange), nullptr);
     if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
   }
-  rc = f.duo ? launch_token(f, mq, mk, mv, a->head_dim, f16, cap, s) : launch_fwd(f, mq, mk, mv, a->head_dim, f16, cap, s);
+  rc = f.duo ? launch_token(f, mq, mk, mv, mo, a->head_dim, f16, cap, s) : launch_fwd(f, mq, mk, mv, mo, a->head_dim, f16, cap, s);
   if (rc || p.splits == 1) return rc;
   const long long rows = (long long)p.bs * p.H * p.sq;
   const dim3 grid(unsigned((rows + 7) / 8));

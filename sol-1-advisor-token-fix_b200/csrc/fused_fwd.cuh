@@ -55,7 +55,8 @@ struct FwdCfg {
   static constexpr int ST = (D == 128 ? 6 : 10) - QT;          // stages of keys or values
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = QT * TILE_BYTES;
-  static constexpr int OFF_LIST = OFF_KV + ST * TILE_BYTES;    // a list for each unit slot
+  static constexpr int OFF_STAGE = OFF_KV + ST * TILE_BYTES;   // 2 KB for each warp of rows
+  static constexpr int OFF_LIST = OFF_STAGE + (DUO ? 0 : 8 * 2048);   // a list for each unit slot
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;            // two slots, the scheduler's answer
   static constexpr int NBAR = 3 + 2 * ST + 8 + 6;
@@ -110,7 +111,9 @@ template <int D, bool F16, bool CAP, bool BIAS, bool DUO>
 __global__ void __launch_bounds__(kThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64, heads of a row, positions, 1)
            const __grid_constant__ CUtensorMap tm_k,   // (d, s, h, b), box (64, 128, 1, 1)
-           const __grid_constant__ CUtensorMap tm_v, const FwdParams prm) {
+           const __grid_constant__ CUtensorMap tm_v,
+           const __grid_constant__ CUtensorMap tm_o,   // (d, h, s, b), box (32, 1, 32, 1): unpacked rows' results
+           const FwdParams prm) {
   using C = FwdCfg<D, DUO>;
   constexpr int ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -379,6 +382,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + t_lane + t * TILE, t_o = tmem + t_lane + 2 * TILE + t * D;
     const int row = int(warp & 3) * 32 + int(lane);
+    const uint32_t stage = smem_u32(smem + C::OFF_STAGE) + warp * 2048;
     // scores that are only scaled stay raw and are scaled inside the exponent
     const float c = BIAS || CAP ? 1.f : p.scale_log2;
     const float grow = fminf(8.f / c, 3e38f);
@@ -645,13 +649,19 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               w[e] = empty ? 0u : pack2<F16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-            if (valid) write_row(w, dst + x * 64);
+            if (DUO || prm.packed) {
+              if (valid) write_row(w, dst + x * 64);
+            } else {
+              store_rows(stage, &tm_o, w, x * 32, head, pos - int(lane), f.b, lane);
+            }
           }
         }
         tc_fence_before();   // the next unit's first product overwrites the accumulator
       }
       unit_done(sched, k);
     }
+    if (lane == 0) bulk_wait_all0();   // no store may outlive the block
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -703,34 +713,34 @@ __global__ void __launch_bounds__(256) fwd_join_kernel(const FwdParams prm) {
 }
 
 // fused_fwd.cu, fused_token.cu (units of one tile)
-int launch_fwd(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int d, bool f16,
+int launch_fwd(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, int d, bool f16,
                bool cap, cudaStream_t s);
-int launch_token(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int d, bool f16,
+int launch_token(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, int d, bool f16,
                  bool cap, cudaStream_t s);
 
 #define ATTN_BWD_FWD_LAUNCHER(NAME, DUO)                                                                               \
   template <int D, bool F16, bool CAP, bool BIAS>                                                                      \
   static int NAME##_one(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,          \
-                        cudaStream_t stream) {                                                                         \
+                        const CUtensorMap& o, cudaStream_t stream) {                                                                         \
     using C = FwdCfg<D, DUO>;                                                                                               \
     const auto kern = fwd_kernel<D, F16, CAP, BIAS, DUO>;                                                              \
     const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);                                 \
     if (rc) return rc;                                                                                                 \
-    kern<<<dim3(unsigned(f.blocks_q) * f.head_slots, f.c.bs, f.cta_splits), kThreads, C::SMEM_BYTES, stream>>>(q, k, v, f); \
+    kern<<<dim3(unsigned(f.blocks_q) * f.head_slots, f.c.bs, f.cta_splits), kThreads, C::SMEM_BYTES, stream>>>(q, k, v, o, f); \
     return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;                                        \
   }                                                                                                                    \
-  int NAME(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int d, bool f16,      \
+  int NAME(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, int d, bool f16,      \
            bool cap, cudaStream_t s) {                                                                                 \
     const bool bias = f.c.slopes != nullptr;                                                                           \
     if (d == 128)                                                                                                      \
-      return f16 ? (cap ? (bias ? NAME##_one<128, true, true, true>(f, q, k, v, s) : NAME##_one<128, true, true, false>(f, q, k, v, s))     \
-                        : (bias ? NAME##_one<128, true, false, true>(f, q, k, v, s) : NAME##_one<128, true, false, false>(f, q, k, v, s)))  \
-                 : (cap ? (bias ? NAME##_one<128, false, true, true>(f, q, k, v, s) : NAME##_one<128, false, true, false>(f, q, k, v, s))   \
-                        : (bias ? NAME##_one<128, false, false, true>(f, q, k, v, s) : NAME##_one<128, false, false, false>(f, q, k, v, s))); \
-    return f16 ? (cap ? (bias ? NAME##_one<64, true, true, true>(f, q, k, v, s) : NAME##_one<64, true, true, false>(f, q, k, v, s))         \
-                      : (bias ? NAME##_one<64, true, false, true>(f, q, k, v, s) : NAME##_one<64, true, false, false>(f, q, k, v, s)))      \
-               : (cap ? (bias ? NAME##_one<64, false, true, true>(f, q, k, v, s) : NAME##_one<64, false, true, false>(f, q, k, v, s))       \
-                      : (bias ? NAME##_one<64, false, false, true>(f, q, k, v, s) : NAME##_one<64, false, false, false>(f, q, k, v, s)));   \
+      return f16 ? (cap ? (bias ? NAME##_one<128, true, true, true>(f, q, k, v, o, s) : NAME##_one<128, true, true, false>(f, q, k, v, o, s))     \
+                        : (bias ? NAME##_one<128, true, false, true>(f, q, k, v, o, s) : NAME##_one<128, true, false, false>(f, q, k, v, o, s)))  \
+                 : (cap ? (bias ? NAME##_one<128, false, true, true>(f, q, k, v, o, s) : NAME##_one<128, false, true, false>(f, q, k, v, o, s))   \
+                        : (bias ? NAME##_one<128, false, false, true>(f, q, k, v, o, s) : NAME##_one<128, false, false, false>(f, q, k, v, o, s))); \
+    return f16 ? (cap ? (bias ? NAME##_one<64, true, true, true>(f, q, k, v, o, s) : NAME##_one<64, true, true, false>(f, q, k, v, o, s))         \
+                      : (bias ? NAME##_one<64, true, false, true>(f, q, k, v, o, s) : NAME##_one<64, true, false, false>(f, q, k, v, o, s)))      \
+               : (cap ? (bias ? NAME##_one<64, false, true, true>(f, q, k, v, o, s) : NAME##_one<64, false, true, false>(f, q, k, v, o, s))       \
+                      : (bias ? NAME##_one<64, false, false, true>(f, q, k, v, o, s) : NAME##_one<64, false, false, false>(f, q, k, v, o, s)));   \
   }
 
 }  // namespace fused
