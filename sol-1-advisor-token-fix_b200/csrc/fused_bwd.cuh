@@ -46,7 +46,7 @@ struct BwdCfg {
   static constexpr int OFF_LIST = OFF_STAGE + 8 * 2048;
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;
-  static constexpr int NBAR = 3 + 2 * ST + 8 + 6;
+  static constexpr int NBAR = 3 + 2 * ST + 8 + 6 + 4;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int SMEM_BYTES = OFF_MISC + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024, "backward kernel shared memory");
@@ -55,6 +55,7 @@ struct BwdCfg {
 struct BwdShared {
   uint8_t* smem;
   uint64_t *res_full, *res_empty, *all_done, *full, *empty, *s_full, *p_ready, *dp_full, *ds_ready, *done;
+  uint64_t* pair;   // dq: [quadrant] the two warps of its rows
   uint32_t* tmem_slot;
   volatile int* abort_flag;
   uint16_t* lists;
@@ -82,6 +83,7 @@ __device__ __forceinline__ BwdShared bwd_shared(uint8_t* raw) {
   s.sched.empty = s.sched.full + 2;
   s.sched.answer = s.sched.empty + 2;
   s.sched.ask = s.sched.answer + 1;
+  s.pair = s.sched.ask + 1;
   s.tmem_slot = reinterpret_cast<uint32_t*>(s.smem + C::OFF_MISC);
   s.abort_flag = reinterpret_cast<volatile int*>(s.smem + C::OFF_MISC + 4);
   s.lists = reinterpret_cast<uint16_t*>(s.smem + C::OFF_LIST);
@@ -102,6 +104,7 @@ __device__ __forceinline__ uint32_t bwd_begin(const BwdShared& s, int st, int re
     for (int i = 0; i < 2; ++i) { mbar_init(&s.p_ready[i], 8); mbar_init(&s.ds_ready[i], 8); }
     mbar_init(s.dp_full, 1);
     mbar_init(s.done, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&s.pair[i], 2);
     scheduler_init(s.sched);
     *s.abort_flag = 0;
     fence_barrier_init();

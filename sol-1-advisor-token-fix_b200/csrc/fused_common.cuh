@@ -70,6 +70,13 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatil
       : "memory");
   return __all_sync(0xffffffffu, ok != 0);
 }
+// Barrier of some warps of one block, bounded like every wait (a named barrier would hold warps for
+// good if one of them had given up): bar counts the warps, n their meetings so far.
+__device__ __forceinline__ bool meet(uint64_t* bar, uint32_t& n, volatile int* flag, int code) {
+  __syncwarp();
+  if (lane_id() == 0) mbar_arrive(bar);
+  return wait_for(bar, n++ & 1, flag, code);
+}
 __device__ __forceinline__ void report_error(volatile int* flag, int* err) {
   if (threadIdx.x == 0 && *flag) raise_error(err, *flag);
 }

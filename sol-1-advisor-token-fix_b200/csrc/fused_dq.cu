@@ -200,7 +200,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
     const int half = int(warp) >> 2;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t dp = t_dp + t_lane + half * 64;
-    uint32_t it = 0, di = 0;
+    uint32_t it = 0, di = 0, met = 0;
     bool ok = true;
     for (uint32_t k = 0; ok && next_unit(sh.sched, k, u, sh.abort_flag, 0x4304); ++k) {
       const DqUnit f = dq_unit(prm, u);
@@ -304,7 +304,8 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(sh.res_empty);
-          named_bar_sync(1 + (warp & 3), 64);   // the two warps of these rows
+          ok = meet(&sh.pair[warp & 3], met, sh.abort_flag, 0x4306);   // the two warps of these rows
+          if (!ok) break;
           const float d = part[r] + part[TILE + r];
           const float nd = none ? 0.f : -d;
           nd2 = f2(nd, nd);

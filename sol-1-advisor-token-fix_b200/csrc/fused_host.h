@@ -79,8 +79,8 @@ inline Params base_params(const attn_bwd_fused_t* a) {
 
 // Map of a [bs, heads, seq, d] tensor with given element strides in the dimension order
 // (d, position, head, batch); the box is 64 elements of `rows` positions of one head.
-// seq_first = false: order (d, head, position, batch), box 64 x box_heads x rows.  store: the box of
-// store_rows instead, 32 elements of 32 positions.
+// seq_first = false: order (d, head, position, batch), box 64 x box_heads x rows.  store: boxes of
+// 32 elements instead, for store_rows.
 inline bool map_bhsd(CUtensorMap* m, const void* ptr, const int64_t* st, int bs, int heads, int seq, int d, bool f16,
                      int rows, int box_heads, bool seq_first, bool store = false) {
   // an extent of 1 is never stepped over, but its stride must still be a valid one
@@ -97,11 +97,7 @@ inline bool map_bhsd(CUtensorMap* m, const void* ptr, const int64_t* st, int bs,
     box[1] = (cuuint32_t)box_heads;
     box[2] = (cuuint32_t)rows;
   }
-  if (store) {
-    box[0] = 32;
-    box[1] = seq_first ? 32 : 1;
-    box[2] = seq_first ? 1 : 32;
-  }
+  if (store) box[0] = 32;
   return host_make_map(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, ptr, dims, str,
                        box, store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
