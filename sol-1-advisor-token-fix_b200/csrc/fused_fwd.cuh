@@ -635,7 +635,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             tmem_ld32(t_o + x * 32, o);
             tmem_wait_ld();
           }
-          if (p.splits > 1) {
+          if (DUO || p.splits > 1) {   // DUO leaves two parts at least
             if (valid) {
               float4* part = reinterpret_cast<float4*>(prm.part_o + ri * D + x * 32);
 #pragma unroll
@@ -649,7 +649,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               w[e] = empty ? 0u : pack2<F16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-            if (DUO || prm.packed) {   // (position, head) rows are no box
+            if (prm.packed) {   // (position, head) rows are no box
               if (valid) write_row(w, dst + x * 64);
             } else {
               store_rows(stage, &tm_o, w, x * 32, head, pos - int(lane), f.b, lane);
