@@ -424,12 +424,6 @@ __device__ __forceinline__ void same_ids(const int (&v)[N], int id, uint32_t (&s
     todo &= ~__ballot_sync(0xffffffffu, id == cur);
   }
 }
-__device__ __forceinline__ uint32_t same_id(int v, int id) {
-  uint32_t same[1];
-  const int w[1] = {v};
-  same_ids<1>(w, id, same);
-  return same[0];
-}
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // kind::f16 instruction descriptor for fp16 (0) or bf16 (1) operands, f32 accumulator.
