@@ -1,4 +1,5 @@
-// fused_dkv.cu — gradients of keys and values (see fused_bwd.cuh).
+// fused_dkv.cu — gradients of keys and values (see fused_bwd.cuh).  8192 packed positions in documents of
+// about 2500, 80 + 8 heads of 128: 831 us; 48 sequences of 640, capped: 1030 us.
 #include "fused_bwd.cuh"
 #include "fused_host.h"
 
@@ -384,7 +385,8 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
   bwd_end(sh, tmem, p.err);
 }
 
-// Sums the splits of dk and dv, in order.  D / 4 lanes a row of one of the two.
+// Sums the splits of dk and dv, in order.  D / 4 lanes a row of one of the two.  Bound by its launch (2 x
+// 96 keys of 8 heads: 3.5 us).
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) dkv_join_kernel(const BwdParams prm) {
   const Params& p = prm.c;

@@ -1,7 +1,6 @@
 // fused_fwd.cu — C entry point of the fused attention forward: the plan (which rows share a
 // tile, how the keys are split), descriptors and launches.
 #include "fused_fwd.cuh"
-#include "fused_host.h"
 
 using namespace attn_bwd;
 using namespace attn_bwd::fused;
@@ -18,21 +17,27 @@ static FwdParams plan_fwd(const attn_bwd_fused_t* a, int sm_count) {
   const long long whole = (long long)p.H * ((p.sq + TILE - 1) / TILE);
   const int ppt = p.G <= TILE ? TILE / p.G : 0;
   const long long packed = ppt ? (long long)p.Hkv * ((p.sq + ppt - 1) / ppt) : whole;
+  // Rows of a group share a tile where that takes fewer tiles (one token over 40000 keys, 80 + 8
+  // heads: 50 us, 200 with a tile a head; 77 tokens over 32013 keys: 142 and 175), though the rows
+  // of whole tiles are written faster.
   f.packed = p.G > 1 && packed < whole;
   f.pos_per_tile = f.packed ? ppt : TILE;
   // two heads of a group have the same keys and the same masks, so a pair of them wastes
-  // nothing at the diagonal; an odd group takes 256 positions of a head instead
+  // nothing at the diagonal (16 documents of 640, causal, 10 heads a group: 204 us, 260 with 256
+  // positions of a head, which is what an odd group takes)
   f.pair_heads = !f.packed && p.G % 2 == 0;
   f.head_slots = f.packed ? p.Hkv : f.pair_heads ? p.H / 2 : p.H;
   f.div_slots = fast_div(f.head_slots);
   const int pos_per_unit = f.packed ? 2 * ppt : f.pair_heads ? TILE : 2 * TILE;
   f.blocks_q = (p.sq + pos_per_unit - 1) / pos_per_unit;
   p.n_tiles = (p.skv + TILE - 1) / TILE;
-  // Too few units for the GPU: split the keys, two tiles a split at least (below that the
-  // join costs more than it saves), and never more tiles than a unit's list holds.
-  // (two chains in a CTA: the same two tiles for each)
+  // Two chains in a CTA where a unit's rows fit one tile and there is more than one key tile (4 tokens
+  // over 8191 keys: 32 us, 38 with one chain).
   f.duo = p.n_tiles > 1 && !f.pair_heads && f.blocks_q == 1 && p.sq <= f.pos_per_tile;
   const int parts = f.duo ? 2 : 1;
+  // Too few units for the GPU: the keys are split (one token over 40000 keys: 50 us, 292 without; 77
+  // tokens over 32013: 142 and 463), two tiles a split at least (one a split is no faster and
+  // leaves more to join), and never more tiles than a unit's list holds.
   const long long units = (long long)f.blocks_q * f.head_slots * p.bs;
   long long splits = units > 0 ? sm_count / units : 1;
   if (splits > p.n_tiles / 2) splits = p.n_tiles / 2;
@@ -58,7 +63,9 @@ int64_t fwd_workspace(const attn_bwd_fused_t* a, int sm_count) {
   return range_bytes(f.c) + part_rows(f.c) * (a->head_dim + 1) * 4;
 }
 
-ATTN_BWD_FWD_LAUNCHER(launch_fwd, false)
+int launch_fwd(const FwdParams& f, const FwdMaps& m, int d, bool f16, bool cap, cudaStream_t s) {
+  return launch_any<false>(f, m, d, f16, cap, s);
+}
 
 }  // namespace fused
 }  // namespace attn_bwd
@@ -88,19 +95,16 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
     f.part_lse = f.part_o + part_rows(p) * a->head_dim;
   }
   const bool f16 = a->dtype == ATTN_BWD_DT_FP16;
-  CUtensorMap mq, mk, mv;
-  std::memset(&mk, 0, sizeof(mk));
-  std::memset(&mv, 0, sizeof(mv));
-  if (!map_bhsd(&mq, q, a->q_stride, p.bs, p.H, p.sq, a->head_dim, f16, f.pos_per_tile, f.packed ? p.G : 1, false))
-    return ATTN_BWD_ETMAP;
-  if (p.skv > 0 &&
-      (!map_bhsd(&mk, k, a->k_stride, p.bs, p.Hkv, p.skv, a->head_dim, f16, TILE, 1, true) ||
-       !map_bhsd(&mv, v, a->v_stride, p.bs, p.Hkv, p.skv, a->head_dim, f16, TILE, 1, true)))
-    return ATTN_BWD_ETMAP;
-  if (p.skv == 0) mk = mv = mq;   // never loaded from, only prefetched
+  FwdMaps m;
   const int64_t os[3] = {(int64_t)p.sq * p.H * a->head_dim, a->head_dim, (int64_t)p.H * a->head_dim};
-  CUtensorMap mo;
-  if (!map_bhsd(&mo, o, os, p.bs, p.H, p.sq, a->head_dim, f16, 32, 1, false, true)) return ATTN_BWD_ETMAP;
+  if (!map_bhsd(&m.q, q, a->q_stride, p.bs, p.H, p.sq, a->head_dim, f16, f.pos_per_tile, f.packed ? p.G : 1, false) ||
+      !map_bhsd(&m.o, o, os, p.bs, p.H, p.sq, a->head_dim, f16, 32, 1, false, true))
+    return ATTN_BWD_ETMAP;
+  m.k = m.v = m.q;   // without keys: never loaded from, only prefetched
+  if (p.skv > 0 &&
+      (!map_bhsd(&m.k, k, a->k_stride, p.bs, p.Hkv, p.skv, a->head_dim, f16, TILE, 1, true) ||
+       !map_bhsd(&m.v, v, a->v_stride, p.bs, p.Hkv, p.skv, a->head_dim, f16, TILE, 1, true)))
+    return ATTN_BWD_ETMAP;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_);
   const bool cap = a->softcap > 0.f;
   if (p.has_docs && p.n_tiles > 0) {
@@ -109,7 +113,7 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
                                                                const_cast<DocRange*>(p.krange), nullptr);
     if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
   }
-  rc = f.duo ? launch_token(f, mq, mk, mv, mo, a->head_dim, f16, cap, s) : launch_fwd(f, mq, mk, mv, mo, a->head_dim, f16, cap, s);
+  rc = f.duo ? launch_token(f, m, a->head_dim, f16, cap, s) : launch_fwd(f, m, a->head_dim, f16, cap, s);
   if (rc || p.splits == 1) return rc;
   const long long rows = (long long)p.bs * p.H * p.sq;
   const dim3 grid(unsigned((rows + 7) / 8));

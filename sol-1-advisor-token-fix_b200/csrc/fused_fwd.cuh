@@ -21,6 +21,12 @@
 // tiles for the same rows instead (DUO): what bounds such a unit is the chain of scores, softmax and
 // product per tile, and two chains run side by side.  Each leaves its part to be joined.
 //
+// What bounds it: with few rows the keys and values, read once (4 tokens over 8191 keys, 80 + 8 heads of
+// 128: 28 us, 4.8 TB/s); with many, turning scores into weights: 4096 x 4096, 80 + 8 heads of 128, bf16
+// take 560 us without a mask (1.23 PFLOP/s) and 300 us causal (1.15 of what is seen), where the
+// tensor cores are active half of the time and the exponentials' unit as long.  A bias costs 455
+// us, a cap 430 (both causal), since each adds instructions to every score.
+//
 // Rows of a query tile are 128 positions of one head or, where that needs fewer tiles, up to
 // 128 (position, head) pairs of one group (few positions, as when tokens are generated): a
 // group's heads read the same keys.
@@ -28,6 +34,7 @@
 #include <type_traits>
 
 #include "fused_common.cuh"
+#include "fused_host.h"
 
 namespace attn_bwd {
 namespace fused {
@@ -685,7 +692,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
 }
 
 // Joins the splits of every row: o = sum_s 2^(lse_s - lse) o_s.  One warp a row; the sum
-// over splits runs in order, so equal inputs give equal bits.
+// over splits runs in order, so equal inputs give equal bits.  Bound by its launch and the latency of
+// its loads: 4 us for 320 rows of 8 parts, 6 us for 3080 rows of 18.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) fwd_join_kernel(const FwdParams prm) {
   const Params& p = prm.c;
@@ -723,36 +731,35 @@ __global__ void __launch_bounds__(256) fwd_join_kernel(const FwdParams prm) {
   if (lane == 0) prm.lse[r] = mx == -INFINITY ? -INFINITY : mx + logf(l);
 }
 
+// The tensor maps of a call.
+struct FwdMaps {
+  CUtensorMap q, k, v, o;
+};
 // fused_fwd.cu, fused_token.cu (units of one tile)
-int launch_fwd(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, int d, bool f16,
-               bool cap, cudaStream_t s);
-int launch_token(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, int d, bool f16,
-                 bool cap, cudaStream_t s);
+int launch_fwd(const FwdParams& f, const FwdMaps& m, int d, bool f16, bool cap, cudaStream_t s);
+int launch_token(const FwdParams& f, const FwdMaps& m, int d, bool f16, bool cap, cudaStream_t s);
 
-#define ATTN_BWD_FWD_LAUNCHER(NAME, DUO)                                                                               \
-  template <int D, bool F16, bool CAP, bool BIAS>                                                                      \
-  static int NAME##_one(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,          \
-                        const CUtensorMap& o, cudaStream_t stream) {                                                                         \
-    using C = FwdCfg<D, DUO>;                                                                                               \
-    const auto kern = fwd_kernel<D, F16, CAP, BIAS, DUO>;                                                              \
-    const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);                                 \
-    if (rc) return rc;                                                                                                 \
-    kern<<<dim3(unsigned(f.blocks_q) * f.head_slots, f.c.bs, f.cta_splits), kThreads, C::SMEM_BYTES, stream>>>(q, k, v, o, f); \
-    return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;                                        \
-  }                                                                                                                    \
-  int NAME(const FwdParams& f, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, int d, bool f16,      \
-           bool cap, cudaStream_t s) {                                                                                 \
-    const bool bias = f.c.slopes != nullptr;                                                                           \
-    if (d == 128)                                                                                                      \
-      return f16 ? (cap ? (bias ? NAME##_one<128, true, true, true>(f, q, k, v, o, s) : NAME##_one<128, true, true, false>(f, q, k, v, o, s))     \
-                        : (bias ? NAME##_one<128, true, false, true>(f, q, k, v, o, s) : NAME##_one<128, true, false, false>(f, q, k, v, o, s)))  \
-                 : (cap ? (bias ? NAME##_one<128, false, true, true>(f, q, k, v, o, s) : NAME##_one<128, false, true, false>(f, q, k, v, o, s))   \
-                        : (bias ? NAME##_one<128, false, false, true>(f, q, k, v, o, s) : NAME##_one<128, false, false, false>(f, q, k, v, o, s))); \
-    return f16 ? (cap ? (bias ? NAME##_one<64, true, true, true>(f, q, k, v, o, s) : NAME##_one<64, true, true, false>(f, q, k, v, o, s))         \
-                      : (bias ? NAME##_one<64, true, false, true>(f, q, k, v, o, s) : NAME##_one<64, true, false, false>(f, q, k, v, o, s)))      \
-               : (cap ? (bias ? NAME##_one<64, false, true, true>(f, q, k, v, o, s) : NAME##_one<64, false, true, false>(f, q, k, v, o, s))       \
-                      : (bias ? NAME##_one<64, false, false, true>(f, q, k, v, o, s) : NAME##_one<64, false, false, false>(f, q, k, v, o, s)));   \
-  }
+template <bool DUO, int D, bool F16, bool CAP, bool BIAS>
+static int launch_one(const FwdParams& f, const FwdMaps& m, cudaStream_t stream) {
+  using C = FwdCfg<D, DUO>;
+  const auto kern = fwd_kernel<D, F16, CAP, BIAS, DUO>;
+  const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
+  if (rc) return rc;
+  const dim3 grid(unsigned(f.blocks_q) * f.head_slots, f.c.bs, f.cta_splits);
+  kern<<<grid, kThreads, C::SMEM_BYTES, stream>>>(m.q, m.k, m.v, m.o, f);
+  return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;
+}
+template <bool DUO, int D, bool F16>
+static int launch_scores(const FwdParams& f, const FwdMaps& m, bool cap, cudaStream_t s) {
+  if (f.c.slopes)
+    return cap ? launch_one<DUO, D, F16, true, true>(f, m, s) : launch_one<DUO, D, F16, false, true>(f, m, s);
+  return cap ? launch_one<DUO, D, F16, true, false>(f, m, s) : launch_one<DUO, D, F16, false, false>(f, m, s);
+}
+template <bool DUO>
+static int launch_any(const FwdParams& f, const FwdMaps& m, int d, bool f16, bool cap, cudaStream_t s) {
+  if (d == 128) return f16 ? launch_scores<DUO, 128, true>(f, m, cap, s) : launch_scores<DUO, 128, false>(f, m, cap, s);
+  return f16 ? launch_scores<DUO, 64, true>(f, m, cap, s) : launch_scores<DUO, 64, false>(f, m, cap, s);
+}
 
 }  // namespace fused
 }  // namespace attn_bwd
