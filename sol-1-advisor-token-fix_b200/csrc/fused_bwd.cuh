@@ -122,6 +122,7 @@ __device__ __forceinline__ uint32_t bwd_begin(const BwdShared& s, int st, int re
     prefetch_tmap(v);
   }
   if (warp == 9) { tmem_alloc(s.tmem_slot, 512); tmem_relinquish(); }
+  wait_for_previous();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -81,6 +81,13 @@ __device__ __forceinline__ void report_error(volatile int* flag, int* err) {
   if (threadIdx.x == 0 && *flag) raise_error(err, *flag);
 }
 
+// The kernels of a call follow one another closely (programmatic dependent launch): each lets the next
+// one's blocks in when its own blocks are on their last unit, and waits, after setting up barriers and
+// TMEM and before it touches any tensor, for the one before it to have finished and its results to be
+// visible.  Without such a launch neither does anything.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Number of keys (from key 0) that query row `r` of batch row b sees when documents are left
 // out of account: a prefix, then causal.  Never above skv; 0 or less: none.
 __device__ __forceinline__ int row_limit(const Params& p, int r, int pre) {
@@ -117,6 +124,7 @@ __device__ __forceinline__ DocRange warp_doc_range(const int* ids, int n, uint32
 static __global__ void __launch_bounds__(256) doc_ranges_kernel(const int* __restrict__ kdoc, int skv,
                                                                 const int* __restrict__ qdoc, int sq, int bs,
                                                                 DocRange* __restrict__ kr, DocRange* __restrict__ qr) {
+  let_next_start();
   const int nk = (skv + TILE - 1) / TILE, nq = (sq + TILE - 1) / TILE;
   long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const uint32_t lane = threadIdx.x & 31;
@@ -218,7 +226,10 @@ __device__ __forceinline__ void run_scheduler(const Scheduler& s, volatile int* 
       s.slot[i] = Unit{have ? x : -1, y, z, n};
       mbar_arrive(&s.full[i]);
     }
-    if (!have) return;
+    if (!have) {
+      if (lane == 0) let_next_start();
+      return;
+    }
     // not earlier: a CTA that took its next unit at once would hold it while others run dry
     if (!wait_for(s.ask, k & 1, abort, code + 2)) return;
     if (lane == 0) {

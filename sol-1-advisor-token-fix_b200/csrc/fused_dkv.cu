@@ -389,6 +389,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
 // 96 keys of 8 heads: 3.5 us).
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) dkv_join_kernel(const BwdParams prm) {
+  wait_for_previous();
   const Params& p = prm.c;
   constexpr int L = D / 4;
   const long long idx = ((long long)blockIdx.x * 256 + threadIdx.x) / L;   // (b, kvh, j, which)
@@ -412,16 +413,13 @@ static int launch(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& g
   using C = BwdCfg<D>;
   const Params& p = f.c;
   const auto kern = dkv_kernel<D, F16, CAP, BIAS>;
-  const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
+  int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
   if (rc) return rc;
-  kern<<<dim3(unsigned(f.n_kt) * p.Hkv, p.bs, p.splits), kThreads, C::SMEM_BYTES, s>>>(q, go, k, v, f);
-  if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
-  if (p.splits > 1) {
-    const long long t = (long long)p.bs * p.Hkv * p.skv * 2 * (D / 4);
-    dkv_join_kernel<D, F16><<<unsigned((t + 255) / 256), 256, 0, s>>>(f);
-    if (cudaPeekAtLastError() != cudaSuccess) return ATTN_BWD_ECUDA;
-  }
-  return ATTN_BWD_OK;
+  const dim3 grid(unsigned(f.n_kt) * p.Hkv, p.bs, p.splits);
+  rc = launch_kernel(kern, grid, kThreads, C::SMEM_BYTES, s, p.sq > 0 || p.has_docs, q, go, k, v, f);
+  if (rc || p.splits == 1) return rc;
+  const long long t = (long long)p.bs * p.Hkv * p.skv * 2 * (D / 4);
+  return launch_kernel(dkv_join_kernel<D, F16>, dim3(unsigned((t + 255) / 256)), 256, 0, s, true, f);
 }
 
 int launch_dkv(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& go, const CUtensorMap& k,

@@ -390,8 +390,8 @@ static int launch(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& g
   const auto kern = dq_kernel<D, F16, CAP, BIAS>;
   const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
   if (rc) return rc;
-  kern<<<dim3(unsigned(f.c.n_tiles) * f.c.H, f.c.bs), kThreads, C::SMEM_BYTES, s>>>(q, go, k, v, dq, f);
-  return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;
+  const dim3 grid(unsigned(f.c.n_tiles) * f.c.H, f.c.bs);
+  return launch_kernel(kern, grid, kThreads, C::SMEM_BYTES, s, f.c.has_docs, q, go, k, v, dq, f);
 }
 
 int launch_dq(const BwdParams& f, const CUtensorMap& q, const CUtensorMap& go, const CUtensorMap& k,

@@ -117,12 +117,7 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
   if (rc || p.splits == 1) return rc;
   const long long rows = (long long)p.bs * p.H * p.sq;
   const dim3 grid(unsigned((rows + 7) / 8));
-  if (a->head_dim == 128) {
-    if (f16) fwd_join_kernel<128, true><<<grid, 256, 0, s>>>(f);
-    else fwd_join_kernel<128, false><<<grid, 256, 0, s>>>(f);
-  } else {
-    if (f16) fwd_join_kernel<64, true><<<grid, 256, 0, s>>>(f);
-    else fwd_join_kernel<64, false><<<grid, 256, 0, s>>>(f);
-  }
-  return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;
+  const auto join = a->head_dim == 128 ? (f16 ? fwd_join_kernel<128, true> : fwd_join_kernel<128, false>)
+                                       : (f16 ? fwd_join_kernel<64, true> : fwd_join_kernel<64, false>);
+  return launch_kernel(join, grid, 256, 0, s, true, f);
 }

@@ -164,6 +164,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
     prefetch_tmap(&tm_v);
   }
   if (warp == 9) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  wait_for_previous();
   if (prm.packed) {
     // rows behind the last (position, head) pair of a tile are never loaded; what stood there
     // would take part in the warps' votes, and results would not be the same bits each time
@@ -696,6 +697,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
 // its loads: 4 us for 320 rows of 8 parts, 6 us for 3080 rows of 18.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) fwd_join_kernel(const FwdParams prm) {
+  wait_for_previous();
   const Params& p = prm.c;
   const long long rows = (long long)p.bs * p.H * p.sq;
   const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -746,8 +748,7 @@ static int launch_one(const FwdParams& f, const FwdMaps& m, cudaStream_t stream)
   const int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::SMEM_BYTES);
   if (rc) return rc;
   const dim3 grid(unsigned(f.blocks_q) * f.head_slots, f.c.bs, f.cta_splits);
-  kern<<<grid, kThreads, C::SMEM_BYTES, stream>>>(m.q, m.k, m.v, m.o, f);
-  return cudaPeekAtLastError() == cudaSuccess ? ATTN_BWD_OK : ATTN_BWD_ECUDA;
+  return launch_kernel(kern, grid, kThreads, C::SMEM_BYTES, stream, f.c.has_docs && f.c.n_tiles > 0, m.q, m.k, m.v, m.o, f);
 }
 template <bool DUO, int D, bool F16>
 static int launch_scores(const FwdParams& f, const FwdMaps& m, bool cap, cudaStream_t s) {
