@@ -128,8 +128,8 @@ def fused_attn_fwd(query_states, key_states, value_states, scale=None, softcap=0
     """Attention forward.  Returns (attn_output [bs, seq_q, heads, d], lse [bs, heads, seq_q] float32).
 
     query_states [bs, heads, seq_q, d], key_states and value_states [bs, kv_heads, seq_kv, d], bfloat16 or float16,
-    d 64 or 128, heads a multiple of kv_heads; any strides (copied only where head elements are
-    not contiguous or rows not 16-byte aligned).  The queries are the last seq_q positions: one
+    d 64 or 128, heads a multiple of kv_heads, batch and heads at most 65535; any strides (copied
+    only where head elements are not contiguous or rows not 16-byte aligned).  The queries are the last seq_q positions: one
     row of queries over a long cache is a decoding step.
 
     The score of head h, query position i and key j is x = scale * q.k (default scale
@@ -162,8 +162,8 @@ def fused_attn_bwd(grad_attn_output, query_states, key_states, value_states, att
     """Gradients (grad_query, grad_key, grad_value) of :func:`fused_attn_fwd`'s first three
     arguments, from grad_attn_output [bs, seq_q, heads, d] and that call's results; the other
     arguments as they were given there.  The gradients have the shapes of the states (keys' and
-    values' summed over the heads that share them) and their order in memory.  Equal inputs
-    give equal bits."""
+    values' summed over the heads that share them) and their order in memory.  With documents,
+    at most 262144 positions.  Equal inputs give equal bits."""
     softcap = softcap or 0.0
     mods = (query_states, key_states, value_states, scale, softcap, slopes, causal, prefix_lens, documents)
     r = _bound("fused_bwd", (grad_attn_output, query_states, key_states, value_states, attn_output, lse), *mods)
