@@ -46,9 +46,9 @@ struct BwdCfg {
   static constexpr int ST = 4;
   static constexpr int OFF_A = 0;                               // two resident tiles
   static constexpr int OFF_RING = 2 * TILE_BYTES;
-  // dkv: 2 x (nlse, ndelta) of 128 rows; dq: 2 x (halves of 128 rows' delta)
+  // dkv: 2 x (nlse, ndelta) of 128 rows; dq: 2 x (halves of 128 rows' delta), then 2 x (of what it lacks)
   static constexpr int OFF_STAT = OFF_RING + ST * TILE_BYTES;
-  static constexpr int OFF_STAGE = OFF_STAT + 2 * 2 * TILE * 4;   // 2 KB for each warp of rows
+  static constexpr int OFF_STAGE = OFF_STAT + 4 * 2 * TILE * 4;   // 2 KB for each warp of rows
   static constexpr int OFF_LIST = OFF_STAGE + 8 * 2048;
   static constexpr int OFF_UNIT = OFF_LIST + 2 * kMaxList * 2;
   static constexpr int OFF_BAR = OFF_UNIT + 3 * 16;

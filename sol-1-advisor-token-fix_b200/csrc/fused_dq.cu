@@ -279,7 +279,8 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
               for (int z = 0; z < 4; ++z) w[y][e + z] = __float_as_uint(m[z]);
             }
         };
-        if (CAP && cap_small(p, fmaxf(highest_abs(w[0]), highest_abs(w[1])))) phase(std::true_type{});
+        const bool small = CAP && cap_small(p, fmaxf(highest_abs(w[0]), highest_abs(w[1])));
+        if (CAP && small) phase(std::true_type{});
         else phase(std::false_type{});
         if (i == 0) {
           // delta of the row: each half of the warps takes half of the columns
@@ -313,13 +314,64 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
           nd2 = f2(nd, nd);
           if (half == 0) {
             prm.nlse[ri] = nlse;
-            prm.ndelta[ri] = nd;
+            if (f.n > 1) prm.ndelta[ri] = nd;
           }
         }
         // masked scores are taken out of ds below
         ok = wait_for(sh.dp_full, it & 1, sh.abort_flag, 0x4302);
         if (!ok) break;
         tc_fence_after();
+        if (f.n == 1) {
+          // o in 16 bits makes delta inexact, which shows where a row sees few keys and ds is small
+          // beside it.  All of the row's weights are here, and they sum to 1, so sum(p (dp - delta))
+          // is what delta lacks.  (Rows of more tiles would need their tiles twice.)
+          uint64_t lack2 = f2(0.f, 0.f);
+          auto lacking = [&](auto small_tag) {
+            constexpr bool SMALL = decltype(small_tag)::value;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              uint32_t d[32];
+              tmem_ld32(dp + y * 32, d);
+              if (CAP) tmem_ld32(st + y * 32, w[y]);   // the weights without tanh', from the scores once more
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                float x[4], a[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) x[z] = __uint_as_float(w[y][e + z]);
+                if (CAP) {
+                  float add[4], m[4];
+#pragma unroll
+                  for (int z = 0; z < 4; ++z)
+                    add[z] = BIAS ? fmaf(-slope2, fabsf(dist0 - float(y * 32 + e + z)), nlse) : nlse;
+                  weights4<CAP, SMALL>(p, tanh_small, x, add, m);
+#pragma unroll
+                  for (int z = 0; z < 4; ++z) w[y][e + z] = __float_as_uint(m[z]);
+                }
+                f2_split(f2_mul(f2(x[0], x[1]), f2_add(f2(d[e], d[e + 1]), nd2)), a[0], a[1]);
+                f2_split(f2_mul(f2(x[2], x[3]), f2_add(f2(d[e + 2], d[e + 3]), nd2)), a[2], a[3]);
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                  if (!((see[y] >> (e + z)) & 1u)) a[z] = 0.f;
+                lack2 = f2_add(lack2, f2_add(f2(a[0], a[1]), f2(a[2], a[3])));
+              }
+            }
+          };
+          if (CAP && small) lacking(std::true_type{});
+          else lacking(std::false_type{});
+          float l0, l1;
+          f2_split(lack2, l0, l1);
+          const int r = int(warp & 3) * 32 + int(lane);
+          float* part = reinterpret_cast<float*>(sh.smem + C::OFF_STAT) + (2 + (k & 1)) * (2 * TILE);
+          part[half * TILE + r] = l0 + l1;
+          ok = meet(&sh.pair[warp & 3], met, sh.abort_flag, 0x4307);
+          if (!ok) break;
+          float nd;
+          f2_split(nd2, nd, l1);
+          if (!none) nd -= part[r] + part[TILE + r];
+          nd2 = f2(nd, nd);
+          if (half == 0) prm.ndelta[ri] = nd;
+        }
         auto gradients = [&](auto mask_tag) {
           constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll

@@ -33,11 +33,12 @@ def seen(sq, skv, b, causal=False, prefix_lens=None, documents=None):
 
 
 def attention(q, k, v, do=None, scale=None, softcap=0.0, slopes=None, causal=False, prefix_lens=None, documents=None,
-              half=None, subnormal=0.0):
+              half=None, subnormal=0.0, one_tile=False):
     """Dict of o, lse (and dq, dk, dv with do) in float64 on the CPU, and for each a bound "<name>_tol"
     on the error of a computation with fp32 scores and sums whose weights p and ds are rounded to
     the inputs' type (half: half a step; subnormal: half the smallest step of the type) before
-    they are multiplied, and whose results are rounded once."""
+    they are multiplied, and whose results are rounded once.  one_tile: delta does not depend on the
+    rounded output."""
     q, k, v = q.detach().cpu(), k.detach().cpu(), v.detach().cpu()
     half = HALF_STEP[q.dtype] if half is None else half
     if q.dtype == torch.float16:
@@ -94,7 +95,12 @@ def attention(q, k, v, do=None, scale=None, softcap=0.0, slopes=None, causal=Fal
             delta = (G * O).sum(1, keepdim=True)
             ddelta = (G.abs() * eo).sum(1, keepdim=True) + 2.0 ** -20 * (G.abs() * O.abs()).sum(1, keepdim=True)
             dS = p * (dP - delta) * slope
-            # ds before rounding: p and dp are fp32, delta takes the rounded output
+            if one_tile:
+                # delta + sum(p (dp - delta)) = sum(p dp) + delta (1 - sum(p)): what is left is p's own
+                # error on the terms and the fp32 rounding of dp
+                ddelta = (p * (2 * rel * ((dP - delta).abs() + ddelta) + 2.0 ** -18 * (G.abs() @ V.abs().t()))).sum(
+                    1, keepdim=True)
+            # ds before rounding: p and dp are fp32, delta takes the rounded output (if not one_tile)
             eS = p * slope.abs() * (ddelta + 2.0 ** -18 * (G.abs() @ V.abs().t()))
             eS = eS + (2 * rel) * (p * (dP - delta).abs()) if skv else eS
             eS = eS + half * dS.abs() + subnormal * ok

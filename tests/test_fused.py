@@ -253,6 +253,26 @@ def test_unordered_documents_and_masks_that_leave_rows_empty(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 128), (BF, 64), (HF, 64)])
+@pytest.mark.parametrize("mods", [{}, {"softcap": 15.0}, {"softcap": 1e5}, {"slopes": True}, {"softcap": 4.0, "slopes": True},
+                                  {"documents": True}])
+@pytest.mark.parametrize("sq,skv", [(8, 8), (1, 128), (100, 100), (64, 96), (256, 100)])
+def test_gradients_of_few_keys(cuda, sq, skv, mods, dtype, d):
+    """Rows of one, two, three keys, where ds is small beside what the output's rounding does to delta."""
+    q, k, v, do = _inputs(2, 4, 2, sq, skv, d, dtype, seed=sq, std=3.0)
+    mods = dict(mods, causal=True)
+    if "slopes" in mods:
+        mods["slopes"] = torch.tensor([0.5, 0.25, 0.03, 1.0], device="cuda")
+    if "documents" in mods:
+        docs = _docs(2, max(sq, skv), 5, pad=3).cuda()
+        mods["documents"] = (docs[:, -sq:].contiguous(), docs[:, -skv:].contiguous())
+    o, lse = ab.fused_attn_fwd(q, k, v, **mods)
+    r = attention(q, k, v, do, one_tile=True, **mods)
+    for g, n in zip(ab.fused_attn_bwd(do, q, k, v, o, lse, **mods), ("dq", "dk", "dv")):
+        _within(g, r[n], r[n + "_tol"], n)
+
+
+@pytest.mark.gpu
 def test_nothing_to_see(cuda):
     q, k, v, do = _inputs(1, 4, 2, 5, 0, 128, BF)
     o, lse = _check(q, k, v, do)
