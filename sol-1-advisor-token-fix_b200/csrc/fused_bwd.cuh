@@ -13,7 +13,7 @@
 // lists of tiles), and warps 0-7 turn scores into weights: TMEM lane quadrant warp % 4, columns
 // 64 * (warp / 4).. of each tile.
 //
-// What bounds them: neither the tensor cores (active 45 % of the time in dq, 51 % in dkv) nor memory (6 %
+// What bounds them: neither the tensor cores (active 45 % of the time in dq, 54 % in dkv) nor memory (6 %
 // of its rate), but the chain of a tile: scores, weights, ds, product, with 256 threads to hide
 // its waits.  4096 x 4096, 80 + 8 heads of 128, bf16: 2130 us without a mask (0.81 PFLOP/s by the five
 // products, 1.13 by the seven that are computed), 1030 us causal.  Accumulating dq by atomics

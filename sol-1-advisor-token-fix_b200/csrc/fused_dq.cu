@@ -1,6 +1,7 @@
 // fused_dq.cu — gradient of the queries (see fused_bwd.cuh).  8192 packed positions in documents of
-// about 2500, 80 + 8 heads of 128: 615 us; 48 sequences of 640, capped: 1410 us (units of three key
-// tiles, where beginning and ending a unit takes about 4 of its 11 us).
+// about 2500, 80 + 8 heads of 128: 615 us; 48 sequences of 640, capped: 1490 us (units of three key
+// tiles, where beginning and ending a unit takes about 4 of its 11 us; 75 us of it for the exact
+// delta of the units of one tile).
 #include "fused_bwd.cuh"
 #include "fused_host.h"
 
@@ -324,7 +325,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         if (f.n == 1) {
           // o in 16 bits makes delta inexact, which shows where a row sees few keys and ds is small
           // beside it.  All of the row's weights are here, and they sum to 1, so sum(p (dp - delta))
-          // is what delta lacks.  (Rows of more tiles would need their tiles twice.)
+          // is what delta lacks.  (Rows of more tiles would need their tiles twice: a fifth of the pass.)
           uint64_t lack2 = f2(0.f, 0.f);
           auto lacking = [&](auto small_tag) {
             constexpr bool SMALL = decltype(small_tag)::value;
