@@ -389,6 +389,57 @@ def test_equal_bits_and_graph_replay(cuda):
 
 
 @pytest.mark.gpu
+def test_documents_change_between_replays(cuda):
+    """A captured training pass over documents reads their numbers, prefixes and slopes at each replay."""
+    q, k, v, do = _inputs(2, 4, 2, 300, 300, 64, HF)
+    docs = [_docs(2, 300, m, seed=m, pad=p).cuda() for m, p in ((40, 0), (90, 37), (300, 5), (10, 299))]
+    pre = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 200], [70, 300], [0, 0], [5, 1])]
+    d, p, sl = docs[0].clone(), pre[0].clone(), torch.tensor([0.5, 0.1, 0.02, 0.0], device="cuda")
+    mods = dict(causal=True, documents=d, prefix_lens=p, slopes=sl)
+
+    def step():
+        o, lse = ab.fused_attn_fwd(q, k, v, **mods)
+        t, tl = ab.fused_attn_fwd(q[:, :, -1:], k, v, causal=True, documents=(d[:, -1:].contiguous(), d))
+        return (o, lse, t, tl) + ab.fused_attn_bwd(do, q, k, v, o, lse, **mods)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for x, y in zip(docs + docs[:1], pre + pre[:1]):
+        d.copy_(x)
+        p.copy_(y)
+        graph.replay()
+        held = [t.clone() for t in got]
+        assert all(torch.equal(a, b) for a, b in zip(held, step()))
+    assert ab.poll_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("docs", [False, True])
+def test_calls_close_behind_one_another(cuda, docs):
+    """Calls that take the last one's workspace at once (kernels of a call overlap, calls do not)."""
+    sets = [_inputs(1, 10, 1, 3, 2000, 128, BF, seed=s) for s in range(4)]
+    ids = [_docs(1, 2000, 50 + 400 * s, seed=s).cuda() for s in range(4)]
+
+    def step(i):
+        q, k, v, do = sets[i]
+        mods = dict(causal=True, documents=(ids[i][:, -3:].contiguous(), ids[i])) if docs else dict(causal=True)
+        o, lse = ab.fused_attn_fwd(q, k, v, **mods)
+        return (o, lse) + ab.fused_attn_bwd(do, q, k, v, o, lse, **mods)
+
+    alone = []
+    for i in range(4):
+        alone.append(step(i))
+        torch.cuda.synchronize()
+    runs = [step(i % 4) for i in range(64)]
+    for i, r in enumerate(runs):
+        assert all(torch.equal(a, b) for a, b in zip(alone[i % 4], r)), i
+    assert ab.poll_error() == 0
+
+
+@pytest.mark.gpu
 def test_layer_step_with_rope(cuda):
     """The operators as a training step calls them: rotate, attend, and back through both; the
     gradients of the unrotated queries and keys against the formulas'."""
