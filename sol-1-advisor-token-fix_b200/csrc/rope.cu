@@ -150,7 +150,8 @@ template <typename T, int VEC>
 cudaError_t launch_width(RopeParams p, int dim, bool inter, cudaStream_t stream) {
   p.pair_chunks = inter && VEC > 1 ? p.rotary_dim / VEC : p.half / VEC;
   p.chunks = p.pair_chunks + (dim - p.rotary_dim) / VEC;
-  // a block's rows keep its threads busy for a few rounds; at most 16 KB of angles
+  // A block's rows keep its threads busy for a few rounds; at most 16 KB of angles.  2 x 16001 tokens, 88
+  // heads: 238 us; 248 with 96 rows a block, 247 with 720.  12 x 467 tokens: 53; 59 from 360 rows on.
   int tpb = 192 / p.heads;
   if (tpb > kMaxTokens) tpb = kMaxTokens;
   if ((long long)tpb * p.half * 8 > 16384) tpb = 16384 / (p.half * 8);
@@ -168,6 +169,8 @@ cudaError_t launch_width(RopeParams p, int dim, bool inter, cudaStream_t stream)
 }
 
 // align: bytes that every row's address is a multiple of (16, 8 or less).
+// The widest pieces that fit: 2 x 16001 tokens take 238 us in pieces of 16 bytes, 308 of 8, 516 element by
+// element; heads of 80 with 40 rotated take 59 us in pieces of 8 bytes, 130 element by element.
 template <typename T>
 cudaError_t launch_rope(const RopeParams& p, int dim, bool inter, int align, cudaStream_t stream) {
   constexpr int V16 = 16 / int(sizeof(T)), V8 = V16 / 2;
