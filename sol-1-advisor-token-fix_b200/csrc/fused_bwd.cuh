@@ -46,7 +46,7 @@ struct BwdCfg {
   static constexpr int ST = 4;
   static constexpr int OFF_A = 0;                               // two resident tiles
   static constexpr int OFF_RING = 2 * TILE_BYTES;
-  // dkv: 2 x (nlse, ndelta) of 128 rows; dq: 2 x (halves of 128 rows' delta), then 2 x (of what it lacks)
+  // dkv: 2 x (nlse, ndelta) of 128 rows; dq: 2 x (halves of 128 rows' sums of p dp and p, or of delta)
   static constexpr int OFF_STAT = OFF_RING + ST * TILE_BYTES;
   static constexpr int OFF_STAGE = OFF_STAT + 4 * 2 * TILE * 4;   // 2 KB for each warp of rows
   static constexpr int OFF_LIST = OFF_STAGE + 8 * 2048;

@@ -1,7 +1,6 @@
 // fused_dq.cu — gradient of the queries (see fused_bwd.cuh).  8192 packed positions in documents of
-// about 2500, 80 + 8 heads of 128: 615 us; 48 sequences of 640, capped: 1490 us (units of three key
-// tiles, where beginning and ending a unit takes about 4 of its 11 us; 75 us of it for the exact
-// delta of the units of one tile).
+// about 2500, 80 + 8 heads of 128: 615 us; 48 sequences of 640, capped: 1340 us (units of three key
+// tiles, where beginning and ending a unit takes about 4 of its 10 us).
 #include "fused_bwd.cuh"
 #include "fused_host.h"
 
@@ -216,11 +215,13 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
       // part together (a lane reading its own row's would touch 32 lines a load).  Used, like
       // lse, only after the wait for the first scores.
       uint4 ov[LR];
+      if (f.n > 1) {
 #pragma unroll
-      for (int c = 0; c < LR; ++c) {
-        const int r = min(f.r1, f.r0 + int(warp & 3) * 32 + c * (32 / LR) + int(lane) / LR);
-        ov[c] = __ldg(reinterpret_cast<const uint4*>(prm.o + (((size_t)f.b * p.sq + r) * p.H + f.h) * (D * 2) + half * D) +
-                      int(lane) % LR);
+        for (int c = 0; c < LR; ++c) {
+          const int r = min(f.r1, f.r0 + int(warp & 3) * 32 + c * (32 / LR) + int(lane) / LR);
+          ov[c] = __ldg(reinterpret_cast<const uint4*>(prm.o + (((size_t)f.b * p.sq + r) * p.H + f.h) * (D * 2) + half * D) +
+                        int(lane) % LR);
+        }
       }
       bool none = false;       // the row sees nothing
       float nlse = 0.f;
@@ -281,14 +282,16 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
             }
         };
         const bool small = CAP && cap_small(p, fmaxf(highest_abs(w[0]), highest_abs(w[1])));
-        if (CAP && small) phase(std::true_type{});
-        else phase(std::false_type{});
-        if (i == 0) {
+        if (!CAP || f.n > 1) {   // (below otherwise)
+          if (CAP && small) phase(std::true_type{});
+          else phase(std::false_type{});
+        }
+        if (i == 0 && f.n > 1) {
           // delta of the row: each half of the warps takes half of the columns
           ok = wait_for(sh.res_full, di & 1, sh.abort_flag, 0x4305);
           if (!ok) break;
           const int r = int(warp & 3) * 32 + int(lane);
-          float* part = reinterpret_cast<float*>(sh.smem + C::OFF_STAT) + (k & 1) * (2 * TILE);
+          float* part = reinterpret_cast<float*>(sh.smem + C::OFF_STAT) + (k & 1) * (4 * TILE);
 #pragma unroll
           for (int c = 0; c < LR; ++c) {
             const int rr = int(warp & 3) * 32 + c * (32 / LR) + int(lane) / LR, cg = half * LR + int(lane) % LR;
@@ -315,7 +318,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
           nd2 = f2(nd, nd);
           if (half == 0) {
             prm.nlse[ri] = nlse;
-            if (f.n > 1) prm.ndelta[ri] = nd;
+            prm.ndelta[ri] = nd;
           }
         }
         // masked scores are taken out of ds below
@@ -323,21 +326,20 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         if (!ok) break;
         tc_fence_after();
         if (f.n == 1) {
-          // o in 16 bits makes delta inexact, which shows where a row sees few keys and ds is small
-          // beside it.  All of the row's weights are here, and they sum to 1, so sum(p (dp - delta))
-          // is what delta lacks.  (Rows of more tiles would need their tiles twice: a fifth of the pass.)
-          uint64_t lack2 = f2(0.f, 0.f);
-          auto lacking = [&](auto small_tag) {
+          // All of the row's weights are here: delta = sum(p dp) / sum(p), without o, whose 16 bits cost
+          // delta most where a row sees few keys and ds is small beside it.  (Rows of more tiles would
+          // need their tiles twice: a fifth of the pass.)
+          uint64_t pd2 = f2(0.f, 0.f), ps2 = f2(0.f, 0.f);
+          auto whole = [&](auto small_tag) {
             constexpr bool SMALL = decltype(small_tag)::value;
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               uint32_t d[32];
               tmem_ld32(dp + y * 32, d);
-              if (CAP) tmem_ld32(st + y * 32, w[y]);   // the weights without tanh', from the scores once more
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; e += 4) {
-                float x[4], a[4];
+                float x[4];
 #pragma unroll
                 for (int z = 0; z < 4; ++z) x[z] = __uint_as_float(w[y][e + z]);
                 if (CAP) {
@@ -349,29 +351,38 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
 #pragma unroll
                   for (int z = 0; z < 4; ++z) w[y][e + z] = __float_as_uint(m[z]);
                 }
-                f2_split(f2_mul(f2(x[0], x[1]), f2_add(f2(d[e], d[e + 1]), nd2)), a[0], a[1]);
-                f2_split(f2_mul(f2(x[2], x[3]), f2_add(f2(d[e + 2], d[e + 3]), nd2)), a[2], a[3]);
 #pragma unroll
                 for (int z = 0; z < 4; ++z)
-                  if (!((see[y] >> (e + z)) & 1u)) a[z] = 0.f;
-                lack2 = f2_add(lack2, f2_add(f2(a[0], a[1]), f2(a[2], a[3])));
+                  if (!((see[y] >> (e + z)) & 1u)) {
+                    x[z] = 0.f;
+                    d[e + z] = 0u;
+                  }
+#pragma unroll
+                for (int z = 0; z < 4; z += 2) {
+                  pd2 = f2_fma(f2(x[z], x[z + 1]), f2(d[e + z], d[e + z + 1]), pd2);
+                  ps2 = f2_add(ps2, f2(x[z], x[z + 1]));
+                }
               }
             }
           };
-          if (CAP && small) lacking(std::true_type{});
-          else lacking(std::false_type{});
-          float l0, l1;
-          f2_split(lack2, l0, l1);
+          if (CAP && small) whole(std::true_type{});
+          else whole(std::false_type{});
+          float a0, a1, b0, b1;
+          f2_split(pd2, a0, a1);
+          f2_split(ps2, b0, b1);
           const int r = int(warp & 3) * 32 + int(lane);
-          float* part = reinterpret_cast<float*>(sh.smem + C::OFF_STAT) + (2 + (k & 1)) * (2 * TILE);
-          part[half * TILE + r] = l0 + l1;
+          float2* part = reinterpret_cast<float2*>(sh.smem + C::OFF_STAT) + (k & 1) * (2 * TILE);
+          part[half * TILE + r] = make_float2(a0 + a1, b0 + b1);
+          if (lane == 0) mbar_arrive(sh.res_empty);
           ok = meet(&sh.pair[warp & 3], met, sh.abort_flag, 0x4307);
           if (!ok) break;
-          float nd;
-          f2_split(nd2, nd, l1);
-          if (!none) nd -= part[r] + part[TILE + r];
+          const float2 u = part[r], v = part[TILE + r];
+          const float nd = none ? 0.f : -(u.x + v.x) / (u.y + v.y);
           nd2 = f2(nd, nd);
-          if (half == 0) prm.ndelta[ri] = nd;
+          if (half == 0) {
+            prm.nlse[ri] = nlse;
+            prm.ndelta[ri] = nd;
+          }
         }
         auto gradients = [&](auto mask_tag) {
           constexpr bool MASK = decltype(mask_tag)::value;

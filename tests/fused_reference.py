@@ -96,9 +96,9 @@ def attention(q, k, v, do=None, scale=None, softcap=0.0, slopes=None, causal=Fal
             ddelta = (G.abs() * eo).sum(1, keepdim=True) + 2.0 ** -20 * (G.abs() * O.abs()).sum(1, keepdim=True)
             dS = p * (dP - delta) * slope
             if one_tile:
-                # delta + sum(p (dp - delta)) = sum(p dp) + delta (1 - sum(p)): what is left is p's own
-                # error on the terms and the fp32 rounding of dp
-                ddelta = (p * (2 * rel * ((dP - delta).abs() + ddelta) + 2.0 ** -18 * (G.abs() @ V.abs().t()))).sum(
+                # sum(p dp) / sum(p): what p's common error does cancels, each p's own acts on dp - delta, and
+                # dp has its fp32 rounding
+                ddelta = (p * (2 * rel * (dP - delta).abs() + 2.0 ** -18 * (G.abs() @ V.abs().t()))).sum(
                     1, keepdim=True)
             # ds before rounding: p and dp are fp32, delta takes the rounded output (if not one_tile)
             eS = p * slope.abs() * (ddelta + 2.0 ** -18 * (G.abs() @ V.abs().t()))
