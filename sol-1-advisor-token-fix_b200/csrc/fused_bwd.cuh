@@ -8,7 +8,8 @@
 //        transposed scores (keys are rows), so p^T and ds^T are A operands in TMEM and the sum over
 //        the group's heads happens in the accumulators.
 //   dq:  one query tile of one head a CTA, streams the key tiles.  It runs first and leaves the
-//        rows' statistics (delta from the resident do and a read of o) to dkv.
+//        rows' statistics to dkv (delta from the resident do and a read of o; from the weights where
+//        the rows have one key tile).
 // In both, warp 8 is the TMA producer, warp 9 issues tcgen05, warp 10 fetches units (and makes their
 // lists of tiles), and warps 0-7 turn scores into weights: TMEM lane quadrant warp % 4, columns
 // 64 * (warp / 4).. of each tile.
