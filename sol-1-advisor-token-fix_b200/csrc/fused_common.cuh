@@ -378,8 +378,9 @@ __device__ __forceinline__ float highest_abs(const uint32_t (&x)[32]) {
   for (int e = 0; e < 32; e += 2) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1]))));
   return big;
 }
-__device__ __forceinline__ bool cap_small(const Params& p, float big) {
-  return __all_sync(0xffffffffu, big * p.cap_u <= kTanhSmall);
+// pad: this lane's row (or key) belongs to no document, so what it holds has no part in the choice.
+__device__ __forceinline__ bool cap_small(const Params& p, float big, bool pad) {
+  return __all_sync(0xffffffffu, pad || big * p.cap_u <= kTanhSmall);
 }
 // One raw score to softcap tanh(scale x / softcap) log2(e).  (Through the reciprocal alone a high
 // cap would leave nothing of a low score.)

@@ -291,7 +291,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
             if (lane == 0) mbar_arrive(&sh.p_ready[y]);
           }
         };
-        const bool small = CAP && cap_small(p, fmaxf(highest_abs(w[0]), highest_abs(w[1])));
+        const bool small = CAP && cap_small(p, fmaxf(highest_abs(w[0]), highest_abs(w[1])), p.has_docs && kd < 0);
         if (__builtin_expect(masked, 0)) {
           if (CAP && small) phase(std::true_type{}, std::true_type{});
           else phase(std::true_type{}, std::false_type{});

@@ -281,7 +281,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
               for (int z = 0; z < 4; ++z) w[y][e + z] = __float_as_uint(m[z]);
             }
         };
-        const bool small = CAP && cap_small(p, fmaxf(highest_abs(w[0]), highest_abs(w[1])));
+        const bool small = CAP && cap_small(p, fmaxf(highest_abs(w[0]), highest_abs(w[1])), p.has_docs && qd < 0);
         if (!CAP || f.n > 1) {   // (below otherwise)
           if (CAP && small) phase(std::true_type{});
           else phase(std::false_type{});

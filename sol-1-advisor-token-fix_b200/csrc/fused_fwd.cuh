@@ -262,6 +262,15 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
       for (uint32_t k = 0; next_unit(sched, k, u, abort_flag, 0x2200); ++k) {
         const FwdUnit f = fwd_unit(prm, u);
         const uint16_t* list = lists + (k & 1) * kMaxList;
+        // clears the padding of a key or value tile (the unit's i-th, ring index r).  Values: a NaN there times
+        // a weight of 0 is NaN.  Keys: only below a cap, where four scores share a reciprocal and a warp
+        // its choice of the tanh's form; their scores are hidden after it.
+        auto scrub = [&](uint32_t r, int i) {
+          if (p.has_docs && (list[i] & kEntScrub)) {
+            const int j0 = (f.t0 + int(list[i] & kEntTile)) * TILE;
+            scrub_rows<D>(stage(r), p.kdoc + (size_t)f.b * p.skv + j0, p.skv - j0, lane);
+          }
+        };
         if (DUO && f.n > 0) {
           if (!wait_for(q_full, qi & 1, abort_flag, 0x2201)) break;
           ++qi;
@@ -269,6 +278,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           auto scores = [&](uint32_t r, int j) {
             if (!full(r, 0x2202)) return false;
             if (j < f.n) {
+              if (CAP) scrub(r, j);
               tc_fence_after();
               mma_kk<D>(one, tmem + (j & 1) * TILE, desc_k(qs), desc_k(stage(r)), id_s);
               commit1(one, &s_full[j & 1]);
@@ -283,10 +293,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
               const uint32_t r = si + 2 + t;
               if (!(ok = full(r, 0x2203))) break;
               if (j < f.n) {
-                if (p.has_docs && (list[j] & kEntScrub)) {
-                  const int j0 = (f.t0 + int(list[j] & kEntTile)) * TILE;
-                  scrub_rows<D>(stage(r), p.kdoc + (size_t)f.b * p.skv + j0, p.skv - j0, lane);
-                }
+                scrub(r, j);
                 const uint32_t t_s = tmem + t * TILE, t_o = tmem + 2 * TILE + t * D;
                 if (!(ok = wait_for(&p_ready[2 * t], cnt[t] & 1, abort_flag, 0x2205))) break;
                 tc_fence_after();
@@ -306,6 +313,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
         if (!DUO && f.n > 0) {
           if (!wait_for(q_full, qi & 1, abort_flag, 0x2201) || !full(si, 0x2202)) break;
           ++qi;
+          if (CAP) scrub(si, 0);
           tc_fence_after();
           for (int t = 0; t < f.nt; ++t) {
             mma_kk<D>(one, tmem + t * TILE, desc_k(qs + t * C::TILE_BYTES), desc_k(stage(si)), id_s);
@@ -318,11 +326,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             const uint32_t vi = si + 1, kn = si + 2;
             const bool more = i + 1 < f.n;
             if (!(ok = full(vi, 0x2203))) break;
-            if (p.has_docs && (list[i] & kEntScrub)) {
-              const int j0 = (f.t0 + int(list[i] & kEntTile)) * TILE;
-              scrub_rows<D>(stage(vi), p.kdoc + (size_t)f.b * p.skv + j0, p.skv - j0, lane);
-            }
+            scrub(vi, i);
             if (more && !(ok = full(kn, 0x2204))) break;
+            if (CAP && more) scrub(kn, i + 1);
             for (int t = 0; t < f.nt && ok; ++t) {
               const uint32_t t_s = tmem + t * TILE, t_o = tmem + 2 * TILE + t * D;
               ok = wait_for(&p_ready[2 * t], (cnt[t] + i) & 1, abort_flag, 0x2205);
@@ -466,7 +472,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
           // 32 scores from column 32 g on: cap, bias, mask (log2 units / c, -inf where not seen)
           auto modify = [&](uint32_t (&x)[32], int g) {
             if (CAP) {
-              if (cap_small(p, highest_abs(x))) cap32<true>(p, tanh_small, x);
+              if (cap_small(p, highest_abs(x), p.has_docs && qd < 0)) cap32<true>(p, tanh_small, x);
               else cap32<false>(p, tanh_small, x);
             }
             if (BIAS) {
@@ -514,7 +520,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             m = fmaxf(fmaxf(highest(x[0]), highest(x[1])), fmaxf(highest(x[2]), highest(x[3])));
             if (CAP)
               small = cap_small(p, fmaxf(fmaxf(highest_abs(x[0]), highest_abs(x[1])),
-                                         fmaxf(highest_abs(x[2]), highest_abs(x[3]))));
+                                         fmaxf(highest_abs(x[2]), highest_abs(x[3]))), false);   // not masked: no padding
             if (CAP) m = cap1(p, tanh_small, m);   // the tanh grows with its argument
           } else if constexpr (CAP || BIAS) {
             m = -INFINITY;

@@ -1,0 +1,70 @@
+"""Fused attention where a result could leak or vanish: what padding holds, and numbers that are not
+finite under a cap."""
+import math
+
+import pytest
+import torch
+
+import attn_bwd_b200 as ab
+from fused_reference import attention
+from test_fused import _inputs, _within
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _mods(mod, heads, bs, skv):
+    kw = {}
+    if "cap" in mod:
+        kw["softcap"] = 5.0
+    if "slopes" in mod:
+        kw["slopes"] = torch.tensor([0.5, 0.25, 0.0, 0.03, 0.125, 1.0][:heads], device="cuda")
+    if "prefix" in mod:
+        kw["prefix_lens"] = torch.tensor([skv // 2, 3, 0, skv][:bs], dtype=torch.int32, device="cuda")
+    if mod != "full":
+        kw["causal"] = True
+    return kw
+
+
+# units of one tile, of several tiles, of packed rows, of split keys, and of two chains over the keys
+PADDED = [(2, 4, 2, 300, 300), (2, 4, 2, 100, 100), (1, 6, 1, 70, 460), (2, 4, 2, 1, 2000), (2, 6, 2, 4, 1900), (3, 2, 2, 130, 270)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 128), (BF, 64), (HF, 64)])
+@pytest.mark.parametrize("mod", ["full", "causal", "cap", "slopes", "cap+slopes", "cap+prefix", "slopes+prefix"])
+@pytest.mark.parametrize("bs,heads,kv,sq,skv", PADDED)
+def test_padding_changes_no_bit(cuda, bs, heads, kv, sq, skv, mod, dtype, d):
+    """Padding behind the last document, between documents and inside one, in queries and keys: whatever
+    it holds, the results are the same bits, and those that the formulas give."""
+    q, k, v, do = _inputs(bs, heads, kv, sq, skv, d, dtype, seed=skv, std=3.0)
+    g = torch.Generator().manual_seed(skv)
+    kd = torch.arange(skv, dtype=torch.int32).div(max(1, skv // 3), rounding_mode="floor").repeat(bs, 1)
+    kd[torch.rand(bs, skv, generator=g) < 0.1] = -1
+    kd[:, skv - 3 - skv // 16:skv - sq if sq < 3 else skv] = -1
+    qd = kd[:, skv - sq:].clone()
+    if sq < 3:
+        qd[:] = 2   # a token that its cache's padding does not touch
+    kw = dict(_mods(mod, heads, bs, skv), documents=(qd.cuda(), kd.cuda()))
+    qp, kp = (qd < 0).cuda(), (kd < 0).cuda()
+    assert kp.any()
+
+    def step(fill):
+        for t, p in ((q.transpose(1, 2), qp), (k.transpose(1, 2), kp), (v.transpose(1, 2), kp), (do, qp)):
+            t[p] = fill
+        o, lse = ab.fused_attn_fwd(q, k, v, **kw)
+        return (o, lse) + ab.fused_attn_bwd(do, q, k, v, o, lse, **kw)
+
+    want = step(0.0)
+    r = attention(q, k, v, do, **kw)
+    # An exponential below 2^-126 may be taken as 0 (steep slopes reach that): p is then off by up to 2^-126, ds
+    # by that times |dp - delta| <= 2 max sum|do| max|v| = a, and dq and dk by a times the sums of |k| and |q|
+    # times the scale.  The reference's bound counts this for the rounding of ds, not for p.
+    a = 2.0 ** -126 * 2 * float(do.abs().double().sum(-1).max()) * float(v.abs().max()) / math.sqrt(d)
+    r["dq_tol"] = r["dq_tol"] + a * float(k.abs().double().sum(2).max())
+    r["dk_tol"] = r["dk_tol"] + a * float(q.abs().double().sum((1, 2)).max())
+    for x, n in zip(want, ("o", "lse", "dq", "dk", "dv")):
+        _within(x, r[n], r[n + "_tol"], n)
+    for fill in (3.0, 6e4, math.inf, math.nan):
+        for x, y, n in zip(step(fill), want, ("o", "lse", "dq", "dk", "dv")):
+            assert torch.equal(x, y), f"{n}, padding of {fill}"
+    assert ab.poll_error() == 0
