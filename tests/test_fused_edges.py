@@ -68,3 +68,43 @@ def test_padding_changes_no_bit(cuda, bs, heads, kv, sq, skv, mod, dtype, d):
         for x, y, n in zip(step(fill), want, ("o", "lse", "dq", "dk", "dv")):
             assert torch.equal(x, y), f"{n}, padding of {fill}"
     assert ab.poll_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 128), (BF, 64), (HF, 64)])
+@pytest.mark.parametrize("mod", ["cap", "cap+slopes", "full"])
+@pytest.mark.parametrize("std", [0.01, 8.0])   # scores far below the cap, and at it
+@pytest.mark.parametrize("bs,heads,kv,sq,skv", [(1, 2, 1, 300, 300), (1, 2, 2, 100, 100), (1, 4, 1, 3, 700), (2, 6, 2, 60, 300)])
+def test_nan_under_a_cap_stays_nan(cuda, bs, heads, kv, sq, skv, std, mod, dtype, d):
+    """A NaN query: its row is NaN, output, statistic and gradient, and so are the gradients of the keys
+    that it sees; other rows are what they are without it.  A NaN key: every row that sees it is NaN."""
+    q, k, v, do = _inputs(bs, heads, kv, sq, skv, d, dtype, seed=7, std=std)
+    kw = dict(_mods(mod, heads, bs, skv), softcap=2.0)
+    row, h = sq // 2, heads - 1
+    r = attention(q, k, v, do, **kw)
+    bad = q.clone()
+    bad[0, h, row, d // 3] = math.nan
+    o, lse = ab.fused_attn_fwd(bad, k, v, **kw)
+    assert torch.isnan(o[0, row, h]).all() and torch.isnan(lse[0, h, row])
+    rest = torch.ones(bs, sq, heads, dtype=torch.bool)
+    rest[0, row, h] = False
+    _within(o.cpu()[rest], r["o"][rest], r["o_tol"][rest], "o")
+    rt = rest.transpose(1, 2)
+    _within(lse.cpu()[rt], r["lse"][rt], r["lse_tol"][rt], "lse")
+    dq, dk, dv = ab.fused_attn_bwd(do, bad, k, v, o, lse, **kw)
+    assert torch.isnan(dq[0, h, row]).all()
+    last = skv if mod == "full" else skv - sq + row + 1   # keys that the row sees
+    assert torch.isnan(dv[0, -1, :last]).all() and torch.isnan(dk[0, -1, :last]).all()
+    _within(dq.cpu()[rt], r["dq"][rt], r["dq_tol"][rt], "dq")
+    key = skv - sq + sq // 3
+    bad = k.clone()
+    bad[0, 0, key, 1] = math.nan
+    o, lse = ab.fused_attn_fwd(q, bad, v, **kw)
+    first = 0 if mod == "full" else sq // 3   # rows that see the key
+    grp = heads // kv
+    assert torch.isnan(o[0, first:, :grp]).all() and torch.isnan(lse[0, :grp, first:]).all()
+    dq, dk, dv = ab.fused_attn_bwd(do, q, bad, v, o, lse, **kw)
+    assert torch.isnan(dq[0, :grp, first:]).all() and torch.isnan(dv[0, 0, key]).all() and torch.isnan(dk[0, 0, key]).all()
+    if kv > 1:   # the other groups
+        assert torch.isfinite(o[0, :, grp:]).all() and torch.isfinite(dv[0, 1:]).all()
+    assert ab.poll_error() == 0
