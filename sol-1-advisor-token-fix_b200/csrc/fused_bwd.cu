@@ -104,6 +104,8 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
   };
   set(f.dks, a->dk_stride, a->kv_heads, a->seq_kv);
   set(f.dvs, a->dv_stride, a->kv_heads, a->seq_kv);
+  f.wide = wide_rows(dk, a->dk_stride, a->bs, a->kv_heads, a->seq_kv) &&
+           wide_rows(dv, a->dv_stride, a->bs, a->kv_heads, a->seq_kv);
   const bool f16 = a->dtype == ATTN_BWD_DT_FP16;
   CUtensorMap mq, md, mk, mv;
   std::memset(&mk, 0, sizeof(mk));

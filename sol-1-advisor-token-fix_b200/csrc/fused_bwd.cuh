@@ -38,6 +38,7 @@ struct BwdParams {
   float* ndelta;         // [bs * H, sq_pad]: -sum(do * o); dq writes both, dkv reads them
   void *dk, *dv;
   long long dks[3], dvs[3];   // element strides: batch, head, position
+  int wide;                   // rows of dk and dv start at multiples of 32 bytes
   float* part;           // dkv, splits > 1: [split][bs * Hkv * skv][2][D], dk first
 };
 

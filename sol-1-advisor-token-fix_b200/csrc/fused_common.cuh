@@ -259,14 +259,21 @@ __device__ __forceinline__ void unit_done(const Scheduler& s, uint32_t k) {
 
 // ---- results: one row a lane, 32 values as 16 pairs, in two stores of 32 bytes (a whole sector
 // each).  For rows that are no box of a tensor map: (position, head) rows, and keys' gradients in the
-// caller's strides.
-__device__ __forceinline__ void write_row(const uint32_t (&w)[16], uint8_t* dst) {
+// caller's strides.  A store's address is a multiple of its width, and results need only 16-byte rows: wide
+// (see wide_rows) says that all of them are multiples of 32.
+__device__ __forceinline__ void write_row(const uint32_t (&w)[16], uint8_t* dst, bool wide) {
+  if (__builtin_expect(wide, 1)) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + h * 32), "r"(w[8 * h]),
-                 "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]), "r"(w[8 * h + 4]), "r"(w[8 * h + 5]),
-                 "r"(w[8 * h + 6]), "r"(w[8 * h + 7])
-                 : "memory");
+    for (int h = 0; h < 2; ++h)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + h * 32), "r"(w[8 * h]),
+                   "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]), "r"(w[8 * h + 4]), "r"(w[8 * h + 5]),
+                   "r"(w[8 * h + 6]), "r"(w[8 * h + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+      *reinterpret_cast<uint4*>(dst + h * 16) = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+  }
 }
 
 // The same through the warp's 2 KB of shared memory and one tensor store of 32 rows x 64 bytes (a map

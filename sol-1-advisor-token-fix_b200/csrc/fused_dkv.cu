@@ -375,7 +375,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             o[e] = pack2<F16>(__uint_as_float(v[2 * e]) * fac, __uint_as_float(v[2 * e + 1]) * fac);
-          if (j < p.skv) write_row(o, out + x * 64);
+          if (j < p.skv) write_row(o, out + x * 64, prm.wide != 0);
         }
       }
       tc_fence_before();   // the next unit's first products overwrite the accumulators

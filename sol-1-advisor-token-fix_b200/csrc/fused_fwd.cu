@@ -84,6 +84,8 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
   Params& p = f.c;
   p.err = dev.err;
   f.o = o;
+  const int64_t os[3] = {(int64_t)p.sq * p.H * a->head_dim, a->head_dim, (int64_t)p.H * a->head_dim};
+  f.wide = wide_rows(o, os, p.bs, p.H, p.sq);
   f.lse = lse;
   if (f.blocks_q > (1 << 30) / f.head_slots || f.cta_splits > 65535) return ATTN_BWD_EINVAL;
   const int64_t need = range_bytes(p) + part_rows(p) * (a->head_dim + 1) * 4;
@@ -96,7 +98,6 @@ extern "C" int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* a, const void* q,
   }
   const bool f16 = a->dtype == ATTN_BWD_DT_FP16;
   FwdMaps m;
-  const int64_t os[3] = {(int64_t)p.sq * p.H * a->head_dim, a->head_dim, (int64_t)p.H * a->head_dim};
   if (!map_bhsd(&m.q, q, a->q_stride, p.bs, p.H, p.sq, a->head_dim, f16, f.pos_per_tile, f.packed ? p.G : 1, false) ||
       !map_bhsd(&m.o, o, os, p.bs, p.H, p.sq, a->head_dim, f16, 32, 1, false, true))
     return ATTN_BWD_ETMAP;

@@ -47,6 +47,7 @@ struct FwdParams {
   int duo;             // all rows of a unit in one tile: two chains over alternate key tiles
   int pair_heads;      // unpacked: the two tiles are two heads of one group, else 256 positions
   int blocks_q;        // position blocks per (batch, head slot)
+  int wide;            // rows of o start at multiples of 32 bytes
   int head_slots;      // units along the heads: kv heads, head pairs or heads
   FastDiv div_slots;
   void* o;             // [bs, sq, H, D]
@@ -675,7 +676,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             for (int e = 0; e < 16; ++e)
               w[e] = empty ? 0u : pack2<F16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
             if (prm.packed) {   // (position, head) rows are no box
-              if (valid) write_row(w, dst + x * 64);
+              if (valid) write_row(w, dst + x * 64, prm.wide != 0);
             } else {
               store_rows(stage, &tm_o, w, x * 32, head, pos - int(lane), f.b, lane);
             }

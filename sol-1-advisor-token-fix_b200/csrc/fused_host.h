@@ -21,6 +21,14 @@ inline bool tma_strides_ok(const int64_t* st, int bs, int heads, int seq) {
   return true;
 }
 
+// Whether every row of such a tensor starts at a multiple of 32 bytes (16 elements).
+inline bool wide_rows(const void* x, const int64_t* st, int bs, int heads, int seq) {
+  const int n[3] = {bs, heads, seq};
+  bool ok = (reinterpret_cast<uintptr_t>(x) & 31u) == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (n[i] <= 1 || st[i] % 16 == 0);
+  return ok;
+}
+
 inline int check_args(const attn_bwd_fused_t* a) {
   if (!a || a->bs < 0 || a->seq_q < 0 || a->seq_kv < 0 || a->heads < 1 || a->kv_heads < 1 ||
       a->heads % a->kv_heads || a->bs > 65535 || a->heads > 65535 || a->seq_q >= (1 << 30) || a->seq_kv >= (1 << 30))

@@ -1,0 +1,79 @@
+"""The C entry points of the fused attention with layouts that the Python calls never choose."""
+import ctypes
+
+import pytest
+import torch
+
+import attn_bwd_b200 as ab
+from attn_bwd_b200 import _lib
+from test_fused import _inputs
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _place(shape, strides, offset, dtype):
+    """A tensor of that shape and those strides (in elements) in a buffer of sevens, from an element on."""
+    n = offset + sum((s - 1) * st for s, st in zip(shape, strides)) + 64
+    buf = torch.full((n,), 7.0, dtype=dtype, device="cuda")
+    assert buf.data_ptr() % 256 == 0
+    return buf, buf.as_strided(shape, strides, offset)
+
+
+def _only_there(buf, view):
+    """Nothing but the view's elements was written."""
+    seen = torch.zeros(buf.shape, dtype=torch.bool, device="cuda")
+    seen.as_strided(view.shape, view.stride(), view.storage_offset()).fill_(True)
+    return bool((buf[~seen] == 7).all())
+
+
+def _ptr(t):
+    return t.data_ptr()
+
+
+def _workspace(args, backward):
+    n = _lib.load().attn_bwd_b200_fused_workspace(ctypes.byref(args), backward)
+    assert n >= 0
+    return torch.empty(max(n, 1), dtype=torch.uint8, device="cuda"), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64)])
+@pytest.mark.parametrize("heads,kv,sq", [(6, 2, 20), (4, 4, 150)])   # rows of a group in one tile, and rows of a head
+@pytest.mark.parametrize("offset", [0, 8, 16, 24])
+def test_outputs_at_any_16_bytes(cuda, offset, heads, kv, sq, dtype, d):
+    q, k, v, _ = _inputs(2, heads, kv, sq, sq, d, dtype)
+    want, wl = ab.fused_attn_fwd(q, k, v, causal=True)
+    c = ab.fused._Call(q, k, v, None, 0.0, None, True, None, None)
+    buf, o = _place(want.shape, want.stride(), offset, dtype)
+    lse = torch.empty_like(wl)
+    ws, n = _workspace(c.args, 0)
+    _lib.call("attn_bwd_b200_fused_fwd", ctypes.byref(c.args), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(ws), n,
+              torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(o, want) and torch.equal(lse, wl) and _only_there(buf, o)
+    assert ab.poll_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64)])
+@pytest.mark.parametrize("bs,kv", [(20, 4), (1, 2)])   # key tiles that write their results, and parts that are joined
+@pytest.mark.parametrize("offset,row,gap", [(8, 0, 0), (0, 8, 0), (0, 0, 8), (16, 16, 16), (24, 24, 40)])
+def test_gradients_at_any_16_bytes(cuda, offset, row, gap, bs, kv, dtype, d):
+    """Gradients whose rows lie d + row elements apart and whose heads leave a gap."""
+    q, k, v, do = _inputs(bs, 2 * kv, kv, 90, 130, d, dtype)
+    o, lse = ab.fused_attn_fwd(q, k, v, causal=True)
+    want = ab.fused_attn_bwd(do, q, k, v, o, lse, causal=True)
+    c = ab.fused._Call(q, k, v, None, 0.0, None, True, None, None)
+    bufs, grads = [], []
+    for t, dst in zip(want, (c.args.dq_stride, c.args.dk_stride, c.args.dv_stride)):
+        b, h, s, _ = t.shape
+        head = s * (d + row) + gap
+        buf, g = _place(t.shape, (h * head + gap, head, d + row, 1), offset, dtype)
+        dst[:] = g.stride()[:3]
+        bufs.append(buf)
+        grads.append(g)
+    ws, n = _workspace(c.args, 1)
+    _lib.call("attn_bwd_b200_fused_bwd", ctypes.byref(c.args), _ptr(do), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse),
+              *[_ptr(g) for g in grads], _ptr(ws), n, torch.cuda.current_stream().cuda_stream)
+    for buf, g, w in zip(bufs, grads, want):
+        assert torch.equal(g, w) and _only_there(buf, g)
+    assert ab.poll_error() == 0
