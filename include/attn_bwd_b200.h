@@ -142,7 +142,7 @@ enum { ATTN_BWD_DT_BF16 = 0, ATTN_BWD_DT_FP16 = 1, ATTN_BWD_DT_FP32 = 2 };
  *   (a, b) -> factor * (a cos t - b sin t, b cos t + a sin t),   t = 2 pi position * turns / 2^64,
  * pair n being (n, n + rotary_dim/2), or (2n, 2n+1) with `interleaved`; the rest of the head
  * is copied.  `inverse` negates t: with the same factor that is the gradient of the call.
- * turns[n] is the frequency as a 64-bit fixed-point fraction of a turn (two's complement), so
+ * turns [rotary_dim/2]: turns[n] is the frequency as a 64-bit fixed-point fraction of a turn (two's complement), so
  * position * turns wraps exactly and far positions lose nothing.  Strides are in elements,
  * in the order batch, head, position; the head's own elements are contiguous.  An output may
  * be its own input (same strides).  position_stride is the positions' batch stride (0: one

@@ -14,8 +14,8 @@ _TYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_FP16, torch.float
 class RopeTable:
     """Frequencies of a rotation, made once by :func:`rope_table` and kept by the caller.
 
-    ``turns`` [rotary_dim / 2] int64 on the GPU: each frequency as a 64-bit fixed-point fraction
-    of a turn a position; ``factor`` multiplies the rotated part of a head."""
+    ``turns`` [rotary_dim / 2] int64 on the GPU, contiguous: each frequency as a 64-bit fixed-point
+    fraction of a turn a position; ``factor`` multiplies the rotated part of a head."""
 
     __slots__ = ("turns", "rotary_dim", "factor")
 
@@ -93,6 +93,13 @@ def _rotate(q, k, position_ids, table, interleaved, inverse, out):
             return r
     if not isinstance(table, RopeTable):
         raise TypeError(f"table: expected a RopeTable (rope_table(...)), got {type(table).__name__}")
+    turns = table.turns
+    if not isinstance(turns, torch.Tensor) or turns.dtype != torch.int64:
+        raise TypeError("table: turns must be an int64 tensor")
+    if not isinstance(table.rotary_dim, int) or tuple(turns.shape) != (table.rotary_dim // 2,) or table.rotary_dim % 2:
+        raise ValueError(f"table: turns of {tuple(turns.shape)} do not belong to {table.rotary_dim} rotated elements")
+    if not turns.is_contiguous():
+        raise ValueError("table: turns must be contiguous")
     names = ("query", "key")
     xs = [x for x in (q, k) if x is not None]
     if not xs:
@@ -108,8 +115,8 @@ def _rotate(q, k, position_ids, table, interleaved, inverse, out):
                              f"{[(tuple(x.shape), x.dtype, x.device) for x in xs]}")
     if table.rotary_dim > d:
         raise ValueError(f"table rotates {table.rotary_dim} elements, heads have {d}")
-    if table.turns.device != first.device:
-        raise ValueError(f"table is on {table.turns.device}, tensors on {first.device}")
+    if turns.device != first.device:
+        raise ValueError(f"table is on {turns.device}, tensors on {first.device}")
     if not isinstance(position_ids, torch.Tensor) or position_ids.dtype not in (torch.int64, torch.int32):
         raise TypeError("position_ids: expected an int64 or int32 tensor")
     if position_ids.device != first.device:
@@ -162,7 +169,7 @@ def _rotate(q, k, position_ids, table, interleaved, inverse, out):
                 dst[:] = t.stride()[:3]
         ptr = [0 if t is None else t.data_ptr() for t in (ins[0], ins[1])]
         optr = [0 if t is None else t.data_ptr() for t in outs]
-        _lib.call("attn_bwd_b200_rope", ctypes.byref(a), ptr[0], ptr[1], pos.data_ptr(), table.turns.data_ptr(),
+        _lib.call("attn_bwd_b200_rope", ctypes.byref(a), ptr[0], ptr[1], pos.data_ptr(), turns.data_ptr(),
                   optr[0], optr[1], torch.cuda.current_stream().cuda_stream)
     return outs[0], outs[1]
 

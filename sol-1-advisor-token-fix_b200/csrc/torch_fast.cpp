@@ -82,7 +82,7 @@ inline bool int_sizes(const at::Tensor& t) {
 }
 
 // rope(q, k, positions, turns, rotary_dim, factor, interleaved, inverse): two tensors of one
-// type, int64 positions that are contiguous, results in new tensors.
+// type, int64 positions and turns that are contiguous, results in new tensors.
 py::object rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& turns,
                 int64_t rotary_dim, double factor, bool interleaved, bool inverse) {
   if (!q.is_cuda() || q.dim() != 4 || k.dim() != 4 || q.scalar_type() != k.scalar_type()) return py::none();
@@ -100,6 +100,8 @@ py::object rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos,
   if (k.device() != dev || pos.device() != dev || turns.device() != dev) return py::none();
   if (q.stride(3) != 1 || k.stride(3) != 1) return py::none();
   if (pos.scalar_type() != at::kLong || !pos.is_contiguous()) return py::none();
+  if (turns.scalar_type() != at::kLong || turns.dim() != 1 || turns.size(0) * 2 != rotary_dim || !turns.is_contiguous())
+    return py::none();
   int64_t pstride = 0;
   if (pos.dim() == 2 && pos.size(1) == seq && (pos.size(0) == bs || pos.size(0) == 1)) pstride = pos.size(0) == 1 ? 0 : seq;
   else if (pos.dim() != 1 || pos.size(0) != seq) return py::none();
