@@ -145,7 +145,7 @@ enum { ATTN_BWD_DT_BF16 = 0, ATTN_BWD_DT_FP16 = 1, ATTN_BWD_DT_FP32 = 2 };
  * turns [rotary_dim/2]: turns[n] is the frequency as a 64-bit fixed-point fraction of a turn (two's complement), so
  * position * turns wraps exactly and far positions lose nothing.  Strides are in elements,
  * in the order batch, head, position; the head's own elements are contiguous.  An output may
- * be its own input (same strides).  position_stride is the positions' batch stride (0: one
+ * be its own input (same strides) and else overlaps nothing that the call reads or writes.  position_stride is the positions' batch stride (0: one
  * row for all batches); positions are int64. */
 typedef struct {
   int bs, seq, q_heads, k_heads, head_dim, rotary_dim; /* q_heads or k_heads may be 0 */

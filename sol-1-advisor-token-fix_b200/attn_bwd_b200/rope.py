@@ -82,13 +82,95 @@ def _check(x, name):
         raise ValueError(f"{name}: expected [bs, heads, seq, head_dim], got {tuple(x.shape)}")
 
 
+def _reaches(terms, target, budget):
+    """Whether target is a sum of t * stride, lo <= t <= hi, over terms (stride, lo, hi), strides
+    falling.  Layouts nest, so that each level leaves one or two t; a layout that leaves more than
+    the budget of steps counts as reached."""
+    if not terms:
+        return target == 0
+    lo = sum(s * a for s, a, _ in terms[1:])
+    hi = sum(s * b for s, _, b in terms[1:])
+    st, a, b = terms[0]
+    for t in range(max(a, -((hi - target) // st)), min(b, (target - lo) // st) + 1):
+        budget[0] -= 1
+        if budget[0] < 0 or _reaches(terms[1:], target - t * st, budget):
+            return True
+    return False
+
+
+def _extent(t):
+    """Elements from a tensor's first to its last."""
+    n = 1
+    for size, st in zip(t.shape, t.stride()):
+        n += (size - 1) * st
+    return n
+
+
+def _overlap(x, y):
+    """Whether two tensors of one type (strides not negative) share an element's memory."""
+    if x.numel() == 0 or y.numel() == 0:
+        return False
+    at, es = y.data_ptr() - x.data_ptr(), x.element_size()
+    if at >= _extent(x) * es or -at >= _extent(y) * es:
+        return False
+    span = {}
+    for n, st in zip(x.shape, x.stride()):
+        if n > 1 and st:
+            span[st] = (0, span[st][1] + n - 1) if st in span else (0, n - 1)
+    for n, st in zip(y.shape, y.stride()):
+        if n > 1 and st:
+            a, b = span.get(st, (0, 0))
+            span[st] = (a - n + 1, b)
+    terms = [(st, *span[st]) for st in sorted(span, reverse=True)]
+    return any(_reaches(terms, d, [4096]) for d in {at // es, -(-at // es)})
+
+
+def _same_place(x, y):
+    return x.data_ptr() == y.data_ptr() and all(n <= 1 or a == b for n, a, b in zip(x.shape, x.stride(), y.stride()))
+
+
 def _overlaps_itself(t):
-    return any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape))
+    dims, reach = sorted([(st, n) for st, n in zip(t.stride(), t.shape) if n > 1]), 0
+    for st, n in dims:   # nested: every step passes what the smaller ones reach
+        if st <= reach:
+            break
+        reach += (n - 1) * st
+    else:
+        return False
+    if t.numel() == 0:
+        return False
+    if dims[0][0] == 0:
+        return True
+    dims.reverse()
+    budget = [4096]
+    for i, (st, n) in enumerate(dims):   # two elements whose first different index is this one
+        rest = [(s, 1 - m, m - 1) for s, m in dims[i + 1:]]
+        reach = sum(s * b for s, _, b in rest)
+        if any(_reaches(rest, d * st, budget) for d in range(1, min(n - 1, reach // st) + 1)):
+            return True
+    return False
+
+
+def _check_places(ins, outs, given):
+    """Refuses results that the caller gave (the names in given) where they overlap an input, other than
+    their own in its own place, or each other."""
+    names = ("query", "key")
+    own = [o is not None and n in given and _same_place(o, x) for x, o, n in zip(ins, outs, names)]
+    for i, name in enumerate(names):
+        if name not in given:
+            continue
+        for j, x in enumerate(ins):
+            # (an input that is its own result is looked at as that, below)
+            if x is not None and not own[j] and _overlap(outs[i], x):
+                raise ValueError(f"out: {name} overlaps the input {names[j]}" + (" in another order" if i == j else ""))
+    if len(given) == 2 and _overlap(*outs):
+        raise ValueError("out: query and key overlap")
 
 
 def _rotate(q, k, position_ids, table, interleaved, inverse, out):
-    if out is None and isinstance(table, RopeTable):
-        r = _lib.bound("rope", q, k, position_ids, table.turns, table.rotary_dim, table.factor, bool(interleaved), inverse)
+    if isinstance(table, RopeTable) and (out is None or (isinstance(out, (tuple, list)) and len(out) == 2)):
+        r = _lib.bound("rope", q, k, position_ids, table.turns, table.rotary_dim, table.factor, bool(interleaved), inverse,
+                       *(out or (None, None)))
         if r is not None:
             return r
     if not isinstance(table, RopeTable):
@@ -127,7 +209,7 @@ def _rotate(q, k, position_ids, table, interleaved, inverse, out):
     with torch.cuda.device(first.device):
         pos = position_ids.to(torch.int64).contiguous()
         per_batch = pos.dim() == 2 and pos.shape[0] == bs and bs > 1
-        outs = []
+        outs, given = [], []
         if out is None:
             out = (None, None)
         elif not isinstance(out, (tuple, list)) or len(out) != 2:
@@ -152,10 +234,10 @@ def _rotate(q, k, position_ids, table, interleaved, inverse, out):
                     raise ValueError(f"out: {name} must match the input's shape, dtype and device, head elements contiguous")
                 if _overlaps_itself(o):
                     raise ValueError(f"out: {name} overlaps itself")
-                if o.data_ptr() == x.data_ptr() and o.stride() != x.stride():
-                    raise ValueError(f"out: {name} shares the input's memory in another order")
+                given.append(name)
             ins.append(x)
             outs.append(o)
+        _check_places(ins, outs, given)
         a = _lib.RopeArgs()
         a.bs, a.seq, a.head_dim, a.rotary_dim = bs, seq, d, table.rotary_dim
         a.q_heads = q.shape[1] if q is not None else 0
@@ -181,7 +263,8 @@ def rope_fwd(query_states, key_states, position_ids, table, interleaved=False, o
     The first ``table.rotary_dim`` elements of a head are rotated, the rest is copied.  Pairs are
     (n, n + rotary_dim / 2), or neighbours with ``interleaved``.  bfloat16, float16 or float32;
     any strides (heads inside positions or positions inside heads); the results keep the inputs' order in
-    memory.  ``out`` takes preallocated results and may be the inputs themselves."""
+    memory.  ``out`` takes preallocated results and may be the inputs themselves; results that
+    otherwise overlap an input, each other or themselves are refused."""
     return _rotate(query_states, key_states, position_ids, table, interleaved, False, out)
 
 

@@ -14,6 +14,8 @@
 //             the library through ctypes.
 // rope, fused_fwd and fused_bwd do the same for the rotary positions and the fused attention:
 // a decoding step's calls are shorter than the Python path's checks (30 us of it a call).
+#include <algorithm>
+
 #include <torch/extension.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -81,10 +83,91 @@ inline bool int_sizes(const at::Tensor& t) {
   return true;
 }
 
-// rope(q, k, positions, turns, rotary_dim, factor, interleaved, inverse): two tensors of one
-// type, int64 positions and turns that are contiguous, results in new tensors.
+using OptTensor = std::optional<at::Tensor>;
+
+// Whether results that the caller gave may be written: see _overlap and _check_places in rope.py, whose
+// answer this repeats where it is yes (otherwise the general path says what is wrong).
+struct Term {
+  int64_t stride, lo, hi;
+};
+// Whether target is a sum of t * stride, lo <= t <= hi, strides falling; budget: see _reaches.
+bool reaches(const Term* t, int n, int64_t target, int& budget) {
+  if (n == 0) return target == 0;
+  int64_t lo = 0, hi = 0;
+  for (int i = 1; i < n; ++i) { lo += t[i].stride * t[i].lo; hi += t[i].stride * t[i].hi; }
+  const auto floor_div = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((b - 1 - a) / b); };
+  const int64_t last = std::min(t->hi, floor_div(target - lo, t->stride));
+  for (int64_t k = std::max(t->lo, -floor_div(hi - target, t->stride)); k <= last; ++k)
+    if (--budget < 0 || reaches(t + 1, n - 1, target - k * t->stride, budget)) return true;
+  return false;
+}
+int64_t extent(const at::Tensor& t) {
+  int64_t n = 1;
+  for (int i = 0; i < 4; ++i) n += (t.size(i) - 1) * t.stride(i);
+  return n;
+}
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  const int64_t es = x.element_size();
+  const int64_t at = static_cast<char*>(y.data_ptr()) - static_cast<char*>(x.data_ptr());
+  if (at >= extent(x) * es || -at >= extent(y) * es) return false;
+  if (at % es) return true;
+  Term t[8];
+  int n = 0;
+  for (int side = 0; side < 2; ++side)
+    for (int i = 0; i < 4; ++i) {
+      const at::Tensor& z = side ? y : x;
+      const int64_t len = z.size(i) - 1, st = z.stride(i);
+      if (len == 0 || st == 0) continue;
+      int k = 0;
+      while (k < n && t[k].stride != st) ++k;
+      if (k == n) t[n++] = {st, 0, 0};
+      (side ? t[k].lo : t[k].hi) += side ? -len : len;
+    }
+  std::sort(t, t + n, [](const Term& a, const Term& b) { return a.stride > b.stride; });
+  int budget = 4096;
+  return reaches(t, n, at / es, budget);
+}
+// Every step passes what the smaller ones reach.
+bool nested(const at::Tensor& t) {
+  int order[4] = {0, 1, 2, 3};
+  std::sort(order, order + 4, [&](int a, int b) { return t.stride(a) < t.stride(b); });
+  int64_t reach = 0;
+  for (int i : order) {
+    if (t.size(i) <= 1) continue;
+    if (t.stride(i) <= reach) return false;
+    reach += (t.size(i) - 1) * t.stride(i);
+  }
+  return true;
+}
+bool same_place(const at::Tensor& x, const at::Tensor& y) {
+  if (x.data_ptr() != y.data_ptr()) return false;
+  for (int i = 0; i < 4; ++i)
+    if (x.size(i) > 1 && x.stride(i) != y.stride(i)) return false;
+  return true;
+}
+bool places_ok(const at::Tensor& q, const at::Tensor& k, const OptTensor& qo, const OptTensor& ko) {
+  const at::Tensor* in[2] = {&q, &k};
+  const OptTensor* out[2] = {&qo, &ko};
+  bool own[2];
+  for (int i = 0; i < 2; ++i) {
+    const OptTensor& o = *out[i];
+    if (o.has_value() && (o->sizes() != in[i]->sizes() || o->scalar_type() != in[i]->scalar_type() ||
+                          o->device() != in[i]->device() || o->stride(3) != 1 || !nested(*o)))
+      return false;
+    own[i] = o.has_value() && same_place(*o, *in[i]);
+  }
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j)
+      if (out[i]->has_value() && !own[j] && overlap(**out[i], *in[j])) return false;
+  return !(qo.has_value() && ko.has_value() && overlap(*qo, *ko));
+}
+
+// rope(q, k, positions, turns, rotary_dim, factor, interleaved, inverse, q_out, k_out): two tensors of one
+// type, int64 positions and turns that are contiguous; results in new tensors where none are given.
 py::object rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& turns,
-                int64_t rotary_dim, double factor, bool interleaved, bool inverse) {
+                int64_t rotary_dim, double factor, bool interleaved, bool inverse, const OptTensor& q_out,
+                const OptTensor& k_out) {
   if (!q.is_cuda() || q.dim() != 4 || k.dim() != 4 || q.scalar_type() != k.scalar_type()) return py::none();
   int dtype;
   switch (q.scalar_type()) {
@@ -106,7 +189,8 @@ py::object rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos,
   if (pos.dim() == 2 && pos.size(1) == seq && (pos.size(0) == bs || pos.size(0) == 1)) pstride = pos.size(0) == 1 ? 0 : seq;
   else if (pos.dim() != 1 || pos.size(0) != seq) return py::none();
   DeviceScope scope(dev);
-  at::Tensor qo = at::empty_like(q), ko = at::empty_like(k);
+  if ((q_out.has_value() || k_out.has_value()) && !places_ok(q, k, q_out, k_out)) return py::none();
+  at::Tensor qo = q_out.has_value() ? *q_out : at::empty_like(q), ko = k_out.has_value() ? *k_out : at::empty_like(k);
   if (qo.stride(3) != 1 || ko.stride(3) != 1) return py::none();
   attn_bwd_rope_t a = {};
   a.bs = int(bs);
@@ -129,8 +213,6 @@ py::object rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos,
   if (rc != 0) return py::int_(rc);
   return py::make_tuple(qo, ko);
 }
-
-using OptTensor = std::optional<at::Tensor>;
 
 // A state that the kernels read in place: see _ready in fused.py.
 inline bool ready_state(const at::Tensor& t, const at::Tensor& q) {

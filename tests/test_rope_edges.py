@@ -38,3 +38,68 @@ def test_table_of_another_size_is_refused_on_the_gpu(cuda):
                 ab.rope_fwd(*args, pos, table, out=tuple(None if a is None else torch.empty_like(a) for a in args))
     ok = ab.RopeTable(torch.arange(32, dtype=torch.int64, device="cuda"), 64, 1.0)
     assert ab.rope_fwd(x, x, pos, ok)[0].shape == x.shape
+
+
+# ------------------------------------------------------------------ results that overlap
+def _cells(t):
+    """Addresses of a small tensor's elements, in bytes."""
+    idx = torch.zeros(t.shape, dtype=torch.int64)
+    for n, (size, st) in enumerate(zip(t.shape, t.stride())):
+        shape = [1] * t.dim()
+        shape[n] = size
+        idx = idx + (torch.arange(size) * st * t.element_size()).reshape(shape)
+    return t.data_ptr() + idx.flatten()
+
+
+def test_overlap_against_every_address():
+    """Random small layouts in one buffer: what the check says is what their addresses say."""
+    g = torch.Generator().manual_seed(0)
+    buf = torch.zeros(4096, dtype=BF)
+    rnd = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=g))
+    met = own = 0
+    for _ in range(3000):
+        ts = []
+        for _ in range(2):
+            shape = [rnd(1, 4) for _ in range(4)]
+            if rnd(0, 2):   # nested, as layouts are, in any order and with gaps
+                stride, st = [0] * 4, 1
+                for n in torch.randperm(4, generator=g).tolist():
+                    stride[n] = st
+                    st *= shape[n] + rnd(0, 2)
+            else:
+                stride = [rnd(0, 12) for _ in range(4)]
+            ts.append(buf.as_strided(shape, stride, rnd(0, 60)))
+        a, b = (set(_cells(t).tolist()) for t in ts)
+        assert ab.rope._overlap(*ts) == bool(a & b), [(t.shape, t.stride(), t.storage_offset()) for t in ts]
+        met += bool(a & b)
+        for t, cells in zip(ts, (a, b)):
+            assert ab.rope._overlaps_itself(t) == (len(cells) < t.numel()), (t.shape, t.stride())
+            own += len(cells) < t.numel()
+    assert 500 < met < 2800 and own > 500
+    big = torch.empty(2, 88, 16001, 128, dtype=BF, device="meta")   # sizes of a real layer: no search
+    assert not ab.rope._overlaps_itself(big) and not ab.rope._overlaps_itself(big.transpose(1, 2))
+
+
+@pytest.mark.gpu
+def test_overlapping_results(cuda):
+    g = torch.Generator().manual_seed(1)
+    fused = torch.randn(2, 9, 8, 64, generator=g).to(BF).cuda()   # [bs, seq, 4 + 2 + 2 heads, d]
+    q, k = fused[:, :, :4].transpose(1, 2), fused[:, :, 4:6].transpose(1, 2)
+    pos, t = torch.arange(9, device="cuda"), ab.rope_table(64)
+    want = ab.rope_fwd(q, k, pos, t)
+    rest = fused[:, :, 6:].clone()
+    out = ab.rope_fwd(q, k, pos, t, out=(q, k))                    # in place in one buffer: nothing overlaps
+    assert all(torch.equal(a, b) for a, b in zip(out, want)) and torch.equal(fused[:, :, 6:], rest)
+    x = torch.randn(1, 2, 20, 64, generator=g).to(BF).cuda()
+    a, b, c = x[:, :, :9], x[:, :, 1:10], x[:, :, 10:19]
+    for bad in (dict(q=a, k=None, out=(b, None)),                  # its own input, a position on
+                dict(q=a, k=c, out=(c, torch.empty_like(c))),      # the other input
+                dict(q=a, k=c, out=(torch.empty_like(a), b)),
+                dict(q=a.clone(), k=c.clone(), out=(a, b)),        # each other
+                dict(q=a.clone(), k=c.clone(), out=(a, a)),
+                dict(q=a.clone(), k=None, out=(x.as_strided((1, 2, 9, 64), (0, 64, 64, 1)), None)),
+                dict(q=a, k=None, out=(x.as_strided((1, 2, 9, 64), (64, 64, 128, 1)), None))):
+        with pytest.raises(ValueError, match="overlap"):
+            ab.rope_fwd(bad["q"], bad["k"], pos, t, out=bad["out"])
+    got = ab.rope_fwd(a, None, pos, t, out=(c, None))[0]           # beside the input in its buffer
+    assert torch.equal(got, ab.rope_fwd(a, None, pos, t)[0])
