@@ -11,6 +11,8 @@ __all__ = ["fused_attn_fwd", "fused_attn_bwd"]
 
 _TYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_FP16}
 
+_MIN_CAP = 1e-30   # the library's; checked before the number is narrowed to fp32, where far less is 0: no cap
+
 
 def _check(t, name, like=None):
     if not isinstance(t, torch.Tensor):
@@ -60,7 +62,7 @@ def _bound(name, tensors, q, k, v, scale, softcap, slopes, causal, prefix_lens, 
         if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[3] == 0:
             return None
         scale = 1.0 / math.sqrt(q.shape[3])
-    if not (0 < scale < math.inf and 0 <= softcap < math.inf):
+    if not (0 < scale < math.inf and (softcap == 0 or _MIN_CAP < softcap < math.inf)):
         return None
     return _lib.bound(name, *tensors, scale, softcap, slopes, bool(causal), prefix_lens, qd, kd)
 
@@ -85,8 +87,8 @@ class _Call:
         if not (scale > 0 and math.isfinite(scale)):
             raise ValueError(f"scale must be positive, got {scale}")
         softcap = float(softcap or 0.0)
-        if not (softcap >= 0 and math.isfinite(softcap)):
-            raise ValueError(f"softcap must be positive, or 0 for none, got {softcap}")
+        if not (softcap == 0 or _MIN_CAP < softcap < math.inf):
+            raise ValueError(f"softcap must be above {_MIN_CAP} and finite, or 0 for none, got {softcap}")
         if prefix_lens is not None and not causal:
             raise ValueError("prefix_lens needs causal=True: without it every query sees all keys")
         dev = q.device
@@ -133,7 +135,7 @@ def fused_attn_fwd(query_states, key_states, value_states, scale=None, softcap=0
     row of queries over a long cache is a decoding step.
 
     The score of head h, query position i and key j is x = scale * q.k (default scale
-    1 / sqrt(d)), capped to softcap * tanh(x / softcap) if softcap > 0, minus slopes[h] * |i - j|
+    1 / sqrt(d)), capped to softcap * tanh(x / softcap) if softcap is not 0 (then above 1e-30), minus slopes[h] * |i - j|
     (slopes [heads] float32: constants, no gradient is taken).  A query sees
       - with ``causal``, keys j <= i, and all keys j < prefix_lens[b] (int32 [bs]) besides;
       - with ``documents`` (int32 [bs, seq], or a pair for queries and keys), keys of its own

@@ -108,3 +108,15 @@ def test_nan_under_a_cap_stays_nan(cuda, bs, heads, kv, sq, skv, std, mod, dtype
     if kv > 1:   # the other groups
         assert torch.isfinite(o[0, :, grp:]).all() and torch.isfinite(dv[0, 1:]).all()
     assert ab.poll_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e-60, 5e-324, 1e-46, 1e-35, 1e-30, -1e-60, math.nan, math.inf])
+def test_caps_too_low_to_be_told_from_none_are_refused(cuda, cap):
+    q, k, v, do = _inputs(1, 2, 1, 4, 4, 64, BF)
+    o, lse = ab.fused_attn_fwd(q, k, v)
+    with pytest.raises(ValueError, match="softcap"):
+        ab.fused_attn_fwd(q, k, v, softcap=cap)
+    with pytest.raises(ValueError, match="softcap"):
+        ab.fused_attn_bwd(do, q, k, v, o, lse, softcap=cap)
+    assert torch.equal(ab.fused_attn_fwd(q, k, v, softcap=None)[0], o) and torch.equal(ab.fused_attn_fwd(q, k, v, softcap=-0.0)[0], o)
