@@ -37,7 +37,10 @@ inline int check_args(const attn_bwd_fused_t* a) {
   if (!(a->scale > 0.f) || !(a->scale < 1e38f) || !(a->softcap >= 0.f) || !(a->softcap < 1e38f)) return ATTN_BWD_EINVAL;
   if (a->softcap > 0.f && !(a->softcap > 1e-30f && double(a->scale) / a->softcap < 1e30)) return ATTN_BWD_EINVAL;
   if (a->prefix_lens && !a->causal) return ATTN_BWD_EINVAL;
-  if ((a->q_documents == nullptr) != (a->kv_documents == nullptr)) return ATTN_BWD_EINVAL;
+  // both or neither; an array of no elements may be null
+  if ((a->q_documents == nullptr) != (a->kv_documents == nullptr) &&
+      (a->q_documents ? a->seq_kv : a->seq_q) != 0 && a->bs != 0)
+    return ATTN_BWD_EINVAL;
   if (a->head_dim != 64 && a->head_dim != 128) return ATTN_BWD_EUNSUPPORTED;
   if (a->dtype != ATTN_BWD_DT_BF16 && a->dtype != ATTN_BWD_DT_FP16) return ATTN_BWD_EUNSUPPORTED;
   if (!tma_strides_ok(a->q_stride, a->bs, a->heads, a->seq_q) ||

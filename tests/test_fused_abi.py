@@ -77,3 +77,30 @@ def test_gradients_at_any_16_bytes(cuda, offset, row, gap, bs, kv, dtype, d):
     for buf, g, w in zip(bufs, grads, want):
         assert torch.equal(g, w) and _only_there(buf, g)
     assert ab.poll_error() == 0
+
+
+def test_documents_of_no_queries_without_device():
+    """An array of no elements has no address."""
+    from test_fused import _args
+    lib, a = _lib.load(), _args(seq_q=0, kv_documents=16)
+    assert lib.attn_bwd_b200_fused_fwd(ctypes.byref(a), 0, 16, 16, 0, 0, 0, 0, 0) == _lib.OK
+    a = _args(seq_q=0, seq_kv=0, q_documents=16)
+    assert lib.attn_bwd_b200_fused_bwd(ctypes.byref(a), *[0] * 9, 0, 0, 0) == _lib.OK
+    a = _args(bs=0, q_documents=16)
+    assert lib.attn_bwd_b200_fused_bwd(ctypes.byref(a), *[0] * 9, 0, 0, 0) == _lib.OK
+    for kw in (dict(kv_documents=16), dict(seq_kv=0, kv_documents=16), dict(q_documents=16)):
+        assert lib.attn_bwd_b200_fused_fwd(ctypes.byref(_args(**kw)), 16, 16, 16, 16, 16, 0, 0, 0) == _lib.EINVAL
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs,sq,skv", [(2, 5, 0), (2, 0, 5), (2, 0, 0), (0, 3, 4), (1, 1, 0), (3, 200, 0), (3, 0, 200)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_documents_of_no_positions(cuda, bs, sq, skv, causal):
+    q, k, v, do = _inputs(bs, 4, 2, sq, skv, 64, BF)
+    docs = tuple(torch.zeros(bs, n, dtype=torch.int32, device="cuda") for n in (sq, skv))
+    o, lse = ab.fused_attn_fwd(q, k, v, documents=docs, causal=causal, softcap=5.0)
+    dq, dk, dv = ab.fused_attn_bwd(do, q, k, v, o, lse, documents=docs, causal=causal, softcap=5.0)
+    assert o.shape == (bs, sq, 4, 64) and (o == 0).all() and (lse == -float("inf")).all()
+    for g, t in ((dq, q), (dk, k), (dv, v)):
+        assert g.shape == t.shape and (g == 0).all()
+    assert ab.poll_error() == 0
