@@ -55,7 +55,7 @@ def _bound(name, tensors, q, k, v, scale, softcap, slopes, causal, prefix_lens, 
     """The call through the C++ binding, or None where the general path has to look at it."""
     qd = kd = documents
     if isinstance(documents, (tuple, list)):
-        if len(documents) != 2:
+        if len(documents) != 2 or documents[0] is None or documents[1] is None:
             return None
         qd, kd = documents
     if scale is None:

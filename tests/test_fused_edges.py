@@ -120,3 +120,17 @@ def test_caps_too_low_to_be_told_from_none_are_refused(cuda, cap):
     with pytest.raises(ValueError, match="softcap"):
         ab.fused_attn_bwd(do, q, k, v, o, lse, softcap=cap)
     assert torch.equal(ab.fused_attn_fwd(q, k, v, softcap=None)[0], o) and torch.equal(ab.fused_attn_fwd(q, k, v, softcap=-0.0)[0], o)
+
+
+@pytest.mark.gpu
+def test_a_pair_of_documents_has_two(cuda):
+    """A pair that lacks one or both is refused, not taken for no documents."""
+    q, k, v, do = _inputs(1, 2, 1, 4, 4, 64, BF)
+    o, lse = ab.fused_attn_fwd(q, k, v)
+    one = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    for docs, err in (((None, None), TypeError), ((one, None), TypeError), ((None, one), TypeError), ([None, None], TypeError),
+                      ((one,), ValueError), ((one, one, one), ValueError), ((), ValueError)):
+        with pytest.raises(err, match="documents"):
+            ab.fused_attn_fwd(q, k, v, documents=docs)
+        with pytest.raises(err, match="documents"):
+            ab.fused_attn_bwd(do, q, k, v, o, lse, documents=docs)
