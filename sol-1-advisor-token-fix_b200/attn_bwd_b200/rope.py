@@ -1,5 +1,6 @@
 """Rotary positions of query and key states, forward and gradient, over ``attn_bwd_b200_rope``."""
 import ctypes
+import decimal
 import math
 
 import torch
@@ -52,23 +53,46 @@ def rope_table(rotary_dim, base=10000.0, scaling=None, device="cuda"):
         s = float(scaling.get("factor", 0.0))
         if not (s >= 1.0 and math.isfinite(s)):
             raise ValueError(f"scaling factor must be at least 1, got {s}")
-    if kind == "base":
-        if rotary_dim == 2:
-            raise ValueError("base scaling needs rotary_dim > 2")
-        base *= s ** (rotary_dim / (rotary_dim - 2))
-    f = [base ** (-2.0 * n / rotary_dim) for n in range(rotary_dim // 2)]
-    if kind == "linear":
-        f = [x / s for x in f]
-    elif kind == "ramp":
+    if kind == "base" and rotary_dim == 2:
+        raise ValueError("base scaling needs rotary_dim > 2")
+    if kind == "ramp":
         length, low, high = (float(scaling.get(k, d)) for k, d in (("original_length", 0.0), ("low", 1.0), ("high", 32.0)))
-        if not (length > 0 and high > low):
+        if not (length > 0 and high > low > -math.inf):
             raise ValueError("ramp scaling needs original_length > 0 and high > low")
-        keep = [min(1.0, max(0.0, (length * x / (2 * math.pi) - low) / (high - low))) for x in f]
-        f = [x * w + x / s * (1.0 - w) for x, w in zip(f, keep)]
         factor = float(scaling.get("attention_factor", 0.1 * math.log(s) + 1.0))
-    turns = [round(math.fmod(x / (2 * math.pi), 1.0) * 2.0 ** 64) % 2 ** 64 for x in f]
+    # A frequency's last bits count (position * turns is exact whatever the position), and fp64 has too few:
+    # 64 behind the point, through a power and a division by 2 pi, in decimal digits to spare.
+    with decimal.localcontext() as ctx:
+        ctx.prec = 60 + max(0, -decimal.Decimal(base).adjusted())   # base < 1: frequencies up to 1 / base
+        num = decimal.Decimal
+        two_pi = 2 * _pi(ctx.prec)
+        exponent = num(base).ln()
+        if kind == "base":
+            exponent += num(s).ln() * rotary_dim / (rotary_dim - 2)
+        f = [(exponent * (-2 * n) / rotary_dim).exp() for n in range(rotary_dim // 2)]
+        if kind == "linear":
+            f = [x / num(s) for x in f]
+        elif kind == "ramp":
+            keep = [min(num(1), max(num(0), (num(length) * x / two_pi - num(low)) / (num(high) - num(low)))) for x in f]
+            f = [x * w + x / num(s) * (1 - w) for x, w in zip(f, keep)]
+        turns = [int((x / two_pi % 1 * 2 ** 64).to_integral_value()) % 2 ** 64 for x in f]
     turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
     return RopeTable(torch.tensor(turns, dtype=torch.int64).to(device), rotary_dim, factor)
+
+
+def _pi(digits):
+    """pi = 16 atan(1/5) - 4 atan(1/239) (Machin) to that many digits."""
+    one = 10 ** (digits + 10)
+
+    def atan_inverse(x):
+        total, power, n = 0, one // x, 1
+        while power:
+            total += power // n if n % 4 == 1 else -(power // n)
+            power //= x * x
+            n += 2
+        return total
+
+    return decimal.Decimal(16 * atan_inverse(5) - 4 * atan_inverse(239)) / one
 
 
 def _check(x, name):
