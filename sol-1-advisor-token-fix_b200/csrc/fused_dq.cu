@@ -172,10 +172,16 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
         const DqUnit f = dq_unit(prm, Unit{x, y, z, 0});
         if (int(lane) < 2 * (D / 64))
           prefetch_l2_4d(int(lane) & 1 ? &tm_do : &tm_q, (int(lane) >> 1) * 64, f.r0, f.h, f.b);
-        for (int r = f.r0 + int(lane); r <= f.r1; r += 32)
-          for (int c = 0; c < D * 2; c += 128)
-            prefetch_l2(prm.o + (((size_t)f.b * p.sq + r) * p.H + f.h) * (D * 2) + c);
-        if (!p.has_docs) return 0;
+        auto prefetch_o = [&](int tiles) {   // rows of one key tile read no o
+          if (tiles > 1)
+            for (int r = f.r0 + int(lane); r <= f.r1; r += 32)
+              for (int c = 0; c < D * 2; c += 128)
+                prefetch_l2(prm.o + (((size_t)f.b * p.sq + r) * p.H + f.h) * (D * 2) + c);
+        };
+        if (!p.has_docs) {
+          prefetch_o(f.n);
+          return 0;
+        }
         const DocRange qd = p.qrange[(size_t)f.b * p.n_tiles + f.r0 / TILE];
         const int t1 = max(0, row_limit(p, f.r1, f.pre) + TILE - 1) / TILE;
         int n = 0;
@@ -190,6 +196,7 @@ dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
           }
           n = list_append(sh.lists + slot * kMaxList, n, t + int(lane), st, scrub, lane);
         }
+        prefetch_o(n);
         return n;
       });
     }
