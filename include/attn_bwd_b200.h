@@ -171,7 +171,8 @@ int attn_bwd_b200_rope(const attn_bwd_rope_t* args, const void* q, const void* k
  *   q [bs, heads, seq_q, head_dim], k and v [bs, kv_heads, seq_kv, head_dim]: strides in
  *     elements in the order batch, head, position (positive multiples of 8, head elements
  *     contiguous, 16-byte aligned), heads a multiple of kv_heads, head_dim 64 or 128; bs and
- *     heads at most 65535; the backward call with documents: at most 262144 positions
+ *     heads at most 65535, positions below 2^30; the backward call: at most 33554432 keys, with
+ *     documents at most 262144 positions
  *   o [bs, seq_q, heads, head_dim] contiguous; lse [bs, heads, seq_q] fp32 (natural log)
  *   dq, dk, dv: shaped as q, k, v, strides in dq_stride / dk_stride / dv_stride
  * workspace: at least attn_bwd_b200_fused_workspace() bytes, 256-byte aligned, private to the call until

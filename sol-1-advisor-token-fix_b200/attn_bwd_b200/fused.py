@@ -164,8 +164,8 @@ def fused_attn_bwd(grad_attn_output, query_states, key_states, value_states, att
     """Gradients (grad_query, grad_key, grad_value) of :func:`fused_attn_fwd`'s first three
     arguments, from grad_attn_output [bs, seq_q, heads, d] and that call's results; the other
     arguments as they were given there.  The gradients have the shapes of the states (keys' and
-    values' summed over the heads that share them) and their order in memory.  With documents,
-    at most 262144 positions.  Equal inputs give equal bits."""
+    values' summed over the heads that share them) and their order in memory.  At most
+    33554432 keys; with documents, at most 262144 positions.  Equal inputs give equal bits."""
     softcap = softcap or 0.0
     mods = (query_states, key_states, value_states, scale, softcap, slopes, causal, prefix_lens, documents)
     r = _bound("fused_bwd", (grad_attn_output, query_states, key_states, value_states, attn_output, lse), *mods)

@@ -21,6 +21,8 @@ static int dkv_splits(const attn_bwd_fused_t* a, int sm_count) {
   if (units == 0) return 1;
   long long s = sm_count / units;
   if (s > items) s = items;
+  const long long least = (items + kMaxUnit - 1) / kMaxUnit;
+  if (s < least) s = least;
   if (s <= 1) return 1;
   const long long per = (items + s - 1) / s;
   return int((items + per - 1) / per);   // no split without items
@@ -71,6 +73,7 @@ extern "C" int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* a, const void* go
   if (tiles_of(a->seq_q) > (1 << 30) / a->heads || tiles_of(a->seq_kv) > (1 << 30) / a->kv_heads) return ATTN_BWD_EINVAL;
   // with documents a unit lists its tiles
   if (a->q_documents && (tiles_of(a->seq_q) > kMaxList || tiles_of(a->seq_kv) > kMaxList)) return ATTN_BWD_EUNSUPPORTED;
+  if (tiles_of(a->seq_kv) > kMaxUnit) return ATTN_BWD_EUNSUPPORTED;   // of one unit of dq
   HostDevice dev;
   if ((rc = host_device(&dev))) return rc;
   const BwdLayout l = layout_bwd(a, dev.sm_count);

@@ -14,6 +14,9 @@ using namespace sm100;
 
 constexpr int TILE = 128;        // rows of a query tile, keys of a key tile
 constexpr int kMaxList = 2048;   // documents: tiles of one unit at most
+// Tiles of one unit at most: the scheduler and warps without rows wait for a whole unit, and waits give up
+// after 2 s.  A capped tile takes up to 4 us, so a unit about 1 s.
+constexpr int kMaxUnit = 1 << 18;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

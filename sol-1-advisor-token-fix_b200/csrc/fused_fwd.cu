@@ -37,11 +37,12 @@ static FwdParams plan_fwd(const attn_bwd_fused_t* a, int sm_count) {
   const int parts = f.duo ? 2 : 1;
   // Too few units for the GPU: the keys are split (one token over 40000 keys: 50 us, 292 without; 77
   // tokens over 32013: 142 and 463), two tiles a split at least (one a split is no faster and
-  // leaves more to join), and never more tiles than a unit's list holds.
+  // leaves more to join), and never more tiles than a unit may have.
   const long long units = (long long)f.blocks_q * f.head_slots * p.bs;
   long long splits = units > 0 ? sm_count / units : 1;
   if (splits > p.n_tiles / 2) splits = p.n_tiles / 2;
-  const long long least = p.has_docs ? (p.n_tiles + kMaxList - 1) / kMaxList : 1;
+  const int most = p.has_docs ? kMaxList : kMaxUnit;
+  const long long least = (p.n_tiles + most - 1) / most;
   if (splits < least) splits = least;
   if (splits < 1) splits = 1;
   p.tiles_per_split = int((p.n_tiles + splits - 1) / splits);

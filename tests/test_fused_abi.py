@@ -104,3 +104,27 @@ def test_documents_of_no_positions(cuda, bs, sq, skv, causal):
     for g, t in ((dq, q), (dk, k), (dv, v)):
         assert g.shape == t.shape and (g == 0).all()
     assert ab.poll_error() == 0
+
+
+def test_backward_over_more_keys_than_a_unit_may_have():
+    """A unit of dq runs over all keys; its kernel's waits end after 2 s."""
+    from test_fused import _args
+    lib = _lib.load()
+    for keys, code in (((1 << 25) + 1, _lib.EUNSUPPORTED), ((1 << 30) - 1, _lib.EUNSUPPORTED)):
+        assert lib.attn_bwd_b200_fused_bwd(ctypes.byref(_args(seq_kv=keys)), *[16] * 9, 0, 0, 0) == code
+
+
+@pytest.mark.gpu
+def test_units_stay_below_the_waits_limit(cuda):
+    """Enough rows for every SM, and so no split for their sake: long axes are split all the same."""
+    from test_fused import _args
+    lib = _lib.load()
+    need = lambda back, **kw: lib.attn_bwd_b200_fused_workspace(ctypes.byref(_args(bs=300, heads=1, kv_heads=1, **kw)), back)
+    part = 300 * 4 * 129   # one part: fp32 outputs and statistics of a row, 128 elements a head
+    assert need(0, seq_q=1, seq_kv=1 << 25) == 2 * part          # two chains of one CTA
+    assert need(0, seq_q=1, seq_kv=(1 << 25) + 1) == 4 * part
+    assert need(0, seq_q=300, seq_kv=1 << 25) == 0
+    assert need(0, seq_q=300, seq_kv=1 << 27) == 300 * 4 * part
+    stat = lambda n: 2 * 300 * n * 4
+    assert need(1, seq_q=1 << 25, seq_kv=8) == stat(1 << 25)
+    assert need(1, seq_q=1 << 26, seq_kv=8) == stat(1 << 26) + 2 * 300 * 8 * 2 * 128 * 4
