@@ -69,7 +69,9 @@ def rope_table(rotary_dim, base=10000.0, scaling=None, device="cuda"):
         exponent = num(base).ln()
         if kind == "base":
             exponent += num(s).ln() * rotary_dim / (rotary_dim - 2)
-        f = [(exponent * (-2 * n) / rotary_dim).exp() for n in range(rotary_dim // 2)]
+        ratio, f = (exponent * -2 / rotary_dim).exp(), [num(1)]
+        for _ in range(rotary_dim // 2 - 1):
+            f.append(f[-1] * ratio)
         if kind == "linear":
             f = [x / num(s) for x in f]
         elif kind == "ramp":
@@ -282,7 +284,8 @@ def _rotate(q, k, position_ids, table, interleaved, inverse, out):
 
 def rope_fwd(query_states, key_states, position_ids, table, interleaved=False, out=None):
     """Rotates query_states [bs, heads, seq, d] and key_states [bs, kv_heads, seq, d] (either may
-    be None) at position_ids ([seq], [1, seq] or [bs, seq]; any integer, however far) in one launch.
+    be None) at position_ids ([seq], [1, seq] or [bs, seq]; any integer, and the angle of position p is
+    off by |p| * 2^-65 + 2^-33 turns at most besides fp32's own rounding) in one launch.  Heads of at most 4096.
 
     The first ``table.rotary_dim`` elements of a head are rotated, the rest is copied.  Pairs are
     (n, n + rotary_dim / 2), or neighbours with ``interleaved``.  bfloat16, float16 or float32;
