@@ -144,5 +144,5 @@ def bound(name, *args):
     except TypeError:   # not what it takes: the general path reports it
         return None
     if isinstance(r, int):
-        raise AttnBwdError("attn_bwd_b200_" + name, r)
+        raise AttnBwdError("attn_bwd_b200_" + name.removesuffix("_into"), r)
     return r

@@ -129,20 +129,24 @@ def fused_attn_fwd(query_states, key_states, value_states, scale=None, softcap=0
                    prefix_lens=None, documents=None):
     """Attention forward.  Returns (attn_output [bs, seq_q, heads, d], lse [bs, heads, seq_q] float32).
 
-    query_states [bs, heads, seq_q, d], key_states and value_states [bs, kv_heads, seq_kv, d], bfloat16 or float16,
-    d 64 or 128, heads a multiple of kv_heads, batch and heads at most 65535; any strides (copied
-    only where head elements are not contiguous or rows not 16-byte aligned).  The queries are the last seq_q positions: one
-    row of queries over a long cache is a decoding step.
+    query_states [bs, heads, seq_q, d], key_states and value_states [bs, kv_heads, seq_kv, d], bfloat16 or
+    float16, d 64 or 128, heads a multiple of kv_heads, batch and heads at most 65535; any strides
+    (copied only where head elements are not contiguous or rows not 16-byte aligned).  The queries are
+    the last seq_q positions: one row of queries over a long cache is a decoding step.
 
     The score of head h, query position i and key j is x = scale * q.k (default scale
-    1 / sqrt(d)), capped to softcap * tanh(x / softcap) if softcap is not 0 (then above 1e-30), minus slopes[h] * |i - j|
-    (slopes [heads] float32: constants, no gradient is taken).  A query sees
+    1 / sqrt(d)), capped to softcap * tanh(x / softcap) if softcap is not 0 (then above 1e-30), minus
+    slopes[h] * |i - j| (slopes [heads] float32: constants, no gradient is taken).  A query sees
       - with ``causal``, keys j <= i, and all keys j < prefix_lens[b] (int32 [bs]) besides;
       - with ``documents`` (int32 [bs, seq], or a pair for queries and keys), keys of its own
         document.  Negative numbers are padding: such queries and keys belong to no document, and
         what they hold (NaN included) reaches no result.
-    A query that sees no key has output 0 and lse -inf.  A NaN or infinity in a key or value of
-    a document (or without documents) may reach all queries near it, seen or not."""
+    A query that sees no key has output 0 and lse -inf.  A NaN or infinity in a query, key or value of
+    a document (or without documents) may reach all results near it, seen or not.
+
+    Weights are rounded to the inputs' 16 bits before they are multiplied with the values; scores, their
+    maxima and sums, lse and the products' sums are float32.  There is no dropout: a layer that drops weights
+    keeps them, and :func:`attn_bwd` takes its gradients."""
     softcap = softcap or 0.0
     mods = (query_states, key_states, value_states, scale, softcap, slopes, causal, prefix_lens, documents)
     r = _bound("fused_fwd", (query_states, key_states, value_states), *mods)
@@ -165,7 +169,13 @@ def fused_attn_bwd(grad_attn_output, query_states, key_states, value_states, att
     arguments, from grad_attn_output [bs, seq_q, heads, d] and that call's results; the other
     arguments as they were given there.  The gradients have the shapes of the states (keys' and
     values' summed over the heads that share them) and their order in memory.  At most
-    33554432 keys; with documents, at most 262144 positions.  Equal inputs give equal bits."""
+    33554432 keys; with documents, at most 262144 positions.  Equal inputs give equal bits.
+
+    attn_output and lse have to be that very call's: queries whose keys all lie in one tile of 128 do not
+    read attn_output, so results merged from calls over parts of the keys give wrong gradients.  The
+    weights and the gradients of the scores are rounded to 16 bits before they are multiplied.  In float16 a
+    gradient of a score below 6e-8 is lost and one above 65504 infinite, also where the results would
+    be in range: scale the loss, as for any float16 gradient."""
     softcap = softcap or 0.0
     mods = (query_states, key_states, value_states, scale, softcap, slopes, causal, prefix_lens, documents)
     r = _bound("fused_bwd", (grad_attn_output, query_states, key_states, value_states, attn_output, lse), *mods)

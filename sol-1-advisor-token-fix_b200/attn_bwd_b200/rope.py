@@ -194,9 +194,12 @@ def _check_places(ins, outs, given):
 
 
 def _rotate(q, k, position_ids, table, interleaved, inverse, out):
-    if isinstance(table, RopeTable) and (out is None or (isinstance(out, (tuple, list)) and len(out) == 2)):
-        r = _lib.bound("rope", q, k, position_ids, table.turns, table.rotary_dim, table.factor, bool(interleaved), inverse,
-                       *(out or (None, None)))
+    if isinstance(table, RopeTable):
+        args = (q, k, position_ids, table.turns, table.rotary_dim, table.factor, bool(interleaved), inverse)
+        if out is None:
+            r = _lib.bound("rope", *args)
+        else:
+            r = _lib.bound("rope_into", *args, *out) if isinstance(out, (tuple, list)) and len(out) == 2 else None
         if r is not None:
             return r
     if not isinstance(table, RopeTable):

@@ -163,11 +163,12 @@ bool places_ok(const at::Tensor& q, const at::Tensor& k, const OptTensor& qo, co
   return !(qo.has_value() && ko.has_value() && overlap(*qo, *ko));
 }
 
-// rope(q, k, positions, turns, rotary_dim, factor, interleaved, inverse, q_out, k_out): two tensors of one
-// type, int64 positions and turns that are contiguous; results in new tensors where none are given.
-py::object rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& turns,
-                int64_t rotary_dim, double factor, bool interleaved, bool inverse, const OptTensor& q_out,
-                const OptTensor& k_out) {
+// rope(q, k, positions, turns, rotary_dim, factor, interleaved, inverse) and rope_into(.., q_out, k_out):
+// two tensors of one type, int64 positions and turns that are contiguous; results in new tensors where
+// none are given.
+py::object rope_into(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& turns,
+                     int64_t rotary_dim, double factor, bool interleaved, bool inverse, const OptTensor& q_out,
+                     const OptTensor& k_out) {
   if (!q.is_cuda() || q.dim() != 4 || k.dim() != 4 || q.scalar_type() != k.scalar_type()) return py::none();
   int dtype;
   switch (q.scalar_type()) {
@@ -212,6 +213,11 @@ py::object rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos,
                                     qo.data_ptr(), ko.data_ptr(), stream_of(dev));
   if (rc != 0) return py::int_(rc);
   return py::make_tuple(qo, ko);
+}
+
+py::object rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& turns,
+                int64_t rotary_dim, double factor, bool interleaved, bool inverse) {
+  return rope_into(q, k, pos, turns, rotary_dim, factor, interleaved, inverse, std::nullopt, std::nullopt);
 }
 
 // A state that the kernels read in place: see _ready in fused.py.
@@ -322,6 +328,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "C++ host binding of the attn_bwd_b200 full call for PyTorch tensors";
   m.def("fast", &fast, "full call on ready inputs: (dS, dV), an error code, or None");
   m.def("rope", &rope, "rotary positions of ready inputs: (q, k), an error code, or None");
+  m.def("rope_into", &rope_into, "the same into given results (either may be None)");
   m.def("fused_fwd", &fused_fwd, "fused attention on ready inputs: (o, lse), an error code, or None");
   m.def("fused_bwd", &fused_bwd, "its gradients: (dq, dk, dv), an error code, or None");
 }
