@@ -57,7 +57,7 @@ def rope_table(rotary_dim, base=10000.0, scaling=None, device="cuda"):
         raise ValueError("base scaling needs rotary_dim > 2")
     if kind == "ramp":
         length, low, high = (float(scaling.get(k, d)) for k, d in (("original_length", 0.0), ("low", 1.0), ("high", 32.0)))
-        if not (length > 0 and high > low > -math.inf):
+        if not (length > 0 and high > low > -math.inf) or length == high == math.inf:
             raise ValueError("ramp scaling needs original_length > 0 and high > low")
         factor = float(scaling.get("attention_factor", 0.1 * math.log(s) + 1.0))
     # A frequency's last bits count (position * turns is exact whatever the position), and fp64 has too few:
@@ -72,13 +72,15 @@ def rope_table(rotary_dim, base=10000.0, scaling=None, device="cuda"):
         ratio, f = (exponent * -2 / rotary_dim).exp(), [num(1)]
         for _ in range(rotary_dim // 2 - 1):
             f.append(f[-1] * ratio)
+        part = 1 / num(s)
         if kind == "linear":
-            f = [x / num(s) for x in f]
+            f = [x * part for x in f]
         elif kind == "ramp":
-            keep = [min(num(1), max(num(0), (num(length) * x / two_pi - num(low)) / (num(high) - num(low)))) for x in f]
-            f = [x * w + x / num(s) * (1 - w) for x, w in zip(f, keep)]
-        turns = [int((x / two_pi % 1 * 2 ** 64).to_integral_value()) % 2 ** 64 for x in f]
-    turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
+            slope, start = num(length) / two_pi / (num(high) - num(low)), num(low) / (num(high) - num(low))
+            keep = [min(num(1), max(num(0), x * slope - start)) for x in f]
+            f = [x * (w + part * (1 - w)) for x, w in zip(f, keep)]
+        unit = 2 ** 64 / two_pi
+        turns = [(round(x * unit) + 2 ** 63) % 2 ** 64 - 2 ** 63 for x in f]
     return RopeTable(torch.tensor(turns, dtype=torch.int64).to(device), rotary_dim, factor)
 
 
