@@ -506,13 +506,22 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             for (int g = 0; g < 4; ++g) tmem_ld32(t_s + g * 32, x[g]);
             tmem_wait_ld();
             if (BIAS) {
-              const float a = -slope2 * float(pos + p.off - j0);
+              // the distance itself runs along the row, exact: with slope2 * position taken out of the product
+              // a bias was off by the rounding of up to 254 slopes, however near its key
+              const uint64_t c2 = f2(p.scale_log2, p.scale_log2), s2 = f2(slope2, slope2), two = f2(2.f, 2.f);
 #pragma unroll
-              for (int g = 0; g < 4; ++g)
+              for (int g = 0; g < 4; ++g) {
+                const int d = j0 + g * 32 - pos - p.off;
+                uint64_t t = f2(float(d), float(d + 1));
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  x[g][e] = __float_as_uint(
-                      fmaf(__uint_as_float(x[g][e]), p.scale_log2, fmaf(slope2, float(g * 32 + e), a)));
+                for (int e = 0; e < 32; e += 2) {
+                  float u, v;
+                  f2_split(f2_fma(t, s2, f2_mul(f2(__uint_as_float(x[g][e]), __uint_as_float(x[g][e + 1])), c2)), u, v);
+                  x[g][e] = __float_as_uint(u);
+                  x[g][e + 1] = __float_as_uint(v);
+                  t = f2_add(t, two);
+                }
+              }
             }
             if (!CAP && __builtin_expect(masked, 0)) {
 #pragma unroll

@@ -134,3 +134,30 @@ def test_a_pair_of_documents_has_two(cuda):
             ab.fused_attn_fwd(q, k, v, documents=docs)
         with pytest.raises(err, match="documents"):
             ab.fused_attn_bwd(do, q, k, v, o, lse, documents=docs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64)])
+@pytest.mark.parametrize("sq", [600, 3])
+@pytest.mark.parametrize("dist", [0, 1, 3, 7, 60, 127, 200])
+def test_a_bias_is_as_exact_as_its_distance(cuda, dist, sq, dtype, d):
+    """Each query sees one key, some positions before it, in its own tile of keys or the one before: lse is
+    that score.  Its dot product is off by up to d half steps of the sum of |q k|; slope * distance is one
+    product, and the change to log2 units and back rounds both a few times (8 half steps)."""
+    skv = 600
+    q, k, v, _ = _inputs(1, 4, 2, sq, skv, d, dtype)
+    slopes = torch.tensor([0.01, 1.0, 30.0, 1000.0], device="cuda")
+    pos = torch.arange(skv, dtype=torch.int32, device="cuda")
+    docs = ((pos[skv - sq:] + 5)[None].contiguous(), (pos + 5 + dist)[None].contiguous())
+    o, lse = ab.fused_attn_fwd(q, k, v, causal=True, slopes=slopes, documents=docs)
+    rows = torch.arange(sq, device="cuda")
+    at = rows + skv - sq - dist          # the key of each row
+    has = at >= 0
+    assert torch.isinf(lse[:, :, ~has]).all()
+    Q, K = q[0][:, has].double(), k[0].repeat_interleave(2, 0)[:, at[has]].double()
+    x = (Q * K).sum(-1) / math.sqrt(d)
+    bias = slopes.double()[:, None] * dist
+    tol = 2.0 ** -24 * ((d + 2) * (Q * K).abs().sum(-1) / math.sqrt(d) + 8 * (x.abs() + bias))
+    err = (lse[0][:, has].double() - (x - bias)).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+    assert torch.equal(o[0, has].transpose(0, 1), v[0].repeat_interleave(2, 0)[:, at[has]])   # its weight is 1
