@@ -142,11 +142,13 @@ enum { ATTN_BWD_DT_BF16 = 0, ATTN_BWD_DT_FP16 = 1, ATTN_BWD_DT_FP32 = 2 };
  *   (a, b) -> factor * (a cos t - b sin t, b cos t + a sin t),   t = 2 pi position * turns / 2^64,
  * pair n being (n, n + rotary_dim/2), or (2n, 2n+1) with `interleaved`; the rest of the head
  * is copied.  `inverse` negates t: with the same factor that is the gradient of the call.
- * turns [rotary_dim/2]: turns[n] is the frequency as a 64-bit fixed-point fraction of a turn (two's complement), so
- * position * turns wraps exactly and far positions lose nothing.  Strides are in elements,
- * in the order batch, head, position; the head's own elements are contiguous.  An output may
- * be its own input (same strides) and else overlaps nothing that the call reads or writes.  position_stride is the positions' batch stride (0: one
- * row for all batches); positions are int64. */
+ * turns [rotary_dim/2]: turns[n] is the frequency as a 64-bit fixed-point fraction of a turn (two's
+ * complement), so position * turns wraps exactly: the angle is off by |position| times what turns[n]
+ * is off (half a unit, 2^-65 turns, where it is the nearest number).  Strides are in elements, in the
+ * order batch, head, position; the head's own elements are contiguous.  An output may be its own input
+ * (same strides) and else overlaps nothing that the call reads or writes.  position_stride is the
+ * positions' batch stride (0: one row for all batches); positions are int64.  head_dim at most 4096,
+ * q_heads and k_heads at most 2^20, seq at most 2^30. */
 typedef struct {
   int bs, seq, q_heads, k_heads, head_dim, rotary_dim; /* q_heads or k_heads may be 0 */
   int dtype;                                           /* ATTN_BWD_DT_* */
@@ -165,8 +167,8 @@ int attn_bwd_b200_rope(const attn_bwd_rope_t* args, const void* q, const void* k
  * j is seen if  (!causal || j < max(i + 1, prefix_lens[b]))  and, with documents,
  * q_documents[b, row] == kv_documents[b, j] >= 0.  A row that sees nothing has output 0, row
  * statistic -inf and gradient 0.  Keys and queries whose document is negative are never read
- * into a result, whatever they hold; a NaN or infinity in another key or value may also reach
- * queries of the same tiles that do not see it.  slopes, prefix_lens and documents may be null;
+ * into a result, whatever they hold; a NaN or infinity in another query, key, value or gradient may
+ * also reach results of the same tiles that do not see it.  There is no dropout of the weights.  slopes, prefix_lens and documents may be null;
  * prefix_lens needs causal; both document arrays or neither (one of no elements may be null).
  *   q [bs, heads, seq_q, head_dim], k and v [bs, kv_heads, seq_kv, head_dim]: strides in
  *     elements in the order batch, head, position (positive multiples of 8, head elements
@@ -198,8 +200,13 @@ int64_t attn_bwd_b200_fused_workspace(const attn_bwd_fused_t* args, int backward
 int attn_bwd_b200_fused_fwd(const attn_bwd_fused_t* args, const void* q, const void* k, const void* v, void* o,
                             float* lse, void* workspace, int64_t workspace_bytes, attn_bwd_stream_t stream);
 
-/* Gradients of the call above, from its o and lse.  Sums over the heads of a group and over
- * rows are taken in a fixed order: equal inputs give equal bits. */
+/* Gradients of the call above, from its o and lse: those of that very call.  (Rows whose keys all lie in
+ * one tile take what o is needed for from their weights, other rows read it, so an o and lse merged
+ * from several calls over parts of the keys give wrong gradients.)  The weights p and ds = p (dp - delta)
+ * tanh' are rounded to the operands' 16 bits before they are multiplied; sums are fp32.  In fp16 a ds
+ * below 6e-8 is lost and one above 65504 infinite, also where dq and dk would be in range: scale the
+ * loss.  Sums over the heads of a group and over rows are taken in a fixed order: equal inputs give
+ * equal bits. */
 int attn_bwd_b200_fused_bwd(const attn_bwd_fused_t* args, const void* grad_o, const void* q, const void* k,
                             const void* v, const void* o, const float* lse, void* dq, void* dk, void* dv,
                             void* workspace, int64_t workspace_bytes, attn_bwd_stream_t stream);

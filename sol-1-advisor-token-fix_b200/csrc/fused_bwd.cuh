@@ -16,8 +16,8 @@
 //
 // What bounds them: neither the tensor cores (active 45 % of the time in dq, 54 % in dkv) nor memory (6 %
 // of its rate), but the chain of a tile: scores, weights, ds, product, with 256 threads to hide
-// its waits.  4096 x 4096, 80 + 8 heads of 128, bf16: 2130 us without a mask (0.81 PFLOP/s by the five
-// products, 1.13 by the seven that are computed), 1030 us causal.  Accumulating dq by atomics
+// its waits.  4096 x 4096, 80 + 8 heads of 128, bf16: 2150 us without a mask (0.80 PFLOP/s by the five
+// products, 1.12 by the seven that are computed), 1030 us causal, in bursts (see fused_fwd.cuh).  Accumulating dq by atomics
 // would save two products, and the order of its sums would change from run to run.
 #pragma once
 #include <type_traits>

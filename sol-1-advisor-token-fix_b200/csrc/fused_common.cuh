@@ -123,7 +123,7 @@ __device__ __forceinline__ DocRange warp_doc_range(const int* ids, int n, uint32
   return r;
 }
 // Ranges of all key tiles, then (sq > 0) of all query tiles, one warp a tile: read once here instead of
-// by every unit that looks at the tile (some 4 us, most of them the launch's).
+// by every unit that looks at the tile (some 3 us, most of them the launch's).
 static __global__ void __launch_bounds__(256) doc_ranges_kernel(const int* __restrict__ kdoc, int skv,
                                                                 const int* __restrict__ qdoc, int sq, int bs,
                                                                 DocRange* __restrict__ kr, DocRange* __restrict__ qr) {
@@ -281,8 +281,8 @@ __device__ __forceinline__ void write_row(const uint32_t (&w)[16], uint8_t* dst,
 
 // The same through the warp's 2 KB of shared memory and one tensor store of 32 rows x 64 bytes (a map
 // with a box of 32 x 32 and the 64-byte swizzle): the warp goes on while the rows leave.  Rows behind
-// the end are cut off by the map.  (Against write_row: 16 documents of 640, causal forward, 203 us
-// instead of 230.)
+// the end are cut off by the map.  (When it took write_row's place: 16 documents of 640, causal forward,
+// 230 -> 203 us.)
 __device__ __forceinline__ void store_rows(uint32_t stage, const CUtensorMap* m, const uint32_t (&w)[16], int c0, int c1,
                                            int c2, int c3, uint32_t lane) {
   if (lane == 0) bulk_wait_read0();   // the store before this one has read the place
@@ -361,7 +361,7 @@ __device__ __forceinline__ void cap_r4(float (&z)[4]) {
 }
 
 // softcap tanh(scale x / softcap) log2(e) of raw scores with |scale x / softcap| <= 0.75: x (c0 + c1
-// x^2 + ..), an odd polynomial fitted to the tanh by Remez exchange (largest relative error 3.3e-8)
+// x^2 + ..), an odd polynomial fitted to the tanh by Remez exchange (largest relative error 3.7e-8)
 // with both scales in its coefficients.  Capped layers rarely come near their cap, and this needs
 // no special function: the warps of a tile whose scores all stay below take it.
 constexpr float kTanhSmall = 0.75f;

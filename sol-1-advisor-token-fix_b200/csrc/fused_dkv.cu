@@ -1,5 +1,5 @@
 // fused_dkv.cu — gradients of keys and values (see fused_bwd.cuh).  8192 packed positions in documents of
-// about 2500, 80 + 8 heads of 128: 831 us; 48 sequences of 640, capped: 1030 us.
+// about 2500, 80 + 8 heads of 128: 878 us; 48 sequences of 640, capped: 1085 us.
 #include "fused_bwd.cuh"
 #include "fused_host.h"
 
@@ -386,7 +386,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap tm_q,    // (d, s, h, b), box (64
 }
 
 // Sums the splits of dk and dv, in order.  D / 4 lanes a row of one of the two.  Bound by its launch (2 x
-// 96 keys of 8 heads: 3.5 us).
+// 96 keys of 8 heads: 5 us).
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) dkv_join_kernel(const BwdParams prm) {
   wait_for_previous();

@@ -1,5 +1,5 @@
 // fused_dq.cu — gradient of the queries (see fused_bwd.cuh).  8192 packed positions in documents of
-// about 2500, 80 + 8 heads of 128: 615 us; 48 sequences of 640, capped: 1340 us (units of three key
+// about 2500, 80 + 8 heads of 128: 653 us; 48 sequences of 640, capped: 1340 us (units of three key
 // tiles, where beginning and ending a unit takes about 4 of its 10 us).
 #include "fused_bwd.cuh"
 #include "fused_host.h"

@@ -18,13 +18,13 @@ static FwdParams plan_fwd(const attn_bwd_fused_t* a, int sm_count) {
   const int ppt = p.G <= TILE ? TILE / p.G : 0;
   const long long packed = ppt ? (long long)p.Hkv * ((p.sq + ppt - 1) / ppt) : whole;
   // Rows of a group share a tile where that takes fewer tiles (one token over 40000 keys, 80 + 8
-  // heads: 50 us, 200 with a tile a head; 77 tokens over 32013 keys: 142 and 175), though the rows
-  // of whole tiles are written faster.
+  // heads: 43 us, 196 with a tile a head; 77 tokens over 32013 keys: 140 and 173, capped in fp16 with 40 + 8
+  // heads 101 and 135), though the rows of whole tiles are written faster.
   f.packed = p.G > 1 && packed < whole;
   f.pos_per_tile = f.packed ? ppt : TILE;
   // two heads of a group have the same keys and the same masks, so a pair of them wastes
-  // nothing at the diagonal (16 documents of 640, causal, 10 heads a group: 204 us, 260 with 256
-  // positions of a head, which is what an odd group takes)
+  // nothing at the diagonal (16 documents of 640, causal, 10 heads a group: 196 us, 252 with 256
+  // positions of a head, which is what an odd group takes; a prompt of 4096: 298 and 307)
   f.pair_heads = !f.packed && p.G % 2 == 0;
   f.head_slots = f.packed ? p.Hkv : f.pair_heads ? p.H / 2 : p.H;
   f.div_slots = fast_div(f.head_slots);
@@ -32,11 +32,11 @@ static FwdParams plan_fwd(const attn_bwd_fused_t* a, int sm_count) {
   f.blocks_q = (p.sq + pos_per_unit - 1) / pos_per_unit;
   p.n_tiles = (p.skv + TILE - 1) / TILE;
   // Two chains in a CTA where a unit's rows fit one tile and there is more than one key tile (4 tokens
-  // over 8191 keys: 32 us, 38 with one chain).
+  // over 8191 keys: 33.6 us, 38.8 with one chain).
   f.duo = p.n_tiles > 1 && !f.pair_heads && f.blocks_q == 1 && p.sq <= f.pos_per_tile;
   const int parts = f.duo ? 2 : 1;
-  // Too few units for the GPU: the keys are split (one token over 40000 keys: 50 us, 292 without; 77
-  // tokens over 32013: 142 and 463), two tiles a split at least (one a split is no faster and
+  // Too few units for the GPU: the keys are split (one token over 40000 keys: 43 us, 287 without; 77
+  // tokens over 32013: 140 and 462), two tiles a split at least (one a split is no faster and
   // leaves more to join), and never more tiles than a unit may have.
   const long long units = (long long)f.blocks_q * f.head_slots * p.bs;
   long long splits = units > 0 ? sm_count / units : 1;

@@ -23,9 +23,10 @@
 //
 // What bounds it: with few rows the keys and values, read once (4 tokens over 8191 keys, 80 + 8 heads of
 // 128: 28 us, 4.8 TB/s); with many, turning scores into weights: 4096 x 4096, 80 + 8 heads of 128, bf16
-// take 560 us without a mask (1.23 PFLOP/s) and 300 us causal (1.15 of what is seen), where the
-// tensor cores are active half of the time and the exponentials' unit as long.  A bias costs 455
-// us, a cap 430 (both causal), since each adds instructions to every score.
+// take 557 us without a mask (1.23 PFLOP/s) and 298 us causal (1.15 of what is seen), where the
+// tensor cores are active half of the time and the exponentials' unit as long.  A bias costs 453
+// us, a cap 432 (both causal), since each adds instructions to every score.  (These are bursts on a
+// cool GPU.  Back to back for longer, the power limit lowers the clock: 608 us without a mask, 345 causal.)
 //
 // Rows of a query tile are 128 positions of one head or, where that needs fewer tiles, up to
 // 128 (position, head) pairs of one group (few positions, as when tokens are generated): a
@@ -710,7 +711,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
 
 // Joins the splits of every row: o = sum_s 2^(lse_s - lse) o_s.  One warp a row; the sum
 // over splits runs in order, so equal inputs give equal bits.  Bound by its launch and the latency of
-// its loads: 4 us for 320 rows of 8 parts, 6 us for 3080 rows of 18.
+// its loads: 6 us for 320 rows of 8 parts, 8 us for 3080 rows of 9.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) fwd_join_kernel(const FwdParams prm) {
   wait_for_previous();

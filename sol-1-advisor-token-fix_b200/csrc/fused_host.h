@@ -126,8 +126,8 @@ inline int prepare_kernel(const void* kern, int smem) {
 }
 
 // A launch; after: behind another kernel of the same call, whose end it may overlap (see
-// wait_for_previous).  One token over 8191 keys for each of 4 sequences: 33.2 us,
-// 35.0 launched the plain way.
+// wait_for_previous).  One token over 8191 keys for each of 4 sequences: 33.6 us,
+// 35.1 launched the plain way; the backward of 2 x 64 x 96: 30.7 and 33.9.
 template <typename... P, typename... A>
 int launch_kernel(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream_t s, bool after, const A&... args) {
   cudaLaunchConfig_t cfg = {};

@@ -3,7 +3,8 @@
 // (a, b) -> factor * (a cos t - b sin t, b cos t + a sin t) for every pair of a head's first
 // rotary_dim elements, t = 2 pi * position * f.  The frequency f comes as a 64-bit fixed-point
 // fraction of a turn F = round(f * 2^64): position * F mod 2^64 is the fraction of a turn of
-// the angle with an error of position / 2 * 2^-64, where an fp32 angle would already be off by
+// the angle with an error of |position| / 2 * 2^-64 (the table is made in decimal arithmetic, so that F is
+// the nearest number), where an fp32 angle would already be off by
 // position * 2^-24 radians (0.06 at position 10^6).  The top 32 bits, read as a signed
 // number, are the angle in half-open [-1/2, 1/2) turns; rounding them to fp32 costs 2^-24
 // relative, like any fp32 cosine's own rounding.
@@ -12,8 +13,8 @@
 // once per token and pair into shared memory and shared by all heads of the token; a thread
 // then moves 16 bytes of each half of a pair at a time (8 bytes, or single elements, where
 // sizes or strides leave no more).  Full occupancy hides the latency: 2 x 16001 tokens, 80 + 8
-// heads of 128, bf16: 238 us (6.07 TB/s); 6 blocks an SM 264 us, 4 blocks 315; two rows in flight
-// a thread (48 registers) 266, four 410.
+// heads of 128, bf16: 236 us (6.11 TB/s; in fp32 432 us, 6.67 TB/s, neighbouring pairs 446); 6 blocks an SM
+// 264 us, 4 blocks 315; two rows in flight a thread (48 registers) 266, four 410.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -151,7 +152,8 @@ cudaError_t launch_width(RopeParams p, int dim, bool inter, cudaStream_t stream)
   p.pair_chunks = inter && VEC > 1 ? p.rotary_dim / VEC : p.half / VEC;
   p.chunks = p.pair_chunks + (dim - p.rotary_dim) / VEC;
   // A block's rows keep its threads busy for a few rounds; at most 16 KB of angles.  2 x 16001 tokens, 88
-  // heads: 238 us; 248 with 96 rows a block, 247 with 720.  12 x 467 tokens: 53; 59 from 360 rows on.
+  // heads: 238 us; 248 with 96 rows a block, 247 with 720.  12 x 467 tokens: 53; 59 from 360 rows on.  (A few
+  // tokens fill few blocks, whose threads take up to six rounds: 8 tokens of 88 heads are 4 blocks.)
   int tpb = 192 / p.heads;
   if (tpb > kMaxTokens) tpb = kMaxTokens;
   if ((long long)tpb * p.half * 8 > 16384) tpb = 16384 / (p.half * 8);
