@@ -168,8 +168,9 @@ int attn_bwd_b200_rope(const attn_bwd_rope_t* args, const void* q, const void* k
  * q_documents[b, row] == kv_documents[b, j] >= 0.  A row that sees nothing has output 0, row
  * statistic -inf and gradient 0.  Keys and queries whose document is negative are never read
  * into a result, whatever they hold; a NaN or infinity in another query, key, value or gradient may
- * also reach results of the same tiles that do not see it.  There is no dropout of the weights.  slopes, prefix_lens and documents may be null;
- * prefix_lens needs causal; both document arrays or neither (one of no elements may be null).
+ * also reach results of the same tiles that do not see it.  There is no dropout of the weights.
+ * slopes, prefix_lens and documents may be null; prefix_lens needs causal; both document arrays or
+ * neither (one of no elements may be null).
  *   q [bs, heads, seq_q, head_dim], k and v [bs, kv_heads, seq_kv, head_dim]: strides in
  *     elements in the order batch, head, position (positive multiples of 8, head elements
  *     contiguous, 16-byte aligned), heads a multiple of kv_heads, head_dim 64 or 128; bs and
