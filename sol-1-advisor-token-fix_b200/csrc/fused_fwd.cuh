@@ -507,8 +507,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q,   // (d, h, s, b), box (64,
             for (int g = 0; g < 4; ++g) tmem_ld32(t_s + g * 32, x[g]);
             tmem_wait_ld();
             if (BIAS) {
-              // the distance itself runs along the row (exact below 2^24 positions): with slope2 * position taken out of the product
-              // a bias was off by the rounding of up to 254 slopes, however near its key
+              // the distance itself runs along the row (exact below 2^24 positions): with slope2 * position
+              // taken out of the product a bias was off by the rounding of up to 254 slopes, however near its key
               const uint64_t c2 = f2(p.scale_log2, p.scale_log2), s2 = f2(slope2, slope2), two = f2(2.f, 2.f);
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
